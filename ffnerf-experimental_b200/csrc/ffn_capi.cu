@@ -9,6 +9,7 @@
 #include <string>
 
 #include "ffn_common.cuh"
+#include "ffn_ops.cuh"
 #include "ffn_step.cu"
 #include "ffn_step_tc.cu"
 #include "ffn_dp.cu"
@@ -308,6 +309,9 @@ int mlp_bench(ffn_ctx* c, const void* tiles, int64_t n, void* stream) {
 }
 
 }  // namespace
+
+// The block operators' translation units report through the same message.
+int ffn::op_fail(int code, const std::string& msg) { return fail(nullptr, code, msg); }
 
 extern "C" {
 

@@ -1,0 +1,491 @@
+// ffn_norm.cu -- root-mean-square norm of a residual stream, forward (output in the input's type or in
+// e4m3 with fp32 scales) and backward.  A translation unit of its own.
+//
+//   h = x + r,  s = 1 / sqrt(mean(h^2) + eps),  y = h s g          (mean and sums over a row's d columns)
+//   backward, with xhat = h s and u = dy g:
+//   dx = s (u - xhat mean(u xhat)) + dr,   dg = sum over rows of dy xhat
+//
+// x and r enter once, so dx is the gradient of both.  dr is the gradient that reaches h along the
+// residual stream itself.
+//
+// Both passes read each element once and write each result once, a few operations per element: HBM
+// is the bound.  A row therefore stays in the registers of the threads that loaded it: `tpr` lanes of
+// a warp where the row has at most 32 lanes x NV vectors of 16 bytes (so a 64-wide row takes 8 lanes
+// and a warp takes four rows; no barrier), a whole block above that.  Statistics are fp32.  y is
+// formed from the unrounded fp32 sum x + r; the h that is written for the residual stream and for the
+// backward pass is rounded to the stream's type.
+#include "ffn_ops.cuh"
+
+namespace ffn {
+namespace {
+
+struct NormArgs {
+    const void* x; const void* res; const float* gamma;
+    void* h; void* y; float* scale; float* rstd;
+    int64_t n, x_ld, res_ld;
+    int d, group, tpr;
+    float eps;
+};
+
+struct NormBwdArgs {
+    const void* dy; const void* h; const void* dres; const float* gamma; const float* rstd;
+    void* dx; float* partial;
+    int64_t n, dy_ld, h_ld, dres_ld;
+    int d, tpr;
+};
+
+// Sum (or NaN-keeping maximum) over the threads of one row: `tpr` lanes, or the block (BLOCK).  In a
+// block the warps' values are added in warp order, so a row's result does not depend on timing.
+template <bool BLOCK, bool MAX>
+__device__ __forceinline__ float row_reduce(float v, int tpr, float* sh) {
+    for (int o = (BLOCK ? 32 : tpr) >> 1; o > 0; o >>= 1) {
+        const float w = __shfl_xor_sync(0xffffffffu, v, o);
+        v = MAX ? max_nan(v, w) : v + w;
+    }
+    if constexpr (BLOCK) {
+        const int warps = blockDim.x >> 5;
+        __syncthreads();                       // the previous use of sh is over
+        if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = sh[0];
+        for (int w = 1; w < warps; ++w) v = MAX ? max_nan(v, sh[w]) : v + sh[w];
+    }
+    return v;
+}
+
+// NV vectors of VEC elements per thread: vector i of a thread starts at column (lane + i * threads) * VEC.
+template <typename T, bool OUT8, int VEC, int NV, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? 512 : 256) rmsnorm_kernel(const NormArgs a) {
+    __shared__ float sh[32];
+    const int tpr = BLOCK ? (int)blockDim.x : a.tpr;
+    const int lane = threadIdx.x & (tpr - 1);
+    const int rows = BLOCK ? 1 : (int)blockDim.x / tpr;          // rows of a block at a time
+    const int sub = BLOCK ? 0 : (int)threadIdx.x / tpr;
+    const float inv_d = 1.0f / (float)a.d;
+    const T* x = static_cast<const T*>(a.x);
+    const T* res = static_cast<const T*>(a.res);
+    for (int64_t base = (int64_t)blockIdx.x * rows; base < a.n; base += (int64_t)gridDim.x * rows) {
+        const int64_t row = base + sub;
+        const bool live = row < a.n;
+        float v[NV][VEC];
+        float ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (lane + i * tpr) * VEC;
+            const bool on = live && c < a.d;
+            Pack<T, VEC> p{}, q{};
+            if (on) {
+                p = load_pack<T, VEC>(x + row * a.x_ld + c);
+                if (res) q = load_pack<T, VEC>(res + row * a.res_ld + c);
+            }
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[i][j] = on ? to_f(p.v[j]) + (res ? to_f(q.v[j]) : 0.0f) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) ss = fmaf(v[i][j], v[i][j], ss);
+        ss = row_reduce<BLOCK, false>(ss, tpr, sh);
+        const float s = rsqrtf(fmaf(ss, inv_d, a.eps));
+        if (a.rstd && live && lane == 0) a.rstd[row] = s;
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (lane + i * tpr) * VEC;
+            if (live && c < a.d) {
+                if (a.h) {
+                    Pack<T, VEC> p;
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) p.v[j] = from_f<T>(v[i][j]);
+                    store_pack<T, VEC>(static_cast<T*>(a.h) + row * a.d + c, p);
+                }
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    v[i][j] = v[i][j] * s * __ldg(a.gamma + c + j);
+                    if constexpr (OUT8) top = max_nan(top, fabsf(v[i][j]));
+                }
+                if constexpr (!OUT8) {
+                    Pack<T, VEC> p;
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) p.v[j] = from_f<T>(v[i][j]);
+                    store_pack<T, VEC>(static_cast<T*>(a.y) + row * a.d + c, p);
+                }
+            }
+        }
+        if constexpr (OUT8) {
+            float sc = 1.0f;
+            if (!a.group) {
+                top = row_reduce<BLOCK, true>(top, tpr, sh);
+                sc = e4m3_scale(top);
+                if (live && lane == 0) a.scale[row] = sc;
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = (lane + i * tpr) * VEC;
+                const bool on = live && c < a.d;
+                if (a.group) {   // group / VEC neighbouring lanes hold one group's columns
+                    float m = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) m = max_nan(m, on ? fabsf(v[i][j]) : 0.0f);
+                    for (int o = a.group / VEC / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+                    sc = e4m3_scale(m);
+                    if (on && c % a.group == 0) a.scale[row * (a.d / a.group) + c / a.group] = sc;
+                }
+                if (on) {
+                    const float inv = e4m3_inverse(sc);
+                    uint8_t* q = static_cast<uint8_t*>(a.y) + row * a.d + c;
+                    if constexpr (VEC == 8) {
+                        *reinterpret_cast<uint2*>(q) =
+                            make_uint2(pack_e4m3x4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv),
+                                       pack_e4m3x4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv));
+                    } else if constexpr (VEC == 4) {
+                        *reinterpret_cast<uint32_t*>(q) =
+                            pack_e4m3x4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j)
+                            q[j] = (uint8_t)__nv_cvt_float_to_fp8(v[i][j] * inv, __NV_SATFINITE, __NV_E4M3);
+                    }
+                }
+            }
+        }
+    }
+}
+
+// Rows that do not fit a block's registers, and grouped scales on rows that cannot be read in
+// 16-byte vectors: one block per row, which reads the row again (from L2) for each pass over it.
+template <typename T, bool OUT8>
+__global__ void __launch_bounds__(256) rmsnorm_long_kernel(const NormArgs a) {
+    __shared__ float sh[32];
+    const float inv_d = 1.0f / (float)a.d;
+    for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
+        const T* x = static_cast<const T*>(a.x) + row * a.x_ld;
+        const T* res = a.res ? static_cast<const T*>(a.res) + row * a.res_ld : nullptr;
+        auto at = [&](int c) { return to_f(x[c]) + (res ? to_f(res[c]) : 0.0f); };
+        float ss = 0.0f;
+        for (int c = threadIdx.x; c < a.d; c += blockDim.x) { const float v = at(c); ss = fmaf(v, v, ss); }
+        ss = row_reduce<true, false>(ss, 0, sh);
+        const float s = rsqrtf(fmaf(ss, inv_d, a.eps));
+        if (a.rstd && threadIdx.x == 0) a.rstd[row] = s;
+        if constexpr (!OUT8) {
+            for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
+                const float v = at(c);
+                static_cast<T*>(a.y)[row * a.d + c] = from_f<T>(v * s * a.gamma[c]);
+                if (a.h) static_cast<T*>(a.h)[row * a.d + c] = from_f<T>(v);
+            }
+        } else {
+            // a warp per group, or the block for the whole row
+            const int width = a.group ? a.group : a.d;
+            const int step = a.group ? 32 : (int)blockDim.x, lane = a.group ? (int)threadIdx.x & 31 : (int)threadIdx.x;
+            for (int g = a.group ? (int)threadIdx.x >> 5 : 0; g < a.d / width; g += a.group ? (int)blockDim.x >> 5 : 1) {
+                float top = 0.0f;
+                for (int c = g * width + lane; c < (g + 1) * width; c += step)
+                    top = max_nan(top, fabsf(at(c) * s * a.gamma[c]));
+                top = a.group ? row_reduce<false, true>(top, 32, sh) : row_reduce<true, true>(top, 0, sh);
+                const float sc = e4m3_scale(top), inv = e4m3_inverse(sc);
+                if (lane == 0) a.scale[row * (a.d / width) + g] = sc;
+                for (int c = g * width + lane; c < (g + 1) * width; c += step) {
+                    const float v = at(c);
+                    static_cast<uint8_t*>(a.y)[row * a.d + c] =
+                        (uint8_t)__nv_cvt_float_to_fp8(v * s * a.gamma[c] * inv, __NV_SATFINITE, __NV_E4M3);
+                    if (a.h) static_cast<T*>(a.h)[row * a.d + c] = from_f<T>(v);
+                }
+            }
+        }
+    }
+}
+
+// Backward.  Each thread keeps the sums of dy xhat of its columns over all the rows that it meets;
+// a block adds its own and writes one row of `partial`, which norm_dgamma_kernel sums in block order.
+// The gradient of gamma is therefore the same on every run.
+template <typename T, int VEC, int NV, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? 512 : 256) rmsnorm_bwd_kernel(const NormBwdArgs a) {
+    extern __shared__ float dyn[];                               // [warps][d] (not BLOCK)
+    __shared__ float sh[32];
+    const int tpr = BLOCK ? (int)blockDim.x : a.tpr;
+    const int lane = threadIdx.x & (tpr - 1);
+    const int rows = BLOCK ? 1 : (int)blockDim.x / tpr;
+    const int sub = BLOCK ? 0 : (int)threadIdx.x / tpr;
+    const float inv_d = 1.0f / (float)a.d;
+    const T* dyp = static_cast<const T*>(a.dy);
+    const T* hp = static_cast<const T*>(a.h);
+    const T* drp = static_cast<const T*>(a.dres);
+    float dg[NV][VEC];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) dg[i][j] = 0.0f;
+    for (int64_t base = (int64_t)blockIdx.x * rows; base < a.n; base += (int64_t)gridDim.x * rows) {
+        const int64_t row = base + sub;
+        const bool live = row < a.n;
+        const float s = live ? __ldg(a.rstd + row) : 0.0f;
+        Pack<T, VEC> pd[NV], ph[NV], pr[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (lane + i * tpr) * VEC;
+            pd[i] = Pack<T, VEC>{}; ph[i] = Pack<T, VEC>{}; pr[i] = Pack<T, VEC>{};
+            if (live && c < a.d) {
+                pd[i] = load_pack<T, VEC>(dyp + row * a.dy_ld + c);
+                ph[i] = load_pack<T, VEC>(hp + row * a.h_ld + c);
+                if (drp) pr[i] = load_pack<T, VEC>(drp + row * a.dres_ld + c);
+            }
+        }
+        float dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (lane + i * tpr) * VEC;
+            if (live && c < a.d)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float xh = to_f(ph[i].v[j]) * s, dy = to_f(pd[i].v[j]);
+                    dg[i][j] = fmaf(dy, xh, dg[i][j]);
+                    dot = fmaf(dy * __ldg(a.gamma + c + j), xh, dot);
+                }
+        }
+        dot = row_reduce<BLOCK, false>(dot, tpr, sh) * inv_d;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (lane + i * tpr) * VEC;
+            if (live && c < a.d) {
+                Pack<T, VEC> p;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float xh = to_f(ph[i].v[j]) * s, u = to_f(pd[i].v[j]) * __ldg(a.gamma + c + j);
+                    p.v[j] = from_f<T>(fmaf(s, fmaf(-xh, dot, u), drp ? to_f(pr[i].v[j]) : 0.0f));
+                }
+                store_pack<T, VEC>(static_cast<T*>(a.dx) + row * a.d + c, p);
+            }
+        }
+    }
+    float* out = a.partial + (int64_t)blockIdx.x * a.d;
+    if constexpr (BLOCK) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const int c = (lane + i * tpr) * VEC + j;
+                if (c < a.d) out[c] = dg[i][j];
+            }
+    } else {
+        const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                float v = dg[i][j];
+                for (int o = tpr; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);   // the warp's rows
+                const int c = (lane + i * tpr) * VEC + j;
+                if ((threadIdx.x & 31) < tpr && c < a.d) dyn[warp * a.d + c] = v;
+            }
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
+            float v = 0.0f;
+            for (int w = 0; w < warps; ++w) v += dyn[w * a.d + c];
+            out[c] = v;
+        }
+    }
+}
+
+// Backward of rows beyond a block's registers: dx as above; the sums of dy xhat go to this block's
+// row of `partial` directly (the same thread meets the same columns in every row).
+template <typename T>
+__global__ void __launch_bounds__(256) rmsnorm_bwd_long_kernel(const NormBwdArgs a) {
+    __shared__ float sh[32];
+    const float inv_d = 1.0f / (float)a.d;
+    float* out = a.partial + (int64_t)blockIdx.x * a.d;
+    for (int c = threadIdx.x; c < a.d; c += blockDim.x) out[c] = 0.0f;
+    for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
+        const T* dy = static_cast<const T*>(a.dy) + row * a.dy_ld;
+        const T* h = static_cast<const T*>(a.h) + row * a.h_ld;
+        const T* dr = a.dres ? static_cast<const T*>(a.dres) + row * a.dres_ld : nullptr;
+        const float s = a.rstd[row];
+        float dot = 0.0f;
+        for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
+            const float t = to_f(dy[c]) * (to_f(h[c]) * s);
+            out[c] += t;
+            dot = fmaf(t, a.gamma[c], dot);
+        }
+        dot = row_reduce<true, false>(dot, 0, sh) * inv_d;
+        for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
+            const float u = to_f(dy[c]) * a.gamma[c], xh = to_f(h[c]) * s;
+            static_cast<T*>(a.dx)[row * a.d + c] = from_f<T>(fmaf(s, fmaf(-xh, dot, u), dr ? to_f(dr[c]) : 0.0f));
+        }
+    }
+}
+
+// dgamma[c] = sum over blocks of partial[block][c]: 32 columns x 32 slices of the blocks per block,
+// each slice summed in order, then the slices in order.
+__global__ void __launch_bounds__(1024) norm_dgamma_kernel(const float* __restrict__ partial, float* __restrict__ dgamma,
+                                                           int blocks, int d) {
+    __shared__ float sh[32][33];
+    const int c = blockIdx.x * 32 + threadIdx.x;
+    float v = 0.0f;
+    if (c < d)
+        for (int b = threadIdx.y; b < blocks; b += 32) v += partial[(int64_t)b * d + c];
+    sh[threadIdx.y][threadIdx.x] = v;
+    __syncthreads();
+    if (threadIdx.y == 0 && c < d) {
+        float s = 0.0f;
+        for (int i = 0; i < 32; ++i) s += sh[i][threadIdx.x];
+        dgamma[c] = s;
+    }
+}
+
+// How a row is laid over threads.
+struct Shape { int vec, nv, threads, tpr; bool block, loop; };
+
+Shape norm_shape(int d, int full_vec, bool aligned, int group) {
+    Shape s{};
+    s.vec = aligned ? full_vec : 1;
+    const int vectors = (d + s.vec - 1) / s.vec;
+    const int most = s.vec == 1 ? 8 : 4;                 // vectors (or elements) of a thread
+    s.threads = 256;
+    if (vectors <= 32 * most) {
+        s.tpr = 1;
+        while (s.tpr < 32 && s.tpr < vectors) s.tpr *= 2;
+        s.nv = (vectors + s.tpr - 1) / s.tpr;
+    } else if (vectors <= 512 * most) {
+        s.block = true;
+        s.threads = 64;
+        while (s.threads * most < vectors) s.threads *= 2;
+        s.nv = (vectors + s.threads - 1) / s.threads;
+    } else {
+        s.loop = true;
+    }
+    if (s.vec == 1) s.nv = 8;
+    else if (s.nv == 3) s.nv = 4;
+    if (s.vec == 1 && group) s.loop = true;
+    return s;
+}
+
+int norm_grid(const Shape& s, int64_t n, int sms) {
+    const int64_t rows = s.block || s.loop ? 1 : s.threads / s.tpr;
+    const int64_t want = (n + rows - 1) / rows;
+    const int64_t most = (int64_t)sms * (2048 / s.threads);
+    return (int)(want < most ? want : most);
+}
+
+template <typename T, bool OUT8>
+int norm_launch(const NormArgs& a0, bool aligned, cudaStream_t st) {
+    NormArgs a = a0;
+    constexpr int VEC = 16 / sizeof(T);
+    const Shape s = norm_shape(a.d, VEC, aligned, a.group);
+    const int sms = op_sms();
+    if (sms <= 0) return op_fail(FFN_E_CUDA, "no CUDA device");
+    a.tpr = s.tpr;
+    const int grid = norm_grid(s, a.n, sms);
+    if (s.loop) rmsnorm_long_kernel<T, OUT8><<<grid, 256, 0, st>>>(a);
+    else if (s.vec == 1) {
+        if (s.block) rmsnorm_kernel<T, OUT8, 1, 8, true><<<grid, s.threads, 0, st>>>(a);
+        else rmsnorm_kernel<T, OUT8, 1, 8, false><<<grid, s.threads, 0, st>>>(a);
+    } else if (s.block) {
+        if (s.nv == 1) rmsnorm_kernel<T, OUT8, VEC, 1, true><<<grid, s.threads, 0, st>>>(a);
+        else if (s.nv == 2) rmsnorm_kernel<T, OUT8, VEC, 2, true><<<grid, s.threads, 0, st>>>(a);
+        else rmsnorm_kernel<T, OUT8, VEC, 4, true><<<grid, s.threads, 0, st>>>(a);
+    } else {
+        if (s.nv == 1) rmsnorm_kernel<T, OUT8, VEC, 1, false><<<grid, s.threads, 0, st>>>(a);
+        else if (s.nv == 2) rmsnorm_kernel<T, OUT8, VEC, 2, false><<<grid, s.threads, 0, st>>>(a);
+        else rmsnorm_kernel<T, OUT8, VEC, 4, false><<<grid, s.threads, 0, st>>>(a);
+    }
+    return op_launched("ffn_rmsnorm");
+}
+
+constexpr int BWD_BLOCKS_PER_SM = 4;   // rows of partial sums: bounded, they are written and read again
+
+template <typename T>
+int norm_bwd_launch(const NormBwdArgs& a0, float* dgamma, bool aligned, cudaStream_t st) {
+    NormBwdArgs a = a0;
+    constexpr int VEC = 16 / sizeof(T);
+    const Shape s = norm_shape(a.d, VEC, aligned, 0);
+    const int sms = op_sms();
+    if (sms <= 0) return op_fail(FFN_E_CUDA, "no CUDA device");
+    a.tpr = s.tpr;
+    int grid = norm_grid(s, a.n, sms);
+    grid = grid < sms * BWD_BLOCKS_PER_SM ? grid : sms * BWD_BLOCKS_PER_SM;
+    const size_t sm = (size_t)(s.threads / 32) * a.d * sizeof(float);   // at most 8 x 1024 floats
+    if (s.loop) rmsnorm_bwd_long_kernel<T><<<grid, 256, 0, st>>>(a);
+    else if (s.vec == 1) {
+        if (s.block) rmsnorm_bwd_kernel<T, 1, 8, true><<<grid, s.threads, 0, st>>>(a);
+        else rmsnorm_bwd_kernel<T, 1, 8, false><<<grid, s.threads, sm, st>>>(a);
+    } else if (s.block) {
+        if (s.nv == 1) rmsnorm_bwd_kernel<T, VEC, 1, true><<<grid, s.threads, 0, st>>>(a);
+        else if (s.nv == 2) rmsnorm_bwd_kernel<T, VEC, 2, true><<<grid, s.threads, 0, st>>>(a);
+        else rmsnorm_bwd_kernel<T, VEC, 4, true><<<grid, s.threads, 0, st>>>(a);
+    } else {
+        if (s.nv == 1) rmsnorm_bwd_kernel<T, VEC, 1, false><<<grid, s.threads, sm, st>>>(a);
+        else if (s.nv == 2) rmsnorm_bwd_kernel<T, VEC, 2, false><<<grid, s.threads, sm, st>>>(a);
+        else rmsnorm_bwd_kernel<T, VEC, 4, false><<<grid, s.threads, sm, st>>>(a);
+    }
+    if (int rc = op_launched("ffn_rmsnorm_bwd")) return rc;
+    norm_dgamma_kernel<<<(a.d + 31) / 32, dim3(32, 32), 0, st>>>(a.partial, dgamma, grid, a.d);
+    return op_launched("ffn_rmsnorm_bwd gamma");
+}
+
+}  // namespace
+}  // namespace ffn
+
+using namespace ffn;
+
+extern "C" {
+
+int ffn_rmsnorm(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, const float* gamma, void* h,
+                void* y, float* scale, float* rstd, int64_t n, int32_t d, float eps, int dtype, int out_dtype,
+                int32_t group, void* stream) {
+    if (n < 0 || d < 1) return op_fail(FFN_E_CONFIG, "ffn_rmsnorm: n must be >= 0 and d >= 1");
+    if (dtype != FFN_F32 && dtype != FFN_F16 && dtype != FFN_BF16)
+        return op_fail(FFN_E_CONFIG, "ffn_rmsnorm: dtype must be FFN_F32, FFN_F16 or FFN_BF16");
+    const bool out8 = out_dtype == FFN_E4M3;
+    if (!out8 && out_dtype != dtype) return op_fail(FFN_E_CONFIG, "ffn_rmsnorm: out_dtype must be dtype or FFN_E4M3");
+    if (group != 0 && (!out8 || (group != 32 && group != 64 && group != 128) || d % group))
+        return op_fail(FFN_E_CONFIG, "ffn_rmsnorm: group must be 0, 32, 64 or 128, divide d, and needs an e4m3 output");
+    if (!(eps >= 0.0f)) return op_fail(FFN_E_CONFIG, "ffn_rmsnorm: eps must be >= 0");
+    if (n == 0) return FFN_OK;
+    if (!x || !gamma || !y || (out8 && !scale)) return op_fail(FFN_E_CONFIG, "ffn_rmsnorm: a required pointer is NULL");
+    if (x_ld < d || (residual && residual_ld < d)) return op_fail(FFN_E_CONFIG, "ffn_rmsnorm: a row stride is below d");
+    const size_t z = dtype == FFN_F32 ? 4 : 2;
+    const int vec = (int)(16 / z);
+    const bool aligned = d % vec == 0 && x_ld % vec == 0 && (!residual || residual_ld % vec == 0) && op_aligned(x, 16) &&
+                         op_aligned(residual, 16) && op_aligned(h, 16) && op_aligned(y, out8 ? vec : 16);
+    NormArgs a{x, residual, gamma, h, y, scale, rstd, n, x_ld, residual_ld, d, group, 0, eps};
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == FFN_F32) return out8 ? norm_launch<float, true>(a, aligned, st) : norm_launch<float, false>(a, aligned, st);
+    if (dtype == FFN_F16) return out8 ? norm_launch<__half, true>(a, aligned, st) : norm_launch<__half, false>(a, aligned, st);
+    return out8 ? norm_launch<__nv_bfloat16, true>(a, aligned, st) : norm_launch<__nv_bfloat16, false>(a, aligned, st);
+}
+
+uint64_t ffn_rmsnorm_bwd_workspace(int64_t n, int32_t d) {
+    if (n < 0 || d < 1) return 0;
+    const int sms = op_sms();
+    if (sms <= 0) return 0;
+    const int64_t most = (int64_t)sms * BWD_BLOCKS_PER_SM;
+    return (uint64_t)(n < most ? n : most) * (uint64_t)d * sizeof(float);
+}
+
+int ffn_rmsnorm_bwd(const void* dy, int64_t dy_ld, const void* h, int64_t h_ld, const float* gamma, const float* rstd,
+                    const void* dresidual, int64_t dresidual_ld, void* dx, float* dgamma, void* workspace,
+                    uint64_t workspace_bytes, int64_t n, int32_t d, int dtype, void* stream) {
+    if (n < 0 || d < 1) return op_fail(FFN_E_CONFIG, "ffn_rmsnorm_bwd: n must be >= 0 and d >= 1");
+    if (dtype != FFN_F32 && dtype != FFN_F16 && dtype != FFN_BF16)
+        return op_fail(FFN_E_CONFIG, "ffn_rmsnorm_bwd: dtype must be FFN_F32, FFN_F16 or FFN_BF16");
+    if (!dgamma) return op_fail(FFN_E_CONFIG, "ffn_rmsnorm_bwd: a required pointer is NULL");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (n == 0) {
+        const cudaError_t e = cudaMemsetAsync(dgamma, 0, (size_t)d * sizeof(float), st);
+        return e == cudaSuccess ? FFN_OK : op_fail(FFN_E_CUDA, std::string("ffn_rmsnorm_bwd: ") + cudaGetErrorString(e));
+    }
+    if (!dy || !h || !gamma || !rstd || !dx || !workspace)
+        return op_fail(FFN_E_CONFIG, "ffn_rmsnorm_bwd: a required pointer is NULL");
+    if (dy_ld < d || h_ld < d || (dresidual && dresidual_ld < d))
+        return op_fail(FFN_E_CONFIG, "ffn_rmsnorm_bwd: a row stride is below d");
+    if (workspace_bytes < ffn_rmsnorm_bwd_workspace(n, d) || !op_aligned(workspace, 4))
+        return op_fail(FFN_E_CAPACITY, "ffn_rmsnorm_bwd: the workspace is smaller than ffn_rmsnorm_bwd_workspace says");
+    const int vec = dtype == FFN_F32 ? 4 : 8;
+    const bool aligned = d % vec == 0 && dy_ld % vec == 0 && h_ld % vec == 0 && (!dresidual || dresidual_ld % vec == 0) &&
+                         op_aligned(dy, 16) && op_aligned(h, 16) && op_aligned(dresidual, 16) && op_aligned(dx, 16);
+    NormBwdArgs a{dy, h, dresidual, gamma, rstd, dx, static_cast<float*>(workspace), n, dy_ld, h_ld, dresidual_ld, d, 0};
+    if (dtype == FFN_F32) return norm_bwd_launch<float>(a, dgamma, aligned, st);
+    if (dtype == FFN_F16) return norm_bwd_launch<__half>(a, dgamma, aligned, st);
+    return norm_bwd_launch<__nv_bfloat16>(a, dgamma, aligned, st);
+}
+
+}  // extern "C"

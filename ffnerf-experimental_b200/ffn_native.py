@@ -47,7 +47,7 @@ STEP_TABLE_IMMEDIATE = 1
 STEP_TABLE_APPLIED = 2
 STATUS_NONFINITE, STATUS_TC_TIMEOUT, STATUS_DP_TIMEOUT = 1, 4, 8   # ffn_status bits
 STAGE_SAMPLES = 1 << 20   # samples per group of the split tensor-core step (ffn_capi.cu)
-ABI_VERSION = 6          # include/ffnerf.h FFN_ABI_VERSION
+ABI_VERSION = 7          # include/ffnerf.h FFN_ABI_VERSION
 
 
 _VP = C.c_void_p
@@ -90,6 +90,22 @@ _SIGS = {
     "ffn_camera_rays": (C.c_int, [_VP, _VP, C.c_int, C.c_int, C.c_uint32, C.c_uint32, _VP, _VP]),
     "ffn_batch_feedback": (C.c_int, [_VP, _VP, C.c_int, C.c_int, C.c_int, C.c_int, _VP, _VP, _VP, _VP, C.c_uint32,
                                      _VP, C.c_double, C.c_int, C.c_int, _VP]),
+    "ffn_rmsnorm": (C.c_int, [_VP, C.c_int64, _VP, C.c_int64] + [_VP] * 5 + [C.c_int64, C.c_int32, C.c_float, C.c_int,
+                              C.c_int, C.c_int32, _VP]),
+    "ffn_rmsnorm_bwd_workspace": (C.c_uint64, [C.c_int64, C.c_int32]),
+    "ffn_rmsnorm_bwd": (C.c_int, [_VP, C.c_int64, _VP, C.c_int64, _VP, _VP, _VP, C.c_int64, _VP, _VP, _VP, C.c_uint64,
+                                  C.c_int64, C.c_int32, C.c_int, _VP]),
+    "ffn_gated_scan": (C.c_int, [_VP, C.c_int64, _VP, C.c_int64, _VP, _VP, _VP, _VP, C.c_int64, C.c_int32, C.c_int64,
+                                 C.c_int32, C.c_int, C.c_int, C.c_int, _VP]),
+    "ffn_gated_scan_bwd": (C.c_int, [_VP, C.c_int64, _VP, _VP, C.c_int64, _VP, C.c_int64, _VP, C.c_int64] + [_VP] * 5
+                           + [C.c_int64, C.c_int32, C.c_int64, C.c_int32, C.c_int, C.c_int, C.c_int, _VP]),
+    "ffn_expert_mm_workspace": (C.c_uint64, [_VP, C.c_int64, _VP, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int]),
+    "ffn_expert_mm": (C.c_int, [_VP, C.c_int64] + [_VP] * 5 + [C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int,
+                                C.c_int, _VP, C.c_uint64, _VP]),
+    "ffn_expert_mm_bwd_workspace": (C.c_uint64, [_VP, C.c_int64, _VP, C.c_int64, _VP, C.c_int64, C.c_int32, C.c_int32,
+                                                 C.c_int32, C.c_int]),
+    "ffn_expert_mm_bwd": (C.c_int, [_VP, C.c_int64, _VP, C.c_int64] + [_VP] * 4 + [C.c_int64, C.c_int32, C.c_int32,
+                                    C.c_int32, C.c_int, C.c_int, _VP, C.c_uint64, _VP]),
 }
 EXPORTED = tuple(_SIGS)
 

@@ -38,10 +38,11 @@ extern "C" {
 #endif
 
 #define FFN_N_LEVELS 16
-#define FFN_ABI_VERSION 6   /* 2: ffn_step_scalars.flags; 3: batch/exchange entry points;
+#define FFN_ABI_VERSION 7   /* 2: ffn_step_scalars.flags; 3: batch/exchange entry points;
                                    4: fp16-table hash and MLP microbenchmark entry points;
                                    5: ffn_dp_set_wait_limit, ffn_config.transfer_fmt,
-                                      ffn_probe_random_access; 6: ffn_mlp_bench_f16 */
+                                      ffn_probe_random_access; 6: ffn_mlp_bench_f16; 7: ffn_rmsnorm,
+                                      ffn_gated_scan, ffn_expert_mm and their backward passes */
 
 enum {
     FFN_OK = 0,
@@ -288,6 +289,79 @@ int ffn_forward_backward_noalloc(const ffn_config* cfg, const float* params, flo
                                  const uint32_t* occ_in, uint32_t* occ_st, const void* rays,
                                  const void* targets, void* out, float* grads, int* status,
                                  uint32_t n_rays, const ffn_step_scalars* s, void* stream);
+
+/* ---- Block operators (no reference counterpart): what a residual block over per-sample features
+ * is made of -- a norm of the residual stream, a gated recurrence along each ray's samples, and
+ * matrix products by per-region sub-networks ("experts").  They take no ffn_ctx, allocate nothing
+ * and work on the caller's current device; every device pointer must be on it.  Columns are
+ * contiguous; *_ld is the stride between rows in elements; outputs have rows of exactly d (or k, m)
+ * elements.  Pointers need the alignment of their element type only (16-byte aligned rows take
+ * wider accesses).  Inputs and outputs must not overlap unless said so.  The messages of refused
+ * calls come from ffn_last_error(NULL). */
+enum { FFN_F32 = 0, FFN_F16 = 1, FFN_BF16 = 2, FFN_E4M3 = 3 };
+
+/* Root-mean-square norm of x + residual (residual may be NULL), n rows of d columns:
+ *   h = x + residual, rstd = 1 / sqrt(mean(h^2) + eps), y = h * rstd * gamma   (fp32 throughout)
+ * dtype (FFN_F32, FFN_F16, FFN_BF16): type of x, residual and h.  h and rstd ([n], fp32) may be NULL
+ * when they are not wanted; h is the sum rounded to dtype, y is formed from the unrounded sum.
+ * out_dtype is dtype, or FFN_E4M3: y holds e4m3 (nearest even, at most 448 in magnitude) of the value
+ * divided by its scale, scale = largest magnitude / 448 (1 where that is zero; NaN where a value is),
+ * per row (group 0: scale [n]) or per group of 32, 64 or 128 columns (scale [n][d / group]). */
+int ffn_rmsnorm(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, const float* gamma, void* h,
+                void* y, float* scale, float* rstd, int64_t n, int32_t d, float eps, int dtype, int out_dtype,
+                int32_t group, void* stream);
+/* Its backward pass from the saved h and rstd: dx (the gradient of x and of residual alike) =
+ *   rstd * (dy gamma - xhat mean(dy gamma xhat)) + dresidual, xhat = h rstd,
+ * and dgamma [d] fp32 = sum over rows of dy xhat, summed in a fixed order.  dresidual (the gradient
+ * that reaches h past the norm) may be NULL.  workspace: ffn_rmsnorm_bwd_workspace bytes. */
+uint64_t ffn_rmsnorm_bwd_workspace(int64_t n, int32_t d);
+int ffn_rmsnorm_bwd(const void* dy, int64_t dy_ld, const void* h, int64_t h_ld, const float* gamma, const float* rstd,
+                    const void* dresidual, int64_t dresidual_ld, void* dx, float* dgamma, void* workspace,
+                    uint64_t workspace_bytes, int64_t n, int32_t d, int dtype, void* stream);
+
+/* Gated linear recurrence per channel over n_seq sequences packed along the rows:
+ *   FFN_SCAN_LINEAR:  h_t = gate_t h_{t-1} + value_t          (gates of magnitude at most about 1)
+ *   FFN_SCAN_SIGMOID: h_t = a_t h_{t-1} + (1 - a_t) value_t,  a_t = 1 / (1 + exp(-gate_t))
+ * h0 [n_seq][d] fp32 is the state before the first step (NULL: zero); h_last [n_seq][d] fp32 receives
+ * the state after the last (may be NULL, may be h0 itself).  Sequence s is rows offsets[s] ..
+ * offsets[s+1] - 1 (32-bit, on the device, non-decreasing, at most n_rows; it may be empty: h_last is
+ * then h0), or max_len rows each when offsets is NULL.  With offsets max_len is how long a sequence is
+ * expected to get: it chooses how the work is split and bounds nothing.  Rows of no sequence get
+ * zeros.  reverse != 0 runs each sequence from its last row to its first.  State is fp32; h is dtype. */
+enum { FFN_SCAN_LINEAR = 0, FFN_SCAN_SIGMOID = 1 };
+int ffn_gated_scan(const void* gate, int64_t gate_ld, const void* value, int64_t value_ld, const float* h0,
+                   const int32_t* offsets, void* h, float* h_last, int64_t n_rows, int32_t n_seq, int64_t max_len,
+                   int32_t d, int dtype, int form, int reverse, void* stream);
+/* Its backward pass from the gradient dh of h, the gradient dh_last of h_last (fp32, may be NULL) and the
+ * forward pass's inputs and h: dgate, dvalue (dtype) and dh0 (fp32, may be NULL).  value is not read
+ * in the linear form (may be NULL).  form, reverse and offsets as in the forward call. */
+int ffn_gated_scan_bwd(const void* dh, int64_t dh_ld, const float* dh_last, const void* gate, int64_t gate_ld,
+                       const void* value, int64_t value_ld, const void* h, int64_t h_ld, const float* h0,
+                       const int32_t* offsets, void* dgate, void* dvalue, float* dh0, int64_t n_rows, int32_t n_seq,
+                       int64_t max_len, int32_t d, int dtype, int form, int reverse, void* stream);
+
+/* Matrix products of rows grouped by expert.  Rows are sorted by expert; expert e has rows
+ * offsets[e] .. offsets[e+1] - 1 (32-bit, on the device, experts + 1 of them, offsets[0] = 0,
+ * non-decreasing, at most n; an expert may have none) and weights w[e], [m][k] row-major:
+ *   y[r] = x[r] w[e]^T.
+ * Rows from offsets[experts] on belong to no expert; their results are zero.  dtype FFN_F16 or FFN_BF16
+ * (out_dtype the same), or FFN_E4M3 for x and w with x_scale [n] and w_scale [experts][m] fp32 (the
+ * products' value is x[r] w[e]^T * x_scale[r] * w_scale[e][.]; out_dtype FFN_F16 or FFN_BF16).  Sums are
+ * fp32.  The workspace (ffn_expert_mm_workspace bytes, 16-byte aligned; 0 where rows are 16-byte
+ * multiples) holds copies of operands whose rows cannot be read in 16-byte units. */
+#define FFN_MAX_EXPERTS 1024
+uint64_t ffn_expert_mm_workspace(const void* x, int64_t x_ld, const void* w, int64_t n, int32_t experts, int32_t k,
+                                 int32_t m, int dtype);
+int ffn_expert_mm(const void* x, int64_t x_ld, const void* w, const int32_t* offsets, const float* x_scale,
+                  const float* w_scale, void* y, int64_t n, int32_t experts, int32_t k, int32_t m, int dtype,
+                  int out_dtype, void* workspace, uint64_t workspace_bytes, void* stream);
+/* Both gradients (either may be NULL): dx[r] = dy[r] w[e] in dtype, and dw[e] = the sum over the
+ * expert's rows of dy[r]^T x[r], in dtype or fp32 (dw_dtype); an expert without rows gets zeros. */
+uint64_t ffn_expert_mm_bwd_workspace(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, const void* w,
+                                     int64_t n, int32_t experts, int32_t k, int32_t m, int dtype);
+int ffn_expert_mm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, const void* w, const int32_t* offsets,
+                      void* dx, void* dw, int64_t n, int32_t experts, int32_t k, int32_t m, int dtype, int dw_dtype,
+                      void* workspace, uint64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

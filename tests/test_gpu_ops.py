@@ -1,0 +1,441 @@
+"""The block operators' kernels (RMS norm, gated recurrence, products by expert) against 64-bit forms."""
+import numpy as np
+import pytest
+import torch
+
+import _ops64 as o64
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+TYPES = [F32, F16, BF16]
+
+
+@pytest.fixture(scope="module")
+def ops():
+    import ffn_ops
+    return ffn_ops
+
+
+def draw(seed, *shape, dtype=F32, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale).to(dtype).cuda()
+
+
+def strided(t, extra):
+    """The same matrix with `extra` unused columns between its rows."""
+    wide = torch.full((t.shape[0], t.shape[1] + extra), float("nan"), dtype=t.dtype, device=t.device)
+    wide[:, :t.shape[1]] = t
+    return wide[:, :t.shape[1]]
+
+
+# ------------------------------------------------------------------------------------------- norm
+NORM_SIZES = [(1, 1), (1, 1024), (3, 8), (5, 64), (33, 100), (7, 1000), (2, 1001), (9, 2056), (300, 40), (4, 8200),
+              (3, 16384), (2, 20011), (1000, 72)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,d", NORM_SIZES)
+def test_rmsnorm(ops, n, d, dtype):
+    x, r, g = draw(1, n, d, dtype=dtype, scale=3), draw(2, n, d, dtype=dtype), 1 + 0.3 * draw(3, d)
+    for res in (None, r):
+        y, h, rstd, scale = ops.rmsnorm(x, g, res, eps=1e-5)
+        assert scale is None and y.dtype is dtype and (res is not None or h is x)
+        h64, s64, y64 = o64.norm(x.cpu(), g.cpu(), None if res is None else res.cpu(), 1e-5)
+        rel = o64.norm_rel(d)
+        o64.within(y, y64, rel * y64.abs(), dtype)
+        o64.within(h, h64, 2.0 ** -24 * h64.abs(), dtype)
+        o64.within(rstd, s64, rel * s64, F32)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,d,group", [(1, 64, 0), (5, 1024, 0), (3, 1001, 0), (130, 64, 32), (9, 128, 128), (7, 4096, 64),
+                                       (6, 192, 64), (2, 20000, 0), (2, 32768, 128)])
+def test_rmsnorm_e4m3(ops, n, d, group, dtype):
+    x, r, g = draw(4, n, d, dtype=dtype, scale=2), draw(5, n, d, dtype=dtype), 1 + 0.3 * draw(6, d)
+    y, h, rstd, scale = ops.rmsnorm(x, g, r, out="e4m3", group=group)
+    assert y.dtype is torch.float8_e4m3fn and scale.shape == ((n, d // group) if group else (n,))
+    h64, s64, y64 = o64.norm(x.cpu(), g.cpu(), r.cpu(), 1e-6)
+    z = y64.view(n, -1, group or d)
+    top = z.abs().amax(2) / 448
+    o64.within(scale.view(n, -1), top, o64.norm_rel(d) * top, F32)
+    wide = scale.double().cpu().view(n, -1)[:, :, None]
+    got = y.float().double().cpu().view_as(z) * wide
+    # e4m3 keeps four bits: half a step is 2^-4 of a normal value, 2^-10 of the scale below 2^-6 of it
+    tol = z.abs() * (2.0 ** -4) * (1 + 1e-3) + wide * 2.0 ** -10 * (1 + 1e-3) + z.abs() * o64.norm_rel(d) * 2
+    assert bool(((got - z).abs() <= tol).all())
+    o64.within(h, h64, 2.0 ** -24 * h64.abs(), dtype)
+
+
+def test_rmsnorm_e4m3_rows_of_zeros_and_nan(ops):
+    x = draw(7, 4, 256, dtype=BF16)
+    x[1] = 0
+    x[2, 17] = float("nan")
+    g = torch.ones(256, device="cuda")
+    for group in (0, 64):
+        y, _, _, scale = ops.rmsnorm(x, g, out="e4m3", group=group)
+        s = scale.view(4, -1)
+        assert bool((y[1].float() == 0).all()) and bool((s[1] == 1).all())
+        assert bool(torch.isnan(s[2]).all()) and bool(torch.isnan(y[2].float()).all())     # the row's factor is NaN
+        assert bool(torch.isfinite(s[[0, 3]]).all()) and bool(torch.isfinite(y[[0, 3]].float()).all())
+    y = ops.rmsnorm(x, g)[0]
+    assert bool(torch.isnan(y[2]).all()) and bool(torch.isfinite(y[[0, 1, 3]]).all()) and bool((y[1] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,d", NORM_SIZES + [(3001, 64)])
+def test_rmsnorm_bwd(ops, n, d, dtype):
+    h, dy, dr, g = draw(1, n, d, dtype=dtype, scale=2), draw(2, n, d, dtype=dtype), draw(3, n, d, dtype=dtype), 1 + 0.3 * draw(4, d)
+    rstd = (1 / (h.double().square().mean(1) + 1e-6).sqrt()).float()
+    for res in (None, dr):
+        dx, dg = ops.rmsnorm_bwd(dy, h, g, rstd, res)
+        want, size, wg, sg = o64.norm_bwd(dy.cpu(), h.cpu(), g.cpu(), rstd.cpu(), None if res is None else res.cpu())
+        o64.within(dx, want, o64.norm_rel(d) * size, dtype)
+        # at most 64 rows of a thread one after another, then blocks and trees
+        o64.within(dg, wg, 2.0 ** -24 * 256 * sg, F32)
+        again = ops.rmsnorm_bwd(dy, h, g, rstd, res)
+        assert torch.equal(again[1], dg) and torch.equal(again[0], dx)
+
+
+def test_rmsnorm_strides_and_alignment(ops):
+    n, d = 37, 136
+    x, r, g = draw(1, n, d, dtype=F16), draw(2, n, d, dtype=F16), 1 + 0.3 * draw(3, d)
+    want = ops.rmsnorm(x, g, r)
+    for extra in (3, 8):
+        got = ops.rmsnorm(strided(x, extra), g, strided(r, extra))
+        for a, b in zip(got[:3], want[:3]):
+            torch.testing.assert_close(a, b, rtol=2e-3, atol=1e-4)   # another order of the sum, one fp16 rounding
+    flat = torch.empty(n * d + 1, dtype=F16, device="cuda")
+    off = flat[1:].view(n, d)
+    off.copy_(x)
+    got = ops.rmsnorm(off, g, r)
+    torch.testing.assert_close(got[0], want[0], rtol=2e-3, atol=1e-4)
+    dx, dg = ops.rmsnorm_bwd(strided(x, 8), strided(want[1], 3), g, want[2], strided(r, 5))
+    dx2, dg2 = ops.rmsnorm_bwd(x, want[1], g, want[2], r)
+    torch.testing.assert_close(dx, dx2, rtol=2e-3, atol=1e-3)
+    torch.testing.assert_close(dg, dg2, rtol=1e-4, atol=1e-4)
+
+
+def test_rmsnorm_gradient_against_differences(ops):
+    n, d = 11, 96
+    x, r, dy, v = (draw(i, n, d) for i in (1, 2, 3, 4))
+    g, vg = 1 + 0.3 * draw(5, d), draw(6, d)
+    _, h, rstd, _ = ops.rmsnorm(x, g, r)
+    dx, dg = ops.rmsnorm_bwd(dy, h, g, rstd)
+    loss = lambda a, b: float((ops.rmsnorm(a, b, r)[0].double() * dy.double()).sum())  # noqa: E731
+    e = 1e-2      # the truncation is e^2 of O(1) terms, the rounding 2^-24 / e of them
+    num = (loss(x + e * v, g) - loss(x - e * v, g)) / (2 * e)
+    ana = float((dx.double() * v.double()).sum())
+    assert abs(num - ana) < 2e-3 * float(dx.double().norm() * v.double().norm())
+    num = (loss(x, g + e * vg) - loss(x, g - e * vg)) / (2 * e)
+    assert abs(num - float((dg.double() * vg.double()).sum())) < 2e-3 * float(dg.double().norm() * vg.double().norm())
+
+
+def test_rmsnorm_no_rows(ops):
+    x, g = torch.empty(0, 32, dtype=BF16, device="cuda"), torch.ones(32, device="cuda")
+    y, h, rstd, _ = ops.rmsnorm(x, g)
+    assert y.shape == (0, 32) and rstd.shape == (0,)
+    dx, dg = ops.rmsnorm_bwd(x, x, g, rstd)
+    assert dx.shape == (0, 32) and bool((dg == 0).all())
+
+
+# ------------------------------------------------------------------------------------------- scan
+def lens_to_offsets(lens):
+    return [0] + np.cumsum(lens).tolist()
+
+
+SCAN_CASES = [  # lengths, channels
+    ([1], 1), ([1] * 40, 64), ([7, 0, 1, 33, 0], 20), ([64] * 9, 64), ([300], 6), ([1000, 3], 34), ([129, 2, 0, 700], 5),
+    ([5] * 300, 3), ([2500], 64)]
+
+
+def scan_inputs(lens, d, dtype, form, seed=0):
+    n = sum(lens)
+    gate = draw(seed + 1, n, d, scale=2.0) + 1
+    gate = (gate if form == "sigmoid" else torch.tanh(gate)).to(dtype)
+    return gate, draw(seed + 2, n, d, dtype=dtype), draw(seed + 3, len(lens), d)
+
+
+@pytest.mark.parametrize("form", ["sigmoid", "linear"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", range(len(SCAN_CASES)))
+def test_gated_scan(ops, case, dtype, form):
+    lens, d = SCAN_CASES[case]
+    off = lens_to_offsets(lens)
+    gate, value, h0 = scan_inputs(lens, d, dtype, form)
+    dh, dlast = draw(8, off[-1], d, dtype=dtype), draw(9, len(lens), d)
+    offsets = torch.tensor(off, dtype=torch.int32, device="cuda")
+    for reverse in (False, True):
+        for init in (None, h0):
+            c0 = None if init is None else init.cpu()
+            h64, l64, e, el = o64.scan(gate.cpu(), value.cpu(), c0, off, form, reverse)
+            # a split chosen for short sequences and one chosen for long ones give the same results
+            for max_len in (1, max(lens), None):
+                h, last = ops.gated_scan(gate, value, init, offsets, max_len, form, reverse)
+                o64.within(h, h64, e, dtype)
+                o64.within(last, l64, el, F32)
+            g64, v64, d64, eg, ev, e0 = o64.scan_bwd(dh.cpu(), dlast.cpu(), gate.cpu(), value.cpu(), h.cpu(), c0, off, form,
+                                                     reverse)
+            for max_len in (1, None):
+                dg, dv, d0 = ops.gated_scan_bwd(dh, gate, value, h, init, dlast, offsets, max_len, form, reverse)
+                o64.within(dg, g64, eg, dtype)
+                o64.within(dv, v64, ev, dtype)
+                o64.within(d0, d64, e0, F32)
+
+
+def test_gated_scan_uniform_layout_matches_offsets(ops):
+    b, t, d = 6, 50, 24
+    p = draw(1, b, t, 2 * d, dtype=BF16)
+    gate, value = p[..., :d], p[..., d:]                     # two halves of one projection
+    h, last = ops.gated_scan(gate, value)
+    off = torch.arange(b + 1, device="cuda", dtype=torch.int32) * t
+    h2, last2 = ops.gated_scan(gate.reshape(b * t, d), value.reshape(b * t, d), offsets=off, max_len=t)
+    assert torch.equal(h.view(-1, d), h2) and torch.equal(last, last2)
+    dh = draw(2, b, t, 2 * d, dtype=BF16)[..., d:]
+    got = ops.gated_scan_bwd(dh, gate, value, h)
+    want = ops.gated_scan_bwd(dh.contiguous(), gate.contiguous(), value.contiguous(), h)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    zero = torch.zeros(b, d, device="cuda")
+    want = ops.gated_scan_bwd(dh, gate, value, h, h0=zero, dh_last=zero)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_gated_scan_step_by_step(ops):
+    """Single steps that carry the state give what one call over the sequence gives."""
+    b, t, d = 5, 9, 40
+    gate, value = draw(1, b, t, d), draw(2, b, t, d)
+    h, last = ops.gated_scan(gate, value)
+    state = torch.zeros(b, d, device="cuda")
+    for i in range(t):
+        hi, state = ops.gated_scan(gate[:, i:i + 1], value[:, i:i + 1], h0=state)
+        torch.testing.assert_close(hi[:, 0], h[:, i], rtol=1e-5, atol=1e-6)
+    torch.testing.assert_close(state, last, rtol=1e-5, atol=1e-6)
+
+
+def test_gated_scan_composites_like_a_ray(ops):
+    """The sigmoid form run backwards is front-to-back compositing: sum of T_i alpha_i c_i."""
+    rays, s, d = 7, 64, 16
+    gate, c = draw(1, rays, s, 1).expand(rays, s, d).contiguous(), draw(2, rays, s, d)
+    _, out = ops.gated_scan(gate, c, reverse=True)
+    alpha = torch.sigmoid(-gate.double())
+    trans = torch.cumprod(torch.cat((torch.ones_like(alpha[:, :1]), 1 - alpha[:, :-1]), 1), 1)
+    torch.testing.assert_close(out.double(), (trans * alpha * c.double()).sum(1), rtol=1e-4, atol=1e-5)
+
+
+def test_gated_scan_extreme_gates(ops):
+    """Infinite logits are exact holds and resets; NaN stays in its channel and sequence; zero times an
+    overflowed product of gates stays zero."""
+    gate = torch.zeros(2, 200, 4, device="cuda")
+    gate[:, :, 0], gate[:, :, 1] = float("inf"), float("-inf")
+    gate[0, 5, 3] = float("nan")
+    value, h0 = draw(1, 2, 200, 4), draw(2, 2, 4)
+    h, last = ops.gated_scan(gate, value, h0=h0)
+    assert torch.equal(h[:, :, 0], h0[:, None, 0].expand(2, 200)) and torch.equal(h[:, :, 1], value[:, :, 1])
+    assert bool(torch.isnan(h[0, 5:, 3]).all()) and bool(torch.isfinite(h[0, :5]).all()) and bool(torch.isfinite(h[1]).all())
+    assert bool(torch.isfinite(h[:, :, :3]).all())
+    big = torch.full((1, 4000, 2), 2.0, device="cuda")
+    h, last = ops.gated_scan(big, torch.zeros_like(big), form="linear")
+    assert bool((h == 0).all()) and bool((last == 0).all())
+
+
+def test_gated_scan_rows_of_no_sequence(ops):
+    gate, value = draw(1, 20, 6), draw(2, 20, 6)
+    off = torch.tensor([3, 7, 7, 15], dtype=torch.int32, device="cuda")
+    for max_len in (1, 1000):
+        h, last = ops.gated_scan(gate, value, offsets=off, max_len=max_len)
+        inner, _ = ops.gated_scan(gate[3:15], value[3:15], offsets=off - 3, max_len=1)
+        torch.testing.assert_close(h[3:15], inner, rtol=1e-5, atol=1e-6)
+        assert bool((h[:3] == 0).all()) and bool((h[15:] == 0).all()) and bool((last[1] == 0).all())
+        dg, dv, _ = ops.gated_scan_bwd(value, gate, value, h, offsets=off, max_len=max_len)
+        assert all(bool((t[:3] == 0).all()) and bool((t[15:] == 0).all()) for t in (dg, dv))
+
+
+def test_gated_scan_gradient_against_differences(ops):
+    b, t, d = 3, 40, 8
+    gate, value, h0, dh, dl = draw(1, b, t, d), draw(2, b, t, d), draw(3, b, d), draw(4, b, t, d), draw(5, b, d)
+    for form in ("sigmoid", "linear"):
+        g = gate if form == "sigmoid" else torch.sigmoid(gate)
+        h, _ = ops.gated_scan(g, value, h0, form=form)
+        grads = ops.gated_scan_bwd(dh, g, value, h, h0, dl, form=form)
+
+        def loss(*a):
+            y, last = ops.gated_scan(*a, form=form)
+            return float((y.double() * dh.double()).sum() + (last.double() * dl.double()).sum())
+        at, e = [g, value, h0], 1e-2
+        for i in range(3):
+            v = draw(10 + i, *at[i].shape)
+            up, dn = list(at), list(at)
+            up[i], dn[i] = at[i] + e * v, at[i] - e * v
+            num, ana = (loss(*up) - loss(*dn)) / (2 * e), float((grads[i].double() * v.double()).sum())
+            assert abs(num - ana) < 4e-3 * float(grads[i].double().norm() * v.double().norm()), (form, i)
+
+
+def test_gated_scan_empty(ops):
+    z = torch.empty(0, 5, 4, device="cuda")
+    h, last = ops.gated_scan(z, z)
+    assert h.shape == (0, 5, 4) and last.shape == (0, 4)
+    z, h0 = torch.empty(3, 0, 4, device="cuda"), draw(1, 3, 4)
+    h, last = ops.gated_scan(z, z, h0=h0)
+    assert h.shape == (3, 0, 4) and torch.equal(last, h0)
+    dg, dv, d0 = ops.gated_scan_bwd(z, z, z, z, h0=h0, dh_last=h0)
+    assert torch.equal(d0, h0)
+
+
+# ---------------------------------------------------------------------------------------- experts
+EXPERT_CASES = [  # rows of each expert, rows of none, in, out
+    ([1], 0, 1, 1), ([1], 0, 64, 64), ([5, 0, 3], 2, 32, 48), ([128, 1, 0, 130], 0, 64, 64), ([0, 0], 3, 64, 64),
+    ([17, 300, 64], 5, 200, 136), ([33] * 8, 0, 256, 512), ([700], 1, 1000, 264), ([9, 40, 0, 21], 7, 77, 131),
+    ([2, 1, 0, 0, 4, 1, 0, 8], 0, 2048, 320), ([63, 65, 127, 129, 255], 1, 72, 40), ([1024, 512], 0, 128, 256),
+    ([10], 0, 8, 8)]
+
+
+def expert_inputs(case, dtype):
+    counts, spare, k, m = EXPERT_CASES[case]
+    off = lens_to_offsets(counts)
+    n = off[-1] + spare
+    x, w = draw(1, n, k, dtype=dtype), draw(2, len(counts), m, k, dtype=dtype, scale=k ** -0.5)
+    return x, w, off, torch.tensor(off, dtype=torch.int32, device="cuda"), draw(3, n, m, dtype=dtype)
+
+
+def sum_bound(terms, size):
+    """fp32 sums of that many terms in any order and rounding direction."""
+    return size * terms * 2.0 ** -23
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("case", range(len(EXPERT_CASES)))
+def test_expert_mm(ops, case, dtype):
+    x, w, off, offsets, dy = expert_inputs(case, dtype)
+    k, m = x.shape[1], w.shape[1]
+    y = ops.expert_mm(x, w, offsets)
+    want, size = o64.experts(x, w, off)
+    o64.within(y, want, sum_bound(k, size), dtype)
+    dx, dw = ops.expert_mm_bwd(dy, x, w, offsets)
+    want, size = o64.experts(dy, w.transpose(1, 2), off)
+    o64.within(dx, want, sum_bound(m, size), dtype)
+    assert bool((y[off[-1]:] == 0).all()) and bool((dx[off[-1]:] == 0).all())
+    _, dwf = ops.expert_mm_bwd(dy, x, w, offsets, need_dx=False, dw_dtype=F32)
+    for e in range(w.shape[0]):
+        xe, ye = x[off[e]:off[e + 1]].double(), dy[off[e]:off[e + 1]].double()
+        want, size = ye.t() @ xe, ye.abs().t() @ xe.abs()
+        o64.within(dw[e], want, sum_bound(len(xe), size), dtype)
+        o64.within(dwf[e], want, sum_bound(len(xe), size), F32)
+    assert ops.expert_mm_bwd(dy, x, w, offsets, need_dw=False)[1] is None
+
+
+@pytest.mark.parametrize("out", [F16, BF16])
+@pytest.mark.parametrize("case", range(len(EXPERT_CASES)))
+def test_expert_mm_e4m3(ops, case, out):
+    x, w, off, offsets, _ = expert_inputs(case, F32)
+    xs = (x.abs().amax(1) / 448).clamp_min(1e-12)
+    ws = (w.abs().amax(2) / 448).clamp_min(1e-12)
+    xq, wq = (x / xs[:, None]).to(torch.float8_e4m3fn), (w / ws[:, :, None]).to(torch.float8_e4m3fn)
+    y = ops.expert_mm(xq, wq, offsets, xs, ws, out_dtype=out)
+    want, size = o64.experts(xq.float().double() * xs[:, None].double(), wq.float().double() * ws[:, :, None].double(), off)
+    o64.within(y, want, sum_bound(x.shape[1] + 4, size), out)
+
+
+def test_expert_mm_ignores_other_rows(ops):
+    """NaN and infinity in the rows of one expert, or of none, reach no other expert's results."""
+    for counts, k, m in (([70, 3, 61, 20], 64, 96), ([5, 2, 9, 3], 256, 64)):
+        off = lens_to_offsets(counts)
+        n = off[-1] + 9
+        offsets = torch.tensor(off, dtype=torch.int32, device="cuda")
+        x, w, dy = draw(1, n, k, dtype=BF16), draw(2, 4, m, k, dtype=BF16), draw(3, n, m, dtype=BF16)
+        y, (dx, dw) = ops.expert_mm(x, w, offsets), ops.expert_mm_bwd(dy, x, w, offsets)
+        bad = torch.ones(n, dtype=torch.bool, device="cuda")
+        bad[off[2]:off[3]] = False
+        x2, dy2, w2 = x.clone(), dy.clone(), w.clone()
+        x2[bad], dy2[bad] = float("nan"), float("inf")
+        w2[[0, 1, 3]] = float("nan")
+        y2, (dx2, dw2) = ops.expert_mm(x2, w2, offsets), ops.expert_mm_bwd(dy2, x2, w2, offsets)
+        assert torch.equal(y2[~bad], y[~bad]) and torch.equal(dx2[~bad], dx[~bad]) and torch.equal(dw2[2], dw[2])
+        assert bool((y2[off[-1]:] == 0).all()) and bool((dx2[off[-1]:] == 0).all())
+
+
+def test_expert_mm_strides_and_alignment(ops):
+    counts, k, m = [40, 7, 100], 96, 80
+    off = lens_to_offsets(counts)
+    offsets = torch.tensor(off, dtype=torch.int32, device="cuda")
+    x, w, dy = draw(1, off[-1], k, dtype=F16), draw(2, 3, m, k, dtype=F16), draw(3, off[-1], m, dtype=F16)
+    y, (dx, dw) = ops.expert_mm(x, w, offsets), ops.expert_mm_bwd(dy, x, w, offsets)
+    for extra in (8, 3):
+        assert torch.equal(ops.expert_mm(strided(x, extra), w, offsets), y)
+        got = ops.expert_mm_bwd(strided(dy, extra), strided(x, 8), w, offsets)
+        assert torch.equal(got[0], dx) and torch.equal(got[1], dw)
+    flat = torch.empty(x.numel() + 1, dtype=F16, device="cuda")
+    odd = flat[1:].view(x.shape)
+    odd.copy_(x)
+    wflat = torch.empty(w.numel() + 1, dtype=F16, device="cuda")
+    wodd = wflat[1:].view(w.shape)
+    wodd.copy_(w)
+    assert torch.equal(ops.expert_mm(odd, wodd, offsets), y)
+    got = ops.expert_mm_bwd(dy, odd, wodd, offsets)
+    assert torch.equal(got[0], dx) and torch.equal(got[1], dw)
+
+
+def test_expert_mm_gradient_against_differences(ops):
+    """Small integers make every product exact, so differences of the (linear) forward are too."""
+    off = [0, 30, 30, 95]
+    offsets = torch.tensor(off, dtype=torch.int32, device="cuda")
+    g = torch.Generator().manual_seed(0)
+    ints = lambda *s: torch.randint(-2, 3, s, generator=g).to(F16).cuda()  # noqa: E731
+    x, w, dy, vx, vw = ints(95, 40), ints(3, 24, 40), ints(95, 24), ints(95, 40), ints(3, 24, 40)
+    dx, dw = ops.expert_mm_bwd(dy, x, w, offsets, dw_dtype=F32)
+    loss = lambda a, b: float((ops.expert_mm(a, b, offsets).double() * dy.double()).sum())  # noqa: E731
+    assert loss(x + vx, w) - loss(x, w) == float((dx.double() * vx.double()).sum())
+    assert loss(x, w + vw) - loss(x, w) == float((dw.double() * vw.double()).sum())
+
+
+def test_expert_mm_is_the_same_on_every_run(ops):
+    x, w, off, offsets, dy = expert_inputs(5, BF16)
+    a, b = ([ops.expert_mm(x, w, offsets), *ops.expert_mm_bwd(dy, x, w, offsets)] for _ in range(2))
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_expert_mm_no_rows(ops):
+    x, w = torch.empty(0, 64, dtype=BF16, device="cuda"), draw(1, 3, 32, 64, dtype=BF16)
+    offsets = torch.zeros(4, dtype=torch.int32, device="cuda")
+    assert ops.expert_mm(x, w, offsets).shape == (0, 32)
+    dx, dw = ops.expert_mm_bwd(torch.empty(0, 32, dtype=BF16, device="cuda"), x, w, offsets)
+    assert dx.shape == (0, 64) and bool((dw == 0).all())
+
+
+# ------------------------------------------------------------------------------------ all of them
+def test_streams(ops):
+    """On a stream of the caller's, ordered after what produced the inputs."""
+    s = torch.cuda.Stream()
+    x, g = draw(1, 500, 256, dtype=BF16), torch.ones(256, device="cuda")
+    want = ops.rmsnorm(x, g)[0]
+    s.wait_stream(torch.cuda.current_stream())
+    y = ops.rmsnorm(x, g, stream=s)[0]
+    h, last = ops.gated_scan(y.view(5, 100, 256), y.view(5, 100, 256), stream=s)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(y, want)
+    h2, last2 = ops.gated_scan(want.view(5, 100, 256), want.view(5, 100, 256))
+    assert torch.equal(h, h2) and torch.equal(last, last2)
+
+
+def test_refusals_on_the_device(ops):
+    x, g = draw(1, 8, 64, dtype=BF16), torch.ones(64, device="cuda")
+    w = draw(2, 2, 32, 64, dtype=BF16)
+    off = torch.tensor([0, 4, 8], dtype=torch.int32, device="cuda")
+    for call in (
+            lambda: ops.rmsnorm(x.double(), g), lambda: ops.rmsnorm(x, g[:32]), lambda: ops.rmsnorm(x, g.to(BF16)),
+            lambda: ops.rmsnorm(x, g, x.half()), lambda: ops.rmsnorm(x, g, x[:4]), lambda: ops.rmsnorm(x.t(), g),
+            lambda: ops.rmsnorm(x, g, out="e5m2"), lambda: ops.rmsnorm(x, g, out="e4m3", group=48),
+            lambda: ops.rmsnorm(x, g, group=32), lambda: ops.rmsnorm(x, g, eps=-1.0), lambda: ops.rmsnorm(x[0], g),
+            lambda: ops.rmsnorm_bwd(x, x, g, torch.ones(7, device="cuda")),
+            lambda: ops.rmsnorm_bwd(x, x.half(), g, torch.ones(8, device="cuda")),
+            lambda: ops.gated_scan(x, x), lambda: ops.gated_scan(x[None], x[None], form="tanh"),
+            lambda: ops.gated_scan(x[None], x[None].float()), lambda: ops.gated_scan(x, x, offsets=off.long()),
+            lambda: ops.gated_scan(x, x, offsets=off.cpu()), lambda: ops.gated_scan(x, x, offsets=off, h0=x.float()),
+            lambda: ops.gated_scan(x[None], x[None, :4]), lambda: ops.gated_scan(x, x, offsets=off, max_len=-1),
+            lambda: ops.gated_scan_bwd(x[None, :, :32], x[None], x[None], x[None]),
+            lambda: ops.expert_mm(x.float(), w.float(), off), lambda: ops.expert_mm(x, w.half(), off),
+            lambda: ops.expert_mm(x[:, :32], w, off), lambda: ops.expert_mm(x, w, off[:2]),
+            lambda: ops.expert_mm(x, w, off, x_scale=torch.ones(8, device="cuda")),
+            lambda: ops.expert_mm(x.to(torch.float8_e4m3fn), w.to(torch.float8_e4m3fn), off),
+            lambda: ops.expert_mm(x, w.transpose(1, 2), off), lambda: ops.expert_mm(x, w, off, out_dtype=F16),
+            lambda: ops.expert_mm_bwd(x, x, w, off), lambda: ops.expert_mm_bwd(x[:, :32], x, w, off, dw_dtype=F16)):
+        with pytest.raises(ValueError):
+            call()

@@ -1,0 +1,80 @@
+"""Refusals of the block operators that need no GPU, and the 64-bit forms the GPU tests compare with."""
+import ctypes as C
+
+import pytest
+import torch
+
+import _ops64 as o64
+import ffn_native as fn
+import ffn_ops as ops
+
+
+def refused(rc, lib, word):
+    assert rc == fn.FFN_E_CONFIG
+    assert word in lib.ffn_last_error(None).decode()
+
+
+def test_entry_points_check_their_arguments():
+    """Sizes, types and missing pointers are refused before anything is launched."""
+    lib = fn.load_library()
+    p = C.c_void_p(0x1000)   # never read: each call is refused on its sizes or types
+    refused(lib.ffn_rmsnorm(p, 8, None, 0, p, None, p, None, None, -1, 8, 1e-6, 0, 0, 0, None), lib, "n must be")
+    refused(lib.ffn_rmsnorm(p, 8, None, 0, p, None, p, None, None, 4, 8, 1e-6, 3, 3, 0, None), lib, "dtype")
+    refused(lib.ffn_rmsnorm(p, 8, None, 0, p, None, p, None, None, 4, 8, 1e-6, 1, 2, 0, None), lib, "out_dtype")
+    refused(lib.ffn_rmsnorm(p, 8, None, 0, p, None, p, p, None, 4, 8, 1e-6, 1, 3, 32, None), lib, "group")
+    refused(lib.ffn_rmsnorm(p, 8, None, 0, p, None, p, None, None, 4, 8, float("nan"), 1, 1, 0, None), lib, "eps")
+    refused(lib.ffn_rmsnorm(None, 8, None, 0, p, None, p, None, None, 4, 8, 1e-6, 1, 1, 0, None), lib, "NULL")
+    refused(lib.ffn_rmsnorm(p, 7, None, 0, p, None, p, None, None, 4, 8, 1e-6, 1, 1, 0, None), lib, "stride")
+    refused(lib.ffn_rmsnorm_bwd(p, 8, p, 8, p, p, None, 0, p, None, p, 0, 4, 8, 1, None), lib, "NULL")
+    refused(lib.ffn_gated_scan(p, 4, p, 4, None, None, p, None, 12, 3, 5, 4, 0, 1, 0, None), lib, "n_seq * max_len")
+    refused(lib.ffn_gated_scan(p, 4, p, 4, None, None, p, None, 15, 3, 5, 4, 0, 2, 0, None), lib, "form")
+    refused(lib.ffn_gated_scan(p, 4, p, 4, None, p, p, None, 1 << 31, 3, 5, 4, 0, 0, 0, None), lib, "32 bits")
+    refused(lib.ffn_gated_scan(p, 3, p, 4, None, None, p, None, 15, 3, 5, 4, 0, 0, 0, None), lib, "stride")
+    refused(lib.ffn_gated_scan_bwd(p, 4, None, p, 4, None, 0, p, 4, None, None, p, p, None, 15, 3, 5, 4, 0, 1, 0, None), lib,
+            "NULL")
+    refused(lib.ffn_expert_mm(p, 8, p, p, None, None, p, 4, 0, 8, 8, 1, 1, None, 0, None), lib, "experts")
+    refused(lib.ffn_expert_mm(p, 8, p, p, None, None, p, 4, 5000, 8, 8, 1, 1, None, 0, None), lib, "experts")
+    refused(lib.ffn_expert_mm(p, 7, p, p, None, None, p, 4, 2, 8, 8, 1, 1, None, 0, None), lib, "stride")
+    refused(lib.ffn_expert_mm(p, 8, p, p, None, None, p, 4, 2, 8, 8, 0, 0, None, 0, None), lib, "dtype")
+    refused(lib.ffn_expert_mm(p, 8, p, p, None, None, p, 4, 2, 8, 8, 3, 1, None, 0, None), lib, "scale")
+    refused(lib.ffn_expert_mm_bwd(p, 8, p, 8, p, p, p, p, 4, 2, 8, 8, 3, 3, None, 0, None), lib, "dtype")
+    refused(lib.ffn_expert_mm_bwd(p, 8, p, 8, p, p, p, p, 4, 2, 8, 8, 1, 2, None, 0, None), lib, "dw_dtype")
+
+
+def test_tensors_on_the_cpu_are_refused():
+    x = torch.zeros(4, 8)
+    off = torch.zeros(3, dtype=torch.int32)
+    for call in (lambda: ops.rmsnorm(x, torch.ones(8)), lambda: ops.gated_scan(x[None], x[None]),
+                 lambda: ops.expert_mm(x.half(), torch.zeros(2, 4, 8).half(), off)):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
+
+
+def test_64_bit_gradients_against_differences():
+    """The gradient formulas of the 64-bit forms against central differences of their forward passes."""
+    g = torch.Generator().manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)  # noqa: E731
+    x, gamma, dy, e = r(4, 12), 1 + 0.1 * r(12), r(4, 12), 1e-6
+    h, s, _ = o64.norm(x, gamma, None, 1e-5)
+    dx, _, dg, _ = o64.norm_bwd(dy, h, gamma, s, None)
+    for at, grad in ((0, dx), (1, dg)):
+        v = r(*grad.shape)
+        move = (lambda t: o64.norm(x + t * v, gamma, None, 1e-5)[2]) if at == 0 else \
+            (lambda t: o64.norm(x, gamma + t * v, None, 1e-5)[2])  # noqa: E731
+        num = float(((move(e) - move(-e)) * dy).sum() / (2 * e))
+        assert abs(num - float((grad * v).sum())) < 1e-6 * float(grad.norm() * v.norm())
+    off = [0, 4, 4, 9]
+    gate, value, h0, dh, dl = r(9, 3), r(9, 3), r(3, 3), r(9, 3), r(3, 3)
+    for form in ("sigmoid", "linear"):
+        for reverse in (False, True):
+            hh = o64.scan(gate, value, h0, off, form, reverse)[0]
+            grads = o64.scan_bwd(dh, dl, gate, value, hh, h0, off, form, reverse)[:3]
+
+            def loss(a):
+                y, last = o64.scan(*a, off, form, reverse)[:2]
+                return float((y * dh).sum() + (last * dl).sum())
+            for i, grad in enumerate(grads):
+                v, args = r(*grad.shape), [gate, value, h0]
+                up, dn = list(args), list(args)
+                up[i], dn[i] = args[i] + e * v, args[i] - e * v
+                assert abs((loss(up) - loss(dn)) / (2 * e) - float((grad * v).sum())) < 1e-6 * float(grad.norm() * v.norm() + 1)
