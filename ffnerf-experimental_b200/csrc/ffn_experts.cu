@@ -6,82 +6,636 @@
 //   dx[r] = dy[r] W_e,       dW_e = sum over the rows of e of dy[r]^T x[r]
 //
 // Rows after offsets[experts] belong to no expert: their y and dx are zero.
+//
+// All four products run in one persistent kernel on the tensor cores: a block per SM walks the output
+// tiles of all experts, which it finds from the offsets on the device (the host never reads them, so a
+// call synchronises nothing and can be captured in a graph).  Warp roles: one thread issues TMA loads
+// into a ring of shared-memory stages (128 bytes of depth each, 128-byte swizzle), one warp issues
+// tcgen05.mma into one of two accumulators in tensor memory, four warps read the other accumulator,
+// scale, convert and store it, so loads, products and stores of neighbouring tiles overlap.
+//
+//   forward  A = x rows,           B = W rows           both with depth k contiguous
+//   few rows A = W rows (128), B = x rows (16 to 64): the weights fill the tensor core's 128 lanes, the
+//            rows its columns; used when an expert has few rows on average and W's bytes are the cost
+//   dx       A = dy rows, B = W read with its columns along N (MN-major), depth m
+//   dW       A = dy and B = x, both read with rows as depth (MN-major); no operand is transposed in memory
+//
+// Tiles at the end of an expert's rows hold rows of the next expert; their products are formed and not
+// stored (a row's products depend on that row only).  In dW the rows are the depth: there the stage that
+// reaches past the expert's last row has the rest of its rows cleared in shared memory, in both
+// operands, since a NaN times zero would not be zero.
+#include <atomic>
+#include <cuda.h>
+
 #include "ffn_ops.cuh"
+#include "ffn_tcgen05.cuh"
 
 namespace ffn {
 namespace {
 
-// An expert's rows, kept inside [0, n] whatever the offsets hold.
-__device__ __forceinline__ void expert_rows(const int32_t* off, int e, int64_t n, int64_t& b, int64_t& end) {
-    b = e == 0 ? 0 : min(max((int64_t)__ldg(off + e), (int64_t)0), n);
-    end = min(max((int64_t)__ldg(off + e + 1), b), n);
-}
+enum { FORWARD = 0, INPUT_GRAD = 1, WEIGHT_GRAD = 2, FEW_ROWS = 3 };
 
-// C[i][j] = sum_l A[i][l] B[j][l] with any strides, 64 x 64 outputs per block, fp32 throughout.
-struct Plain {
-    const void* a; const void* b; void* c;
-    const float* a_scale; const float* b_scale;
+constexpr int BM = 128;                    // lanes of an accumulator
+constexpr int KB = 128;                    // bytes of depth in a stage (K-major), or 64 rows (MN-major)
+constexpr int EPI_WARPS = 4;
+constexpr int THREADS = 32 * (EPI_WARPS + 2);
+constexpr int SLAB = 32 * 128;             // one warp's 32 rows x 128 bytes of output
+constexpr size_t SMEM_MOST = 232448;       // what a block may have
+constexpr uint32_t WAIT_ROUNDS = 1u << 12, WAIT_POLLS = 1u << 10;
+
+__device__ int g_status;                   // ST_TC_TIMEOUT when a wait ran out (ffn_ops_status)
+
+struct Args {
     const int32_t* offsets;
-    int64_t n, a_row, a_col, b_row, b_col, b_expert, c_row, c_expert;
-    int rows, cols, depth, experts, mode;     // mode 0: rows are ragged, 1: depth is ragged
+    const float* a_scale; const float* b_scale;
+    void* out;
+    int64_t n;
+    int experts, cols, depth, rows_m;      // cols: width of the output; rows_m: dW's rows
+    int ntiles, mtiles;                    // tiles along the output's width; dW's tiles along its rows
+    int tma_out;                           // the output can be stored by TMA (16-byte rows)
 };
 
-template <typename T, typename TO>
-__global__ void __launch_bounds__(256) experts_plain_kernel(const Plain p) {
-    __shared__ float sa[16][65], sb[16][65];
-    int64_t begin = 0, end = 0;
-    int e = 0;
-    int64_t i0 = 0;
-    if (p.mode == 0) {
-        int64_t tile = blockIdx.x;
-        for (e = 0; e < p.experts; ++e) {
-            expert_rows(p.offsets, e, p.n, begin, end);
-            const int64_t tiles = (end - begin + 63) / 64;
-            if (tile < tiles) break;
-            tile -= tiles;
-        }
-        if (e == p.experts) {            // rows of no expert
-            int64_t b, last;
-            expert_rows(p.offsets, p.experts - 1, p.n, b, last);
-            for (int64_t r = last + tile * 64; r < min(last + tile * 64 + 64, p.n); ++r)
-                for (int j = threadIdx.x + blockIdx.y * 64; j < min((int)blockIdx.y * 64 + 64, p.cols); j += 256)
-                    static_cast<TO*>(p.c)[r * p.c_row + j] = from_f<TO>(0.0f);
-            return;
-        }
-        i0 = begin + tile * 64;
+// An expert's rows, kept inside [0, n] whatever the offsets hold.
+__device__ __forceinline__ void expert_rows(const Args& p, int e, int64_t& b, int64_t& end) {
+    b = e == 0 ? 0 : min(max((int64_t)__ldg(p.offsets + e), (int64_t)0), p.n);
+    end = min(max((int64_t)__ldg(p.offsets + e + 1), b), p.n);
+}
+
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+    return tc::make_desc(saddr, lbo, sbo) | (2ull << 61);
+}
+__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n"
+                 :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+__device__ __forceinline__ void mma_16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
+                 :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+__device__ __forceinline__ void tma_load2(uint32_t dst, const CUtensorMap* m, int x, int y, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 :: "r"(dst), "l"(m), "r"(x), "r"(y), "r"(tc::smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tma_load3(uint32_t dst, const CUtensorMap* m, int x, int y, int z, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 :: "r"(dst), "l"(m), "r"(x), "r"(y), "r"(z), "r"(tc::smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tma_store2(const CUtensorMap* m, int x, int y, uint32_t src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
+                 :: "l"(m), "r"(x), "r"(y), "r"(src) : "memory");
+}
+__device__ __forceinline__ void tma_store3(const CUtensorMap* m, int x, int y, int z, uint32_t src) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];"
+                 :: "l"(m), "r"(x), "r"(y), "r"(z), "r"(src) : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void bulk_wait_read() {
+    asm volatile("cp.async.bulk.wait_group.read %0;" :: "n"(N) : "memory");
+}
+__device__ __forceinline__ void expect_tx(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(tc::smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(tc::smem_u32(bar)) : "memory");
+}
+// 32 consecutive columns of this thread's lane.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+
+template <typename TO> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Shape of a variant: bytes of a stage, stages, and the layout of shared memory.
+template <int MODE, int BN, int EB>
+struct Plan {
+    static constexpr int A_BYTES = BM * KB;
+    static constexpr int B_BYTES = BN * KB;
+    static constexpr int STAGE = A_BYTES + B_BYTES;
+    static constexpr int EPI = MODE == FEW_ROWS ? 0 : EPI_WARPS * 2 * SLAB;
+    static constexpr int MISC = 1024 + 4 * (FFN_MAX_EXPERTS + 1) + 512;   // alignment, prefix, barriers
+    static constexpr int FIT = (int)((SMEM_MOST - EPI - MISC) / STAGE);
+    static constexpr int STAGES = FIT > 12 ? 12 : FIT;
+    static constexpr size_t BYTES = (size_t)STAGE * STAGES + EPI + MISC;
+    static constexpr int ACC_COLS = BN < 32 ? 32 : BN;
+    static constexpr int TMEM_COLS = 2 * ACC_COLS;                         // a power of two: 64 .. 512
+    [[maybe_unused]] static constexpr int DEPTH = MODE == WEIGHT_GRAD || MODE == INPUT_GRAD ? 64 : KB / EB;   // depth of a stage, elements
+};
+
+struct Tile {
+    int e, blocks;               // expert, stages of depth
+    int64_t row, end;            // first row of the tile (of the depth in dW), end of the expert's rows
+    int col, mrow;               // first output column; dW: first output row
+};
+
+template <int MODE, int BN, int EB>
+__device__ __forceinline__ Tile find_tile(const Args& p, const int* prefix, int t) {
+    Tile k;
+    int64_t b, end;
+    if constexpr (MODE == WEIGHT_GRAD) {
+        const int per = p.ntiles * p.mtiles;
+        k.e = t / per;
+        const int r = t - k.e * per;
+        k.mrow = (r % p.mtiles) * BM;
+        k.col = (r / p.mtiles) * BN;
+        expert_rows(p, k.e, b, end);
+        k.row = b;
+        k.end = end;
+        k.blocks = (int)((end - b + 63) / 64);
     } else {
-        e = blockIdx.z;
-        expert_rows(p.offsets, e, p.n, begin, end);
-        i0 = (int64_t)blockIdx.x * 64;
+        const int q = t / p.ntiles;
+        int lo = 0, hi = p.experts;                    // prefix[lo] <= q < prefix[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (prefix[mid] <= q) lo = mid; else hi = mid;
+        }
+        k.e = lo;
+        const int tiles = prefix[lo + 1] - prefix[lo], r = t - prefix[lo] * p.ntiles;
+        expert_rows(p, lo, b, end);
+        // neighbouring blocks take the same weights and the expert's row tiles in turn
+        k.row = b + (int64_t)(r % tiles) * (MODE == FEW_ROWS ? BN : BM);
+        k.col = (r / tiles) * (MODE == FEW_ROWS ? BM : BN);
+        k.end = end;
+        k.mrow = 0;
+        constexpr int D = Plan<MODE, BN, EB>::DEPTH;
+        k.blocks = (p.depth + D - 1) / D;
     }
-    const int64_t i_end = p.mode == 0 ? end : p.rows;
-    const int64_t l0 = p.mode == 0 ? 0 : begin, l1 = p.mode == 0 ? p.depth : end;
-    const int64_t j0 = (int64_t)blockIdx.y * 64;
-    const T* A = static_cast<const T*>(p.a);
-    const T* B = static_cast<const T*>(p.b) + (int64_t)e * p.b_expert;
-    float acc[4][4] = {};
-    const int ti = threadIdx.x / 16, tj = threadIdx.x % 16;
-    for (int64_t l = l0; l < l1; l += 16) {
-        for (int q = threadIdx.x; q < 1024; q += 256) {
-            const int64_t i = i0 + q / 16, j = j0 + q / 16, ll = l + q % 16;
-            sa[q % 16][q / 16] = i < i_end && ll < l1 ? to_f(A[i * p.a_row + ll * p.a_col]) : 0.0f;
-            sb[q % 16][q / 16] = j < p.cols && ll < l1 ? to_f(B[j * p.b_row + ll * p.b_col]) : 0.0f;
+    return k;
+}
+
+// Waits for a phase of an mbarrier; false when the wait ran out here or in another role of the block.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* gone) {
+    for (uint32_t i = 0; i < WAIT_ROUNDS; ++i) {
+        if (tc::mbar_wait(bar, parity, WAIT_POLLS)) return true;
+        if (*gone) return false;
+    }
+    *gone = 1;
+    atomicOr(&g_status, 4);
+    return false;
+}
+
+template <int MODE, int BN, int EB, typename TO, bool BF>
+__global__ void __launch_bounds__(THREADS, 1)
+experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb,
+               const __grid_constant__ CUtensorMap mo) {
+    using P = Plan<MODE, BN, EB>;
+    constexpr int S = P::STAGES;
+    extern __shared__ unsigned char raw[];
+    unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    unsigned char* slabs = base + (size_t)P::STAGE * S;
+    int* prefix = reinterpret_cast<int*>(slabs + P::EPI);
+    uint64_t* full = reinterpret_cast<uint64_t*>(slabs + P::EPI + ((4 * (FFN_MAX_EXPERTS + 1) + 15) & ~15));
+    uint64_t* empty = full + S;
+    uint64_t* done = empty + S;              // accumulator filled
+    uint64_t* freed = done + 2;              // accumulator read
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(freed + 2);
+    volatile int* gone = reinterpret_cast<volatile int*>(tmem_at + 1);
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+
+    if (warp == EPI_WARPS + 1) {
+        tc::tmem_alloc(tmem_at, P::TMEM_COLS);
+        if (lane == 0) {
+            for (int i = 0; i < S; ++i) { tc::mbar_init(full + i, 1); tc::mbar_init(empty + i, 1); }
+            for (int i = 0; i < 2; ++i) { tc::mbar_init(done + i, 1); tc::mbar_init(freed + i, EPI_WARPS); }
+            *gone = 0;
+        }
+    }
+    int total;
+    if constexpr (MODE == WEIGHT_GRAD) {
+        total = p.experts * p.ntiles * p.mtiles;
+    } else {
+        // tiles of the experts before each: counts side by side, then one warp adds them up
+        constexpr int R = MODE == FEW_ROWS ? BN : BM;
+        for (int e = threadIdx.x; e < p.experts; e += THREADS) {
+            int64_t b, end;
+            expert_rows(p, e, b, end);
+            prefix[e + 1] = (int)((end - b + R - 1) / R);
         }
         __syncthreads();
-        for (int s = 0; s < 16; ++s)
-            for (int u = 0; u < 4; ++u)
-                for (int v = 0; v < 4; ++v) acc[u][v] = fmaf(sa[s][ti + 16 * u], sb[s][tj + 16 * v], acc[u][v]);
-        __syncthreads();
-    }
-    TO* C = static_cast<TO*>(p.c) + (int64_t)e * p.c_expert;
-    for (int u = 0; u < 4; ++u)
-        for (int v = 0; v < 4; ++v) {
-            const int64_t i = i0 + ti + 16 * u, j = j0 + tj + 16 * v;
-            if (i >= i_end || j >= p.cols) continue;
-            float r = acc[u][v];
-            if (p.a_scale) r *= p.a_scale[i] * p.b_scale[(int64_t)e * p.cols + j];
-            C[i * p.c_row + j] = from_f<TO>(r);
+        if (warp == 0) {
+            // valid offsets give at most `most` tiles; sums stop there, so that offsets that are not
+            // (decreasing ones, whose experts overlap) cannot wrap
+            const int most = (int)(p.n / R) + p.experts;
+            int sum = 0;
+            for (int e0 = 0; e0 < p.experts; e0 += 32) {
+                int v = e0 + lane < p.experts ? prefix[e0 + lane + 1] : 0;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int u = __shfl_up_sync(0xffffffffu, v, o);
+                    if (lane >= o) v = min(v + u, most);
+                }
+                v = min(sum + v, most);
+                if (e0 + lane < p.experts) prefix[e0 + lane + 1] = v;
+                sum = __shfl_sync(0xffffffffu, v, 31);
+            }
+            if (lane == 0) prefix[0] = 0;
         }
+        __syncthreads();
+        total = prefix[p.experts] * p.ntiles;
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
+
+    if (warp == EPI_WARPS) {                                     // ---- loads
+        if (lane == 0) {
+            int s = 0, issued = 0;
+            uint32_t ph = 1;
+            bool ok = true;
+            for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+                const Tile k = find_tile<MODE, BN, EB>(p, prefix, t);
+                for (int b = 0; b < k.blocks; ++b) {
+                    if (!(ok = wait(empty + s, ph, gone))) break;
+                    const uint32_t sa = tc::smem_u32(base + (size_t)s * P::STAGE), sb = sa + P::A_BYTES;
+                    if constexpr (MODE == FORWARD) {
+                        expect_tx(full + s, P::STAGE);
+                        tma_load2(sa, &ma, b * P::DEPTH, (int)k.row, full + s);
+                        tma_load3(sb, &mb, b * P::DEPTH, k.col, k.e, full + s);
+                    } else if constexpr (MODE == FEW_ROWS) {
+                        expect_tx(full + s, P::STAGE);
+                        tma_load3(sa, &ma, b * P::DEPTH, k.col, k.e, full + s);
+                        tma_load2(sb, &mb, b * P::DEPTH, (int)k.row, full + s);
+                    } else {
+                        // boxes of 64 columns; those wholly outside the matrix are left out (what is in
+                        // their place reaches only outputs that are not stored)
+                        const int nb = min(BN / 64, (p.cols - k.col + 63) / 64);
+                        if constexpr (MODE == INPUT_GRAD) {
+                            expect_tx(full + s, P::A_BYTES + nb * 8192);
+                            tma_load2(sa, &ma, b * 64, (int)k.row, full + s);
+                            for (int j = 0; j < nb; ++j) tma_load3(sb + j * 8192, &mb, k.col + j * 64, b * 64, k.e, full + s);
+                        } else {
+                            const int na = min(BM / 64, (p.rows_m - k.mrow + 63) / 64);
+                            expect_tx(full + s, (na + nb) * 8192);
+                            for (int j = 0; j < na; ++j)
+                                tma_load2(sa + j * 8192, &ma, k.mrow + j * 64, (int)(k.row + b * 64), full + s);
+                            for (int j = 0; j < nb; ++j)
+                                tma_load2(sb + j * 8192, &mb, k.col + j * 64, (int)(k.row + b * 64), full + s);
+                        }
+                    }
+                    ++issued;
+                    if (++s == S) { s = 0; ph ^= 1; }
+                }
+            }
+            if (!ok)                                              // let the copies in flight land
+                for (int i = 0; i < (issued < S ? issued : S); ++i) {
+                    const int q = issued - 1 - i;
+                    tc::mbar_wait(full + q % S, (uint32_t)(q / S) & 1u, 1u << 20);
+                }
+        }
+    } else if (warp == EPI_WARPS + 1) {                           // ---- products
+        constexpr bool A_MN = MODE == WEIGHT_GRAD, B_MN = MODE == INPUT_GRAD || MODE == WEIGHT_GRAD;
+        constexpr uint32_t IDESC = tc::idesc_f16(BM, BN, A_MN, B_MN) |
+                                   (EB == 2 && BF ? (1u << 7) | (1u << 10) : 0u);
+        int s = 0, acc = 0;
+        uint32_t ph = 0, aph = 1;
+        bool ok = true;
+        for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+            const Tile k = find_tile<MODE, BN, EB>(p, prefix, t);
+            if (!(ok = wait(freed + acc, aph, gone))) break;
+            tc::fence_after_sync();
+            const uint32_t d = tmem + acc * P::ACC_COLS;
+            for (int b = 0; b < k.blocks; ++b) {
+                if (!(ok = wait(full + s, ph, gone))) break;
+                tc::fence_after_sync();
+                const uint32_t sa = tc::smem_u32(base + (size_t)s * P::STAGE), sb = sa + P::A_BYTES;
+                int steps = 4;
+                if constexpr (MODE == WEIGHT_GRAD) {
+                    const int64_t left = k.end - k.row - (int64_t)b * 64;
+                    if (left < 64) {                              // rows of the next expert become zeros
+                        steps = ((int)left + 15) / 16;
+                        const int rows = steps * 16 - (int)left;
+                        constexpr int CH = (BM + BN) / 64;
+                        for (int i = lane; i < CH * rows * 8; i += 32) {
+                            const int ch = i / (rows * 8), r = (int)left + (i / 8) % rows;
+                            *reinterpret_cast<uint4*>(base + (size_t)s * P::STAGE + ch * 8192 + r * 128 + (i & 7) * 16) =
+                                make_uint4(0, 0, 0, 0);
+                        }
+                        tc::fence_proxy_async();
+                        __syncwarp();
+                    }
+                }
+                if (lane == 0) {
+                    const uint64_t da = A_MN ? desc_sw128(sa, 8192, 1024) : desc_sw128(sa, 16, 1024);
+                    const uint64_t db = B_MN ? desc_sw128(sb, 8192, 1024) : desc_sw128(sb, 16, 1024);
+                    constexpr uint64_t STEP_A = (A_MN ? 2048 : 32) >> 4, STEP_B = (B_MN ? 2048 : 32) >> 4;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (MODE != WEIGHT_GRAD || i < steps) {
+                            if constexpr (EB == 1) mma_f8(d, da + i * STEP_A, db + i * STEP_B, IDESC, (b | i) != 0);
+                            else mma_16(d, da + i * STEP_A, db + i * STEP_B, IDESC, (b | i) != 0);
+                        }
+                    tc::commit(empty + s);
+                }
+                __syncwarp();
+                if (++s == S) { s = 0; ph ^= 1; }
+            }
+            if (lane == 0 && ok) tc::commit(done + acc);
+            __syncwarp();
+            if (++acc == 2) { acc = 0; aph ^= 1; }
+        }
+    } else {                                                      // ---- results
+        int acc = 0, buf = 0;
+        uint32_t aph = 0;
+        TO* out = static_cast<TO*>(p.out);
+        unsigned char* slab = slabs + warp * 2 * SLAB;
+        for (int t = blockIdx.x; t < total; t += gridDim.x) {
+            const Tile k = find_tile<MODE, BN, EB>(p, prefix, t);
+            const int64_t row = (MODE == WEIGHT_GRAD ? k.mrow : k.row) + warp * 32;     // this warp's first row
+            const int64_t end = MODE == WEIGHT_GRAD ? p.rows_m : k.end;
+            float sr = 1.0f;
+            if constexpr (EB == 1 && MODE == FORWARD) sr = row + lane < end ? __ldg(p.a_scale + row + lane) : 0.0f;
+            if (!wait(done + acc, aph, gone)) break;
+            tc::fence_after_sync();
+            const uint32_t d = tmem + acc * P::ACC_COLS + ((uint32_t)(warp * 32) << 16);
+            const bool none = MODE == WEIGHT_GRAD && k.blocks == 0;
+            if constexpr (MODE == FEW_ROWS) {
+                // a lane is an output column, a column of the accumulator a row
+                const int col = k.col + warp * 32 + lane;
+                const int rows = (int)min((int64_t)BN, k.end - k.row);
+                float sc = 1.0f;
+                if constexpr (EB == 1) sc = col < p.cols ? __ldg(p.b_scale + (int64_t)k.e * p.cols + col) : 0.0f;
+#pragma unroll
+                for (int c = 0; c < BN; c += 16) {
+                    if (c >= rows) break;
+                    float v[16];
+                    tc::tmem_ld16(d + c, v);
+                    tc::tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (c + j < rows && col < p.cols) {
+                            if constexpr (EB == 1) v[j] *= sc * __ldg(p.a_scale + k.row + c + j);
+                            out[(k.row + c + j) * p.cols + col] = from_f<TO>(v[j]);
+                        }
+                }
+            } else {
+                constexpr int W = 128 / (int)sizeof(TO);                  // output columns of a slab
+                const int live = (int)max((int64_t)0, min((int64_t)32, end - row));
+                for (int c = 0; c < BN; c += W) {
+                    const int col = k.col + c;
+                    if (col >= p.cols || live == 0) break;
+                    uint32_t pk[32];
+                    if constexpr (sizeof(TO) == 2) {
+                        uint32_t v[2][32];
+                        tmem_ld32(d + c, v[0]);
+                        tmem_ld32(d + c + 32, v[1]);
+                        tc::tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            float x = __uint_as_float(v[j >> 4][(2 * j) & 31]), y = __uint_as_float(v[j >> 4][(2 * j + 1) & 31]);
+                            if constexpr (EB == 1) {
+                                const int64_t at = (int64_t)k.e * p.cols + col + 2 * j;
+                                x *= sr * (col + 2 * j < p.cols ? __ldg(p.b_scale + at) : 0.0f);
+                                y *= sr * (col + 2 * j + 1 < p.cols ? __ldg(p.b_scale + at + 1) : 0.0f);
+                            }
+                            pk[j] = none ? 0u : pack2<TO>(x, y);
+                        }
+                    } else {
+                        tmem_ld32(d + c, pk);
+                        tc::tmem_wait_ld();
+                        if (none)
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) pk[j] = 0u;
+                    }
+                    // the slab's previous store has been read out of shared memory
+                    if (lane == 0) bulk_wait_read<1>();
+                    __syncwarp();
+                    unsigned char* sl = slab + buf * SLAB;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        *reinterpret_cast<uint4*>(sl + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                            make_uint4(pk[4 * j], pk[4 * j + 1], pk[4 * j + 2], pk[4 * j + 3]);
+                    if (p.tma_out && (MODE == WEIGHT_GRAD || live == 32)) {
+                        tc::fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if constexpr (MODE == WEIGHT_GRAD) tma_store3(&mo, col, (int)row, k.e, tc::smem_u32(sl));
+                            else tma_store2(&mo, col, (int)row, tc::smem_u32(sl));
+                        }
+                    } else {
+                        __syncwarp();
+                        TO* o = out + (MODE == WEIGHT_GRAD ? (int64_t)k.e * p.rows_m * p.cols : 0) + row * p.cols + col;
+                        const int cols = min(W, p.cols - col);
+                        if (p.tma_out) {                          // rows are multiples of 16 bytes
+                            for (int i = lane; i < live * 8; i += 32) {
+                                const int r = i >> 3, j = i & 7;
+                                if (j * (16 / (int)sizeof(TO)) < cols)
+                                    *reinterpret_cast<uint4*>(o + (int64_t)r * p.cols + j * (16 / (int)sizeof(TO))) =
+                                        *reinterpret_cast<const uint4*>(sl + r * 128 + ((j ^ (r & 7)) << 4));
+                            }
+                        } else {
+                            for (int r = 0; r < live; ++r)
+                                for (int j = lane; j < cols; j += 32) {
+                                    const int byte = j * (int)sizeof(TO);
+                                    o[(int64_t)r * p.cols + j] = *reinterpret_cast<const TO*>(
+                                        sl + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15));
+                                }
+                        }
+                        __syncwarp();
+                    }
+                    if (lane == 0) bulk_commit();
+                    buf ^= 1;
+                }
+            }
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) arrive(freed + acc);
+            if (++acc == 2) { acc = 0; aph ^= 1; }
+        }
+        if (lane == 0) bulk_wait_read<0>();
+        if constexpr (MODE != WEIGHT_GRAD) {                      // rows of no expert
+            int64_t b, last;
+            expert_rows(p, p.experts - 1, b, last);
+            const int64_t count = (p.n - last) * p.cols;
+            for (int64_t i = (int64_t)blockIdx.x * (32 * EPI_WARPS) + threadIdx.x; i < count;
+                 i += (int64_t)gridDim.x * (32 * EPI_WARPS))
+                out[last * p.cols + i] = from_f<TO>(0.0f);
+        }
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    if (warp == EPI_WARPS + 1) {
+        tc::fence_after_sync();
+        tc::tmem_dealloc(tmem, P::TMEM_COLS);
+    }
+}
+
+// Rows of `cols` elements copied to rows of `ld` elements (zeros after the columns): operands whose rows
+// are no multiples of 16 bytes, which TMA cannot read.
+template <typename T>
+__global__ void __launch_bounds__(256) pad_rows_kernel(const T* __restrict__ src, int64_t src_ld, T* __restrict__ dst,
+                                                       int64_t rows, int cols, int ld) {
+    const int64_t count = rows * ld;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < count; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t r = i / ld;
+        const int c = (int)(i - r * ld);
+        dst[i] = c < cols ? src[r * src_ld + c] : T(0);
+    }
+}
+
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                            const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                            CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+Encode encoder() {
+    static const Encode f = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<Encode>(p);
+    }();
+    return f;
+}
+
+CUtensorMapDataType map_type(int dtype) {
+    return dtype == FFN_E4M3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+         : dtype == FFN_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+         : dtype == FFN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+}
+size_t type_size(int dtype) { return dtype == FFN_E4M3 ? 1 : dtype == FFN_F32 ? 4 : 2; }
+
+// A map of [planes][rows][cols] with rows ld elements apart (planes 0: a matrix), boxes of 128 bytes x box_rows.
+bool make_map(CUtensorMap* m, const void* p, int dtype, int64_t cols, int64_t rows, int64_t ld, int64_t planes, int box_rows) {
+    const size_t z = type_size(dtype);
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)(planes ? planes : 1)};
+    const cuuint64_t strides[2] = {(cuuint64_t)(ld * z), (cuuint64_t)(rows * ld * z)};
+    const cuuint32_t box[3] = {(cuuint32_t)(128 / z), (cuuint32_t)box_rows, 1}, unit[3] = {1, 1, 1};
+    return encoder() && encoder()(m, map_type(dtype), planes ? 3 : 2, const_cast<void*>(p), dims, strides, box, unit,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// An operand as TMA can read it: as it is, or copied to padded rows.
+struct Operand { const void* p; int64_t ld; };
+
+bool readable(const void* p, int64_t ld, int dtype) { return op_aligned(p, 16) && ld * (int64_t)type_size(dtype) % 16 == 0; }
+int padded(int cols, int dtype) {
+    const int unit = 16 / (int)type_size(dtype);
+    return (cols + unit - 1) / unit * unit;
+}
+uint64_t pad_bytes(const void* p, int64_t ld, int64_t rows, int cols, int dtype) {
+    return readable(p, ld, dtype) ? 0 : ((uint64_t)rows * padded(cols, dtype) * type_size(dtype) + 255) / 256 * 256;
+}
+Operand pad(const void* p, int64_t ld, int64_t rows, int cols, int dtype, unsigned char*& ws, int sms, cudaStream_t st) {
+    if (readable(p, ld, dtype)) return {p, ld};
+    const int to = padded(cols, dtype);
+    const int64_t count = rows * to;
+    const int blocks = (int)((count + 255) / 256 < (int64_t)sms * 16 ? (count + 255) / 256 : (int64_t)sms * 16);
+    if (dtype == FFN_E4M3)
+        pad_rows_kernel<uint8_t><<<blocks, 256, 0, st>>>(static_cast<const uint8_t*>(p), ld, ws, rows, cols, to);
+    else
+        pad_rows_kernel<uint16_t><<<blocks, 256, 0, st>>>(static_cast<const uint16_t*>(p), ld,
+                                                          reinterpret_cast<uint16_t*>(ws), rows, cols, to);
+    const Operand o{ws, to};
+    ws += pad_bytes(p, ld, rows, cols, dtype);
+    return o;
+}
+
+template <int MODE, int BN, int EB, typename TO, bool BF>
+int launch(const Args& a0, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, int sms, cudaStream_t st) {
+    using P = Plan<MODE, BN, EB>;
+    Args a = a0;
+    constexpr int NT = MODE == FEW_ROWS ? BM : BN, RT = MODE == FEW_ROWS ? BN : BM;
+    a.ntiles = (a.cols + NT - 1) / NT;
+    a.mtiles = (a.rows_m + BM - 1) / BM;
+    // an upper bound of the tiles: the counts are on the device
+    const int64_t tiles = MODE == WEIGHT_GRAD ? (int64_t)a.experts * a.ntiles * a.mtiles
+                                              : (a.n / RT + a.experts) * (int64_t)a.ntiles;
+    if (tiles > 0x7fffffff) return op_fail(FFN_E_CAPACITY, "ffn_expert_mm: more than 2^31 output tiles");
+    auto k = experts_kernel<MODE, BN, EB, TO, BF>;
+    static std::atomic<uint64_t> ready{0};            // devices whose limit is set
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev > 63 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {
+        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::BYTES);
+        if (e != cudaSuccess) return op_fail(FFN_E_CUDA, std::string("ffn_expert_mm: ") + cudaGetErrorString(e));
+        if (dev <= 63) ready.fetch_or(1ull << dev, std::memory_order_release);
+    }
+    k<<<(unsigned)(tiles < sms ? tiles : sms), THREADS, P::BYTES, st>>>(a, ma, mb, mo);
+    return op_launched("ffn_expert_mm");
+}
+
+template <int MODE, int BN>
+int launch_typed(const Args& a, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, int dtype, int out_dtype,
+                 int sms, cudaStream_t st) {
+    if constexpr (MODE == FORWARD || MODE == FEW_ROWS) {
+        if (dtype == FFN_E4M3)
+            return out_dtype == FFN_F16 ? launch<MODE, BN, 1, __half, false>(a, ma, mb, mo, sms, st)
+                                        : launch<MODE, BN, 1, __nv_bfloat16, false>(a, ma, mb, mo, sms, st);
+    }
+    if constexpr (MODE == WEIGHT_GRAD) {
+        if (out_dtype == FFN_F32)
+            return dtype == FFN_F16 ? launch<MODE, BN, 2, float, false>(a, ma, mb, mo, sms, st)
+                                    : launch<MODE, BN, 2, float, true>(a, ma, mb, mo, sms, st);
+    }
+    return dtype == FFN_F16 ? launch<MODE, BN, 2, __half, false>(a, ma, mb, mo, sms, st)
+                            : launch<MODE, BN, 2, __nv_bfloat16, true>(a, ma, mb, mo, sms, st);
+}
+
+int bad_map() { return op_fail(FFN_E_CUDA, "ffn_expert_mm: a tensor map could not be made"); }
+
+// Width of a tile: the widest that the output's width fills.
+int tile_width(int cols) { return cols > 128 ? 256 : cols > 64 ? 128 : 64; }
+
+// out[r] = a[r] b[e]^T (FORWARD, FEW_ROWS) or a[r] b[e] (INPUT_GRAD); depth and cols are those of the product.
+int rows_product(int mode, Operand a, Operand b, const float* a_scale, const float* b_scale, const int32_t* offsets, void* out,
+                 int64_t n, int experts, int depth, int cols, int dtype, int out_dtype, int sms, cudaStream_t st) {
+    Args p{offsets, a_scale, b_scale, out, n, experts, cols, depth, 0, 0, 0, 0};
+    p.tma_out = op_aligned(out, 16) && (int64_t)cols * 2 % 16 == 0;
+    CUtensorMap ma, mb, mo{};
+    if (mode == FEW_ROWS) {
+        const int64_t average = n / experts;
+        const int bn = average <= 12 ? 16 : average <= 24 ? 32 : 64;
+        if (!make_map(&ma, b.p, dtype, depth, cols, b.ld, experts, BM) || !make_map(&mb, a.p, dtype, depth, n, a.ld, 0, bn))
+            return bad_map();
+        return bn == 16 ? launch_typed<FEW_ROWS, 16>(p, ma, mb, mo, dtype, out_dtype, sms, st)
+             : bn == 32 ? launch_typed<FEW_ROWS, 32>(p, ma, mb, mo, dtype, out_dtype, sms, st)
+                        : launch_typed<FEW_ROWS, 64>(p, ma, mb, mo, dtype, out_dtype, sms, st);
+    }
+    const int bn = tile_width(cols);
+    if (p.tma_out && !make_map(&mo, out, out_dtype, cols, n, cols, 0, 32)) return bad_map();
+    if (!make_map(&ma, a.p, dtype, depth, n, a.ld, 0, BM)) return bad_map();
+    if (mode == FORWARD) {
+        if (!make_map(&mb, b.p, dtype, depth, cols, b.ld, experts, bn)) return bad_map();
+        return bn == 256 ? launch_typed<FORWARD, 256>(p, ma, mb, mo, dtype, out_dtype, sms, st)
+             : bn == 128 ? launch_typed<FORWARD, 128>(p, ma, mb, mo, dtype, out_dtype, sms, st)
+                         : launch_typed<FORWARD, 64>(p, ma, mb, mo, dtype, out_dtype, sms, st);
+    }
+    if (!make_map(&mb, b.p, dtype, cols, depth, b.ld, experts, 64)) return bad_map();
+    return bn == 256 ? launch_typed<INPUT_GRAD, 256>(p, ma, mb, mo, dtype, out_dtype, sms, st)
+         : bn == 128 ? launch_typed<INPUT_GRAD, 128>(p, ma, mb, mo, dtype, out_dtype, sms, st)
+                     : launch_typed<INPUT_GRAD, 64>(p, ma, mb, mo, dtype, out_dtype, sms, st);
+}
+
+int weight_product(Operand dy, Operand x, const int32_t* offsets, void* dw, int64_t n, int experts, int k, int m, int dtype,
+                   int dw_dtype, int sms, cudaStream_t st) {
+    Args p{offsets, nullptr, nullptr, dw, n, experts, k, 0, m, 0, 0, 0};
+    p.tma_out = op_aligned(dw, 16) && (int64_t)k * (int64_t)type_size(dw_dtype) % 16 == 0;
+    CUtensorMap ma, mb, mo{};
+    if (p.tma_out && !make_map(&mo, dw, dw_dtype, k, m, k, experts, 32)) return bad_map();
+    if (!make_map(&ma, dy.p, dtype, m, n, dy.ld, 0, 64) || !make_map(&mb, x.p, dtype, k, n, x.ld, 0, 64)) return bad_map();
+    const int bn = tile_width(k);
+    return bn == 256 ? launch_typed<WEIGHT_GRAD, 256>(p, ma, mb, mo, dtype, dw_dtype, sms, st)
+         : bn == 128 ? launch_typed<WEIGHT_GRAD, 128>(p, ma, mb, mo, dtype, dw_dtype, sms, st)
+                     : launch_typed<WEIGHT_GRAD, 64>(p, ma, mb, mo, dtype, dw_dtype, sms, st);
 }
 
 int check(const char* who, int64_t n, int32_t experts, int32_t k, int32_t m) {
@@ -97,10 +651,14 @@ using namespace ffn;
 
 extern "C" {
 
+uint64_t ffn_expert_mm_workspace(const void* x, int64_t x_ld, const void* w, int64_t n, int32_t experts, int32_t k, int32_t m,
+                                 int dtype) {
+    return pad_bytes(x, x_ld, n, k, dtype) + pad_bytes(w, k, (int64_t)experts * m, k, dtype);
+}
+
 int ffn_expert_mm(const void* x, int64_t x_ld, const void* w, const int32_t* offsets, const float* x_scale,
                   const float* w_scale, void* y, int64_t n, int32_t experts, int32_t k, int32_t m, int dtype,
                   int out_dtype, void* workspace, uint64_t workspace_bytes, void* stream) {
-    (void)workspace; (void)workspace_bytes;
     if (int rc = check("ffn_expert_mm", n, experts, k, m)) return rc;
     if (dtype == FFN_E4M3 ? (out_dtype != FFN_F16 && out_dtype != FFN_BF16)
                           : ((dtype != FFN_F16 && dtype != FFN_BF16) || out_dtype != dtype))
@@ -111,51 +669,70 @@ int ffn_expert_mm(const void* x, int64_t x_ld, const void* w, const int32_t* off
     if (n == 0) return FFN_OK;
     if (!x || !w || !offsets || !y) return op_fail(FFN_E_CONFIG, "ffn_expert_mm: a required pointer is NULL");
     if (x_ld < k) return op_fail(FFN_E_CONFIG, "ffn_expert_mm: the row stride is below k");
-    Plain p{x, w, y, x_scale, w_scale, offsets, n, x_ld, 1, k, 1, (int64_t)m * k, m, 0, 0, m, k, experts, 0};
+    if (workspace_bytes < ffn_expert_mm_workspace(x, x_ld, w, n, experts, k, m, dtype) || !op_aligned(workspace, 16))
+        return op_fail(FFN_E_CAPACITY, "ffn_expert_mm: the workspace is smaller than ffn_expert_mm_workspace says, or not "
+                                       "16-byte aligned");
+    const int sms = op_sms();
+    if (sms <= 0) return op_fail(FFN_E_CUDA, "no CUDA device");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const dim3 grid((unsigned)((n + 63) / 64 + experts + 1), (unsigned)((m + 63) / 64));
-    if (dtype == FFN_F16) experts_plain_kernel<__half, __half><<<grid, 256, 0, st>>>(p);
-    else if (dtype == FFN_BF16) experts_plain_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, 256, 0, st>>>(p);
-    else if (out_dtype == FFN_F16) experts_plain_kernel<__nv_fp8_e4m3, __half><<<grid, 256, 0, st>>>(p);
-    else experts_plain_kernel<__nv_fp8_e4m3, __nv_bfloat16><<<grid, 256, 0, st>>>(p);
-    return op_launched("ffn_expert_mm");
+    unsigned char* ws = static_cast<unsigned char*>(workspace);
+    const Operand a = pad(x, x_ld, n, k, dtype, ws, sms, st), b = pad(w, k, (int64_t)experts * m, k, dtype, ws, sms, st);
+    const int mode = n <= (int64_t)experts * 48 ? FEW_ROWS : FORWARD;
+    return rows_product(mode, a, b, x_scale, w_scale, offsets, y, n, experts, k, m, dtype, out_dtype, sms, st);
 }
 
-uint64_t ffn_expert_mm_workspace(const void*, int64_t, const void*, int64_t, int32_t, int32_t, int32_t, int) { return 0; }
-
-uint64_t ffn_expert_mm_bwd_workspace(const void*, int64_t, const void*, int64_t, const void*, int64_t, int32_t, int32_t,
-                                     int32_t, int) { return 0; }
+uint64_t ffn_expert_mm_bwd_workspace(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, const void* w, int64_t n,
+                                     int32_t experts, int32_t k, int32_t m, int dtype) {
+    return pad_bytes(dy, dy_ld, n, m, dtype) + pad_bytes(x, x_ld, n, k, dtype) +
+           pad_bytes(w, k, (int64_t)experts * m, k, dtype);
+}
 
 int ffn_expert_mm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, const void* w, const int32_t* offsets,
                       void* dx, void* dw, int64_t n, int32_t experts, int32_t k, int32_t m, int dtype, int dw_dtype,
                       void* workspace, uint64_t workspace_bytes, void* stream) {
-    (void)workspace; (void)workspace_bytes;
     if (int rc = check("ffn_expert_mm_bwd", n, experts, k, m)) return rc;
     if (dtype != FFN_F16 && dtype != FFN_BF16)
         return op_fail(FFN_E_CONFIG, "ffn_expert_mm_bwd: dtype must be FFN_F16 or FFN_BF16");
     if (dw_dtype != dtype && dw_dtype != FFN_F32)
         return op_fail(FFN_E_CONFIG, "ffn_expert_mm_bwd: dw_dtype must be dtype or FFN_F32");
     if (!dx && !dw) return FFN_OK;
-    if (!offsets || (n > 0 && (!dy || !x || !w)))
-        return op_fail(FFN_E_CONFIG, "ffn_expert_mm_bwd: a required pointer is NULL");
-    if (dy_ld < m || x_ld < k) return op_fail(FFN_E_CONFIG, "ffn_expert_mm_bwd: a row stride is below the columns");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dx && n > 0) {
-        Plain p{dy, w, dx, nullptr, nullptr, offsets, n, dy_ld, 1, 1, k, (int64_t)m * k, k, 0, 0, k, m, experts, 0};
-        const dim3 grid((unsigned)((n + 63) / 64 + experts + 1), (unsigned)((k + 63) / 64));
-        if (dtype == FFN_F16) experts_plain_kernel<__half, __half><<<grid, 256, 0, st>>>(p);
-        else experts_plain_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, 256, 0, st>>>(p);
+    if (n == 0) {
+        if (!dw) return FFN_OK;
+        const cudaError_t e = cudaMemsetAsync(dw, 0, (size_t)experts * m * k * type_size(dw_dtype), st);
+        return e == cudaSuccess ? FFN_OK : op_fail(FFN_E_CUDA, std::string("ffn_expert_mm_bwd: ") + cudaGetErrorString(e));
+    }
+    if (!offsets || !dy || !x || !w) return op_fail(FFN_E_CONFIG, "ffn_expert_mm_bwd: a required pointer is NULL");
+    if (dy_ld < m || x_ld < k) return op_fail(FFN_E_CONFIG, "ffn_expert_mm_bwd: a row stride is below the columns");
+    if (workspace_bytes < ffn_expert_mm_bwd_workspace(dy, dy_ld, x, x_ld, w, n, experts, k, m, dtype) ||
+        !op_aligned(workspace, 16))
+        return op_fail(FFN_E_CAPACITY, "ffn_expert_mm_bwd: the workspace is smaller than ffn_expert_mm_bwd_workspace says, or "
+                                       "not 16-byte aligned");
+    const int sms = op_sms();
+    if (sms <= 0) return op_fail(FFN_E_CUDA, "no CUDA device");
+    unsigned char* ws = static_cast<unsigned char*>(workspace);
+    const Operand a = pad(dy, dy_ld, n, m, dtype, ws, sms, st);
+    if (dx) {
+        const Operand b = pad(w, k, (int64_t)experts * m, k, dtype, ws, sms, st);
+        if (int rc = rows_product(INPUT_GRAD, a, b, nullptr, nullptr, offsets, dx, n, experts, m, k, dtype, dtype, sms, st))
+            return rc;
     }
     if (dw) {
-        Plain p{dy, x, dw, nullptr, nullptr, offsets, n, 1, dy_ld, 1, x_ld, 0, k, (int64_t)m * k, m, k, 0, experts, 1};
-        const dim3 grid((unsigned)((m + 63) / 64), (unsigned)((k + 63) / 64), (unsigned)experts);
-        if (dw_dtype == FFN_F32) {
-            if (dtype == FFN_F16) experts_plain_kernel<__half, float><<<grid, 256, 0, st>>>(p);
-            else experts_plain_kernel<__nv_bfloat16, float><<<grid, 256, 0, st>>>(p);
-        } else if (dtype == FFN_F16) experts_plain_kernel<__half, __half><<<grid, 256, 0, st>>>(p);
-        else experts_plain_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, 256, 0, st>>>(p);
+        const Operand b = pad(x, x_ld, n, k, dtype, ws, sms, st);
+        if (int rc = weight_product(a, b, offsets, dw, n, experts, k, m, dtype, dw_dtype, sms, st)) return rc;
     }
-    return op_launched("ffn_expert_mm_bwd");
+    return FFN_OK;
+}
+
+int ffn_ops_status(uint32_t* status) {
+    if (!status) return op_fail(FFN_E_CONFIG, "ffn_ops_status: status is NULL");
+    int v = 0;
+    cudaError_t e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&v, g_status, sizeof v);
+    const int zero = 0;
+    if (e == cudaSuccess && v) e = cudaMemcpyToSymbol(g_status, &zero, sizeof zero);
+    *status = (uint32_t)v;
+    return e == cudaSuccess ? FFN_OK : op_fail(FFN_E_CUDA, std::string("ffn_ops_status: ") + cudaGetErrorString(e));
 }
 
 }  // extern "C"

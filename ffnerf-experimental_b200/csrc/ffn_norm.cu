@@ -12,8 +12,9 @@
 // is the bound.  A row therefore stays in the registers of the threads that loaded it: `tpr` lanes of
 // a warp where the row has at most 32 lanes x NV vectors of 16 bytes (so a 64-wide row takes 8 lanes
 // and a warp takes four rows; no barrier), a whole block above that.  Statistics are fp32.  y is
-// formed from the unrounded fp32 sum x + r; the h that is written for the residual stream and for the
-// backward pass is rounded to the stream's type.
+// formed from the unrounded fp32 sum x + r; the h that is written for the residual stream is rounded to
+// the stream's type.  The backward pass forms the same fp32 sum again: from the rounded h its dg, an fp32
+// sum over rows, would be off by the stream's rounding (1.7e-3 of it in bf16 against 2e-7).
 #include "ffn_ops.cuh"
 
 namespace ffn {
@@ -28,9 +29,9 @@ struct NormArgs {
 };
 
 struct NormBwdArgs {
-    const void* dy; const void* h; const void* dres; const float* gamma; const float* rstd;
+    const void* dy; const void* x; const void* res; const void* dres; const float* gamma; const float* rstd;
     void* dx; float* partial;
-    int64_t n, dy_ld, h_ld, dres_ld;
+    int64_t n, dy_ld, x_ld, res_ld, dres_ld;
     int d, tpr;
 };
 
@@ -208,7 +209,8 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 256) rmsnorm_bwd_kernel(const No
     const int sub = BLOCK ? 0 : (int)threadIdx.x / tpr;
     const float inv_d = 1.0f / (float)a.d;
     const T* dyp = static_cast<const T*>(a.dy);
-    const T* hp = static_cast<const T*>(a.h);
+    const T* xp = static_cast<const T*>(a.x);
+    const T* rp = static_cast<const T*>(a.res);
     const T* drp = static_cast<const T*>(a.dres);
     float dg[NV][VEC];
 #pragma unroll
@@ -219,16 +221,21 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 256) rmsnorm_bwd_kernel(const No
         const int64_t row = base + sub;
         const bool live = row < a.n;
         const float s = live ? __ldg(a.rstd + row) : 0.0f;
-        Pack<T, VEC> pd[NV], ph[NV], pr[NV];
+        Pack<T, VEC> pd[NV], pr[NV];
+        float v[NV][VEC];                                        // h, then xhat
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (lane + i * tpr) * VEC;
-            pd[i] = Pack<T, VEC>{}; ph[i] = Pack<T, VEC>{}; pr[i] = Pack<T, VEC>{};
+            Pack<T, VEC> px{}, pq{};
+            pd[i] = Pack<T, VEC>{}; pr[i] = Pack<T, VEC>{};
             if (live && c < a.d) {
                 pd[i] = load_pack<T, VEC>(dyp + row * a.dy_ld + c);
-                ph[i] = load_pack<T, VEC>(hp + row * a.h_ld + c);
+                px = load_pack<T, VEC>(xp + row * a.x_ld + c);
+                if (rp) pq = load_pack<T, VEC>(rp + row * a.res_ld + c);
                 if (drp) pr[i] = load_pack<T, VEC>(drp + row * a.dres_ld + c);
             }
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[i][j] = (to_f(px.v[j]) + (rp ? to_f(pq.v[j]) : 0.0f)) * s;
         }
         float dot = 0.0f;
 #pragma unroll
@@ -237,9 +244,9 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 256) rmsnorm_bwd_kernel(const No
             if (live && c < a.d)
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    const float xh = to_f(ph[i].v[j]) * s, dy = to_f(pd[i].v[j]);
-                    dg[i][j] = fmaf(dy, xh, dg[i][j]);
-                    dot = fmaf(dy * __ldg(a.gamma + c + j), xh, dot);
+                    const float dy = to_f(pd[i].v[j]);
+                    dg[i][j] = fmaf(dy, v[i][j], dg[i][j]);
+                    dot = fmaf(dy * __ldg(a.gamma + c + j), v[i][j], dot);
                 }
         }
         dot = row_reduce<BLOCK, false>(dot, tpr, sh) * inv_d;
@@ -250,8 +257,8 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 256) rmsnorm_bwd_kernel(const No
                 Pack<T, VEC> p;
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    const float xh = to_f(ph[i].v[j]) * s, u = to_f(pd[i].v[j]) * __ldg(a.gamma + c + j);
-                    p.v[j] = from_f<T>(fmaf(s, fmaf(-xh, dot, u), drp ? to_f(pr[i].v[j]) : 0.0f));
+                    const float u = to_f(pd[i].v[j]) * __ldg(a.gamma + c + j);
+                    p.v[j] = from_f<T>(fmaf(s, fmaf(-v[i][j], dot, u), drp ? to_f(pr[i].v[j]) : 0.0f));
                 }
                 store_pack<T, VEC>(static_cast<T*>(a.dx) + row * a.d + c, p);
             }
@@ -296,18 +303,20 @@ __global__ void __launch_bounds__(256) rmsnorm_bwd_long_kernel(const NormBwdArgs
     for (int c = threadIdx.x; c < a.d; c += blockDim.x) out[c] = 0.0f;
     for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
         const T* dy = static_cast<const T*>(a.dy) + row * a.dy_ld;
-        const T* h = static_cast<const T*>(a.h) + row * a.h_ld;
+        const T* x = static_cast<const T*>(a.x) + row * a.x_ld;
+        const T* res = a.res ? static_cast<const T*>(a.res) + row * a.res_ld : nullptr;
+        auto at = [&](int c) { return to_f(x[c]) + (res ? to_f(res[c]) : 0.0f); };
         const T* dr = a.dres ? static_cast<const T*>(a.dres) + row * a.dres_ld : nullptr;
         const float s = a.rstd[row];
         float dot = 0.0f;
         for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
-            const float t = to_f(dy[c]) * (to_f(h[c]) * s);
+            const float t = to_f(dy[c]) * (at(c) * s);
             out[c] += t;
             dot = fmaf(t, a.gamma[c], dot);
         }
         dot = row_reduce<true, false>(dot, 0, sh) * inv_d;
         for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
-            const float u = to_f(dy[c]) * a.gamma[c], xh = to_f(h[c]) * s;
+            const float u = to_f(dy[c]) * a.gamma[c], xh = at(c) * s;
             static_cast<T*>(a.dx)[row * a.d + c] = from_f<T>(fmaf(s, fmaf(-xh, dot, u), dr ? to_f(dr[c]) : 0.0f));
         }
     }
@@ -461,8 +470,8 @@ uint64_t ffn_rmsnorm_bwd_workspace(int64_t n, int32_t d) {
     return (uint64_t)(n < most ? n : most) * (uint64_t)d * sizeof(float);
 }
 
-int ffn_rmsnorm_bwd(const void* dy, int64_t dy_ld, const void* h, int64_t h_ld, const float* gamma, const float* rstd,
-                    const void* dresidual, int64_t dresidual_ld, void* dx, float* dgamma, void* workspace,
+int ffn_rmsnorm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, const void* residual,
+                    int64_t residual_ld, const float* gamma, const float* rstd, const void* dresidual, int64_t dresidual_ld, void* dx, float* dgamma, void* workspace,
                     uint64_t workspace_bytes, int64_t n, int32_t d, int dtype, void* stream) {
     if (n < 0 || d < 1) return op_fail(FFN_E_CONFIG, "ffn_rmsnorm_bwd: n must be >= 0 and d >= 1");
     if (dtype != FFN_F32 && dtype != FFN_F16 && dtype != FFN_BF16)
@@ -473,16 +482,18 @@ int ffn_rmsnorm_bwd(const void* dy, int64_t dy_ld, const void* h, int64_t h_ld, 
         const cudaError_t e = cudaMemsetAsync(dgamma, 0, (size_t)d * sizeof(float), st);
         return e == cudaSuccess ? FFN_OK : op_fail(FFN_E_CUDA, std::string("ffn_rmsnorm_bwd: ") + cudaGetErrorString(e));
     }
-    if (!dy || !h || !gamma || !rstd || !dx || !workspace)
+    if (!dy || !x || !gamma || !rstd || !dx || !workspace)
         return op_fail(FFN_E_CONFIG, "ffn_rmsnorm_bwd: a required pointer is NULL");
-    if (dy_ld < d || h_ld < d || (dresidual && dresidual_ld < d))
+    if (dy_ld < d || x_ld < d || (residual && residual_ld < d) || (dresidual && dresidual_ld < d))
         return op_fail(FFN_E_CONFIG, "ffn_rmsnorm_bwd: a row stride is below d");
     if (workspace_bytes < ffn_rmsnorm_bwd_workspace(n, d) || !op_aligned(workspace, 4))
         return op_fail(FFN_E_CAPACITY, "ffn_rmsnorm_bwd: the workspace is smaller than ffn_rmsnorm_bwd_workspace says");
     const int vec = dtype == FFN_F32 ? 4 : 8;
-    const bool aligned = d % vec == 0 && dy_ld % vec == 0 && h_ld % vec == 0 && (!dresidual || dresidual_ld % vec == 0) &&
-                         op_aligned(dy, 16) && op_aligned(h, 16) && op_aligned(dresidual, 16) && op_aligned(dx, 16);
-    NormBwdArgs a{dy, h, dresidual, gamma, rstd, dx, static_cast<float*>(workspace), n, dy_ld, h_ld, dresidual_ld, d, 0};
+    const bool aligned = d % vec == 0 && dy_ld % vec == 0 && x_ld % vec == 0 && (!residual || residual_ld % vec == 0) &&
+                         (!dresidual || dresidual_ld % vec == 0) && op_aligned(dy, 16) && op_aligned(x, 16) &&
+                         op_aligned(residual, 16) && op_aligned(dresidual, 16) && op_aligned(dx, 16);
+    NormBwdArgs a{dy, x, residual, dresidual, gamma, rstd, dx, static_cast<float*>(workspace), n,
+                  dy_ld, x_ld, residual_ld, dresidual_ld, d, 0};
     if (dtype == FFN_F32) return norm_bwd_launch<float>(a, dgamma, aligned, st);
     if (dtype == FFN_F16) return norm_bwd_launch<__half>(a, dgamma, aligned, st);
     return norm_bwd_launch<__nv_bfloat16>(a, dgamma, aligned, st);

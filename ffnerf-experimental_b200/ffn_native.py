@@ -93,7 +93,7 @@ _SIGS = {
     "ffn_rmsnorm": (C.c_int, [_VP, C.c_int64, _VP, C.c_int64] + [_VP] * 5 + [C.c_int64, C.c_int32, C.c_float, C.c_int,
                               C.c_int, C.c_int32, _VP]),
     "ffn_rmsnorm_bwd_workspace": (C.c_uint64, [C.c_int64, C.c_int32]),
-    "ffn_rmsnorm_bwd": (C.c_int, [_VP, C.c_int64, _VP, C.c_int64, _VP, _VP, _VP, C.c_int64, _VP, _VP, _VP, C.c_uint64,
+    "ffn_rmsnorm_bwd": (C.c_int, [_VP, C.c_int64, _VP, C.c_int64, _VP, C.c_int64, _VP, _VP, _VP, C.c_int64, _VP, _VP, _VP, C.c_uint64,
                                   C.c_int64, C.c_int32, C.c_int, _VP]),
     "ffn_gated_scan": (C.c_int, [_VP, C.c_int64, _VP, C.c_int64, _VP, _VP, _VP, _VP, C.c_int64, C.c_int32, C.c_int64,
                                  C.c_int32, C.c_int, C.c_int, C.c_int, _VP]),
@@ -106,6 +106,7 @@ _SIGS = {
                                                  C.c_int32, C.c_int]),
     "ffn_expert_mm_bwd": (C.c_int, [_VP, C.c_int64, _VP, C.c_int64] + [_VP] * 4 + [C.c_int64, C.c_int32, C.c_int32,
                                     C.c_int32, C.c_int, C.c_int, _VP, C.c_uint64, _VP]),
+    "ffn_ops_status": (C.c_int, [C.POINTER(C.c_uint32)]),
 }
 EXPORTED = tuple(_SIGS)
 

@@ -13,6 +13,7 @@ call by the caller.
 from __future__ import annotations
 
 import functools
+from typing import NamedTuple
 
 import torch
 
@@ -106,14 +107,22 @@ def _workspace(device, name: str, *args):
 
 
 # ---------------------------------------------------------------------------------------- RMS norm
+class NormState(NamedTuple):
+    """What the backward pass of ``rmsnorm`` needs: the row factors (float32 [n]) and the inputs."""
+    rstd: torch.Tensor
+    x: torch.Tensor
+    residual: torch.Tensor | None
+
+
 @_streamed
 def rmsnorm(x, gamma, residual=None, eps: float = 1e-6, out: str = "same", group: int = 0):
-    """RMS norm of ``x + residual`` over the columns: returns ``(y, h, rstd, scale)``.
+    """RMS norm of ``x + residual`` over the columns: returns ``(y, h, state, scale)``.
 
     x, residual [n, d] (float32, float16 or bfloat16; rows may be strided), gamma [d] float32.  y is in
     x's type, or (``out="e4m3"``) float8_e4m3fn with float32 ``scale`` [n], or [n, d / group] for
-    ``group`` 32, 64 or 128; value = y * scale.  h is the sum (x itself without a residual) and rstd
-    [n] the row factors: what ``rmsnorm_bwd`` takes.  scale is None for ``out="same"``."""
+    ``group`` 32, 64 or 128; value = y * scale (scale is None for ``out="same"``).  h is the sum in x's
+    type, the residual stream that goes on (x itself without a residual); state is what
+    ``rmsnorm_bwd`` takes."""
     if x.dtype not in _WIDE:
         _bad(f"x must be float32, float16 or bfloat16, got {x.dtype}")
     x_ld = _rows(x, "x")
@@ -137,25 +146,33 @@ def rmsnorm(x, gamma, residual=None, eps: float = 1e-6, out: str = "same", group
     _call("ffn_rmsnorm", dev, x.data_ptr(), x_ld, None if residual is None else residual.data_ptr(), res_ld, g,
           None if residual is None else h.data_ptr(), y.data_ptr(), None if scale is None else scale.data_ptr(),
           rstd.data_ptr(), n, d, eps, DTYPES[dt], code, group)
-    return y, h, rstd, scale
+    return y, h, NormState(rstd, x, residual), scale
 
 
 @_streamed
-def rmsnorm_bwd(dy, h, gamma, rstd, dresidual=None):
-    """Backward pass of ``rmsnorm`` from its h and rstd: returns ``(dx, dgamma)``.  dx (the gradient of x
-    and of the residual alike) includes ``dresidual``, the gradient that reaches h past the norm."""
+def rmsnorm_bwd(dy, h, gamma, state, dresidual=None):
+    """Backward pass of ``rmsnorm``: returns ``(dx, dgamma)``.  dx (the gradient of x and of the residual
+    alike) includes ``dresidual``, the gradient that reaches h past the norm.
+
+    state is the NormState of the forward call; the sum is then formed again from its inputs, unrounded,
+    and h is not read.  A caller who kept only h and the row factors passes the float32 [n] tensor
+    ``state.rstd`` instead: xhat then carries the rounding of h, one array less is read, and x and the
+    residual need not be kept."""
     if dy.dtype not in _WIDE:
         _bad(f"dy must be float32, float16 or bfloat16, got {dy.dtype}")
     dy_ld = _rows(dy, "dy")
     n, d = dy.shape
     dev, dt = dy.device, dy.dtype
-    h_ld = _rows(h, "h", d, n, dt, dev)
+    rstd, x, residual = state if isinstance(state, NormState) else (state, h, None)
+    x_ld = _rows(x, "x", d, n, dt, dev)
+    res_ld = 0 if residual is None else _rows(residual, "residual", d, n, dt, dev)
     dr_ld = 0 if dresidual is None else _rows(dresidual, "dresidual", d, n, dt, dev)
     g, r = _plain(gamma, "gamma", (d,), torch.float32, dev), _plain(rstd, "rstd", (n,), torch.float32, dev)
     dx = torch.empty((n, d), dtype=dt, device=dev)
     dgamma = torch.empty(d, dtype=torch.float32, device=dev)
     ws, p, size = _workspace(dev, "ffn_rmsnorm_bwd_workspace", n, d)
-    _call("ffn_rmsnorm_bwd", dev, dy.data_ptr(), dy_ld, h.data_ptr(), h_ld, g, r,
+    _call("ffn_rmsnorm_bwd", dev, dy.data_ptr(), dy_ld, x.data_ptr(), x_ld,
+          None if residual is None else residual.data_ptr(), res_ld, g, r,
           None if dresidual is None else dresidual.data_ptr(), dr_ld, dx.data_ptr(), dgamma.data_ptr(), p, size, n, d,
           DTYPES[dt])
     return dx, dgamma
@@ -329,3 +346,16 @@ def expert_mm_bwd(dy, x, w, offsets, need_dx: bool = True, need_dw: bool = True,
           None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(), n, e, k, m, code,
           DTYPES[dw_dtype], p, size)
     return dx, dw
+
+
+def status(device=None) -> int:
+    """Status word of the block operators on the current (or given) device since the last call; waits for
+    the device.  0 when every kernel completed normally; ``ffn_native.STATUS_TC_TIMEOUT`` when a wait of
+    an expert product ran out and its results are incomplete."""
+    import ctypes
+    v = ctypes.c_uint32()
+    with torch.cuda.device(device):
+        rc = fn.load_library().ffn_ops_status(ctypes.byref(v))
+    if rc != fn.FFN_OK:
+        raise RuntimeError(f"ffn_ops_status failed ({rc}): {fn.load_library().ffn_last_error(None).decode()}")
+    return int(v.value)

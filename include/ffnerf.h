@@ -310,13 +310,14 @@ enum { FFN_F32 = 0, FFN_F16 = 1, FFN_BF16 = 2, FFN_E4M3 = 3 };
 int ffn_rmsnorm(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, const float* gamma, void* h,
                 void* y, float* scale, float* rstd, int64_t n, int32_t d, float eps, int dtype, int out_dtype,
                 int32_t group, void* stream);
-/* Its backward pass from the saved h and rstd: dx (the gradient of x and of residual alike) =
+/* Its backward pass from the same x and residual and from rstd (a caller who kept only h passes it as x
+ * with residual NULL: xhat then carries h's rounding): dx (the gradient of x and of residual alike) =
  *   rstd * (dy gamma - xhat mean(dy gamma xhat)) + dresidual, xhat = h rstd,
  * and dgamma [d] fp32 = sum over rows of dy xhat, summed in a fixed order.  dresidual (the gradient
  * that reaches h past the norm) may be NULL.  workspace: ffn_rmsnorm_bwd_workspace bytes. */
 uint64_t ffn_rmsnorm_bwd_workspace(int64_t n, int32_t d);
-int ffn_rmsnorm_bwd(const void* dy, int64_t dy_ld, const void* h, int64_t h_ld, const float* gamma, const float* rstd,
-                    const void* dresidual, int64_t dresidual_ld, void* dx, float* dgamma, void* workspace,
+int ffn_rmsnorm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, const void* residual,
+                    int64_t residual_ld, const float* gamma, const float* rstd, const void* dresidual, int64_t dresidual_ld, void* dx, float* dgamma, void* workspace,
                     uint64_t workspace_bytes, int64_t n, int32_t d, int dtype, void* stream);
 
 /* Gated linear recurrence per channel over n_seq sequences packed along the rows:
@@ -349,7 +350,7 @@ int ffn_gated_scan_bwd(const void* dh, int64_t dh_ld, const float* dh_last, cons
  * products' value is x[r] w[e]^T * x_scale[r] * w_scale[e][.]; out_dtype FFN_F16 or FFN_BF16).  Sums are
  * fp32.  The workspace (ffn_expert_mm_workspace bytes, 16-byte aligned; 0 where rows are 16-byte
  * multiples) holds copies of operands whose rows cannot be read in 16-byte units. */
-#define FFN_MAX_EXPERTS 1024
+#define FFN_MAX_EXPERTS 256
 uint64_t ffn_expert_mm_workspace(const void* x, int64_t x_ld, const void* w, int64_t n, int32_t experts, int32_t k,
                                  int32_t m, int dtype);
 int ffn_expert_mm(const void* x, int64_t x_ld, const void* w, const int32_t* offsets, const float* x_scale,
@@ -362,6 +363,11 @@ uint64_t ffn_expert_mm_bwd_workspace(const void* dy, int64_t dy_ld, const void* 
 int ffn_expert_mm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, const void* w, const int32_t* offsets,
                       void* dx, void* dw, int64_t n, int32_t experts, int32_t k, int32_t m, int dtype, int dw_dtype,
                       void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Reads and clears the current device's status word of the block operators (waits for the device): 0
+ * when every kernel completed normally; bit 2 = a wait of an expert product exceeded its bound and the
+ * kernel gave up, its results incomplete. */
+int ffn_ops_status(uint32_t* status);
 
 #ifdef __cplusplus
 }

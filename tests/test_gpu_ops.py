@@ -13,7 +13,8 @@ TYPES = [F32, F16, BF16]
 @pytest.fixture(scope="module")
 def ops():
     import ffn_ops
-    return ffn_ops
+    yield ffn_ops
+    assert ffn_ops.status() == 0     # no kernel of this module gave up a wait
 
 
 def draw(seed, *shape, dtype=F32, scale=1.0):
@@ -38,7 +39,7 @@ NORM_SIZES = [(1, 1), (1, 1024), (3, 8), (5, 64), (33, 100), (7, 1000), (2, 1001
 def test_rmsnorm(ops, n, d, dtype):
     x, r, g = draw(1, n, d, dtype=dtype, scale=3), draw(2, n, d, dtype=dtype), 1 + 0.3 * draw(3, d)
     for res in (None, r):
-        y, h, rstd, scale = ops.rmsnorm(x, g, res, eps=1e-5)
+        y, h, (rstd, *_), scale = ops.rmsnorm(x, g, res, eps=1e-5)
         assert scale is None and y.dtype is dtype and (res is not None or h is x)
         h64, s64, y64 = o64.norm(x.cpu(), g.cpu(), None if res is None else res.cpu(), 1e-5)
         rel = o64.norm_rel(d)
@@ -94,6 +95,13 @@ def test_rmsnorm_bwd(ops, n, d, dtype):
         o64.within(dg, wg, 2.0 ** -24 * 256 * sg, F32)
         again = ops.rmsnorm_bwd(dy, h, g, rstd, res)
         assert torch.equal(again[1], dg) and torch.equal(again[0], dx)
+    # from the forward pass's inputs: the sum is formed again, unrounded
+    x, r = draw(5, n, d, dtype=dtype), draw(6, n, d, dtype=dtype)
+    _, hs, state, _ = ops.rmsnorm(x, g, r)
+    dx, dg = ops.rmsnorm_bwd(dy, hs, g, state, dr)
+    want, size, wg, sg = o64.norm_bwd(dy.cpu(), x.cpu().double() + r.cpu().double(), g.cpu(), state.rstd.cpu(), dr.cpu())
+    o64.within(dx, want, o64.norm_rel(d) * size, dtype)
+    o64.within(dg, wg, 2.0 ** -24 * 256 * sg, F32)
 
 
 def test_rmsnorm_strides_and_alignment(ops):
@@ -102,15 +110,15 @@ def test_rmsnorm_strides_and_alignment(ops):
     want = ops.rmsnorm(x, g, r)
     for extra in (3, 8):
         got = ops.rmsnorm(strided(x, extra), g, strided(r, extra))
-        for a, b in zip(got[:3], want[:3]):
+        for a, b in zip((*got[:2], got[2].rstd), (*want[:2], want[2].rstd)):
             torch.testing.assert_close(a, b, rtol=2e-3, atol=1e-4)   # another order of the sum, one fp16 rounding
     flat = torch.empty(n * d + 1, dtype=F16, device="cuda")
     off = flat[1:].view(n, d)
     off.copy_(x)
     got = ops.rmsnorm(off, g, r)
     torch.testing.assert_close(got[0], want[0], rtol=2e-3, atol=1e-4)
-    dx, dg = ops.rmsnorm_bwd(strided(x, 8), strided(want[1], 3), g, want[2], strided(r, 5))
-    dx2, dg2 = ops.rmsnorm_bwd(x, want[1], g, want[2], r)
+    dx, dg = ops.rmsnorm_bwd(strided(x, 8), strided(want[1], 3), g, want[2].rstd, strided(r, 5))
+    dx2, dg2 = ops.rmsnorm_bwd(x, want[1], g, want[2].rstd, r)
     torch.testing.assert_close(dx, dx2, rtol=2e-3, atol=1e-3)
     torch.testing.assert_close(dg, dg2, rtol=1e-4, atol=1e-4)
 
@@ -119,8 +127,8 @@ def test_rmsnorm_gradient_against_differences(ops):
     n, d = 11, 96
     x, r, dy, v = (draw(i, n, d) for i in (1, 2, 3, 4))
     g, vg = 1 + 0.3 * draw(5, d), draw(6, d)
-    _, h, rstd, _ = ops.rmsnorm(x, g, r)
-    dx, dg = ops.rmsnorm_bwd(dy, h, g, rstd)
+    _, h, state, _ = ops.rmsnorm(x, g, r)
+    dx, dg = ops.rmsnorm_bwd(dy, h, g, state)
     loss = lambda a, b: float((ops.rmsnorm(a, b, r)[0].double() * dy.double()).sum())  # noqa: E731
     e = 1e-2      # the truncation is e^2 of O(1) terms, the rounding 2^-24 / e of them
     num = (loss(x + e * v, g) - loss(x - e * v, g)) / (2 * e)
@@ -132,9 +140,9 @@ def test_rmsnorm_gradient_against_differences(ops):
 
 def test_rmsnorm_no_rows(ops):
     x, g = torch.empty(0, 32, dtype=BF16, device="cuda"), torch.ones(32, device="cuda")
-    y, h, rstd, _ = ops.rmsnorm(x, g)
-    assert y.shape == (0, 32) and rstd.shape == (0,)
-    dx, dg = ops.rmsnorm_bwd(x, x, g, rstd)
+    y, h, state, _ = ops.rmsnorm(x, g)
+    assert y.shape == (0, 32) and state.rstd.shape == (0,)
+    dx, dg = ops.rmsnorm_bwd(x, x, g, state)
     assert dx.shape == (0, 32) and bool((dg == 0).all())
 
 
