@@ -25,6 +25,9 @@
 // shared memory (within the block) and distributed shared memory (within the cluster), and each thread
 // then enters its part with the state that the maps before it give.  The elements stay in registers in
 // between, so the split costs no second read; no global memory and no waiting on flags is involved.
+#include <initializer_list>
+#include <type_traits>
+#include <utility>
 #include <cooperative_groups.h>
 
 #include "ffn_ops.cuh"
@@ -53,15 +56,17 @@ struct Affine { float p, h; };
 // above 1 over many steps), and inf * 0 would turn a sequence of zeros into NaN.
 __device__ __forceinline__ float apply(const Affine& m, float x) { return x == 0.0f ? m.h : fmaf(m.p, x, m.h); }
 
-// The gate's a and 1 - a from the value in memory.
+// The gate's a and 1 - a from the value in memory.  With e = exp(-g), a = 1 / (1 + e) and 1 - a = e a,
+// so neither cancels; e is held below 2^126, where a has long reached 0 and 1 - a one (min.NaN keeps a NaN).
+// exp2 and the reciprocal are the hardware's approximations (2 and 1 units in the last place).
 template <bool SIG>
 __device__ __forceinline__ void gate_of(float g, float& a, float& na) {
     if constexpr (SIG) {
-        // 1 / (1 + e) with e = exp(-|g|) never overflows; a and 1 - a are both formed without cancellation
-        const float e = __expf(-fabsf(g)), r = __frcp_rn(1.0f + e);
-        a = g >= 0.0f ? r : e * r;
-        na = g >= 0.0f ? e * r : r;
-        if (g != g) { a = g; na = g; }
+        float x = g * -1.4426950408889634f, e;
+        asm("min.NaN.f32 %0, %0, 0f42FC0000;" : "+f"(x));            // 126
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(1.0f + e));
+        na = e * a;
     } else {
         a = g;
         na = 1.0f;
@@ -89,74 +94,113 @@ __device__ __forceinline__ Span span_of(const ScanArgs& a, int seq) {
     return s;
 }
 
-// U steps of C channels: the packed values in memory, and what the scan needs of them.
+// C neighbouring channels as they lie in memory; they stay packed in registers until they are used.
+template <typename T, int C>
+struct Word {
+    typename Raw<sizeof(T) * C>::type r;
+    __device__ __forceinline__ void load(const T* p) { r = __ldg(reinterpret_cast<const decltype(r)*>(p)); }
+    __device__ __forceinline__ float at(int j) const {
+        if constexpr (sizeof(T) == 4) {
+            if constexpr (C == 1) return __uint_as_float(r);
+            else return __uint_as_float(j ? r.y : r.x);
+        } else if constexpr (C == 1) {
+            return to_f(*reinterpret_cast<const T*>(&r));
+        } else {
+            uint32_t w;
+            if constexpr (C == 2) w = r;
+            else w = j < 2 ? r.x : r.y;
+            if constexpr (std::is_same<T, __nv_bfloat16>::value)
+                return __uint_as_float(j & 1 ? w & 0xffff0000u : w << 16);
+            else
+                return __half2float(__ushort_as_half((unsigned short)(j & 1 ? w >> 16 : w & 0xffffu)));
+        }
+    }
+};
+
+// U steps of C channels.
 template <typename T, bool SIG, bool BACK, int C, int U>
 struct Chunk {
-    Pack<T, C> gate[U], value[U], dh[BACK ? U : 1], before[BACK ? U : 1];
+    Word<T, C> gate[U], value[SIG || !BACK ? U : 1], dh[BACK ? U : 1], before[BACK ? U : 1];
 
     __device__ __forceinline__ void load(const ScanArgs& a, const Span& s, int64_t t0, int ch) {
+        const int64_t row = s.first + t0 * s.dir;
+        const T* pg = static_cast<const T*>(a.gate) + row * a.gate_ld + ch;
+        const T* pv = static_cast<const T*>(a.value) + row * a.value_ld + ch;
+        const T* pd = static_cast<const T*>(a.dh) + row * a.dh_ld + ch;
+        const T* pb = static_cast<const T*>(a.h_in) + (row + s.dir) * a.h_ld + ch;
+        const int64_t sg = a.gate_ld * s.dir, sv = a.value_ld * s.dir, sd = a.dh_ld * s.dir, sb = a.h_ld * s.dir;
+        const int left = (int)min(max(s.len - t0, (int64_t)0), (int64_t)(U + 1));
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            if (t0 + i < s.len) {
-                const int64_t row = s.first + (t0 + i) * s.dir;
-                gate[i] = load_pack<T, C>(static_cast<const T*>(a.gate) + row * a.gate_ld + ch);
-                if (SIG || !BACK) value[i] = load_pack<T, C>(static_cast<const T*>(a.value) + row * a.value_ld + ch);
+            if (i < left) {
+                gate[i].load(pg);
+                pg += sg;
+                if constexpr (SIG || !BACK) {
+                    value[i].load(pv);
+                    pv += sv;
+                }
                 if constexpr (BACK) {
-                    dh[i] = load_pack<T, C>(static_cast<const T*>(a.dh) + row * a.dh_ld + ch);
+                    dh[i].load(pd);
+                    pd += sd;
                     // the state before this step: the next row of this walk (the last step's is h0)
-                    if (t0 + i + 1 < s.len)
-                        before[i] = load_pack<T, C>(static_cast<const T*>(a.h_in) + (row + s.dir) * a.h_ld + ch);
+                    if (i + 1 < left) before[i].load(pb);
+                    pb += sb;
                 }
             }
         }
     }
+};
 
-    // The map of step i for channel j (steps beyond the end leave the state alone).
-    __device__ __forceinline__ Affine map(int i, int j, bool on) const {
-        float al, na;
-        gate_of<SIG>(to_f(gate[i].v[j]), al, na);
-        Affine m;
-        m.p = on ? al : 1.0f;
-        if constexpr (BACK) m.h = on ? al * to_f(dh[i].v[j]) : 0.0f;
-        else m.h = on ? (SIG ? na * to_f(value[i].v[j]) : to_f(value[i].v[j])) : 0.0f;
-        return m;
+// One step of C channels in fp32: the map is m -> a m + b (forward) or m -> a (m + b) (backward, b = dh).
+template <bool SIG, bool BACK, int C>
+struct Step {
+    float a[C], na[SIG && BACK ? C : 1], b[C];
+
+    template <typename T, int U>
+    __device__ __forceinline__ void form(const Chunk<T, SIG, BACK, C, U>& k, int i) {
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            float n;
+            gate_of<SIG>(k.gate[i].at(j), a[j], n);
+            if constexpr (BACK) {
+                b[j] = k.dh[i].at(j);
+                if constexpr (SIG) na[j] = n;
+            } else {
+                b[j] = SIG ? n * k.value[i].at(j) : k.value[i].at(j);
+            }
+        }
     }
 
-    // Goes through the steps from `state` and writes the results.
-    __device__ __forceinline__ void finish(const ScanArgs& a, const Span& s, int64_t t0, int ch, int seq,
-                                           float (&state)[C]) const {
+    // Takes the state through the step and writes its results (element offset `at`); last: the walk's last step.
+    template <typename T, int U>
+    __device__ __forceinline__ void take(const ScanArgs& p, const Chunk<T, SIG, BACK, C, U>& k, int i, bool last, int64_t at,
+                                         int64_t seq_at, float (&state)[C]) const {
+        Pack<T, C> o, og;
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-            if (t0 + i >= s.len) break;
-            const int64_t row = s.first + (t0 + i) * s.dir;
-            Pack<T, C> o, og;
-#pragma unroll
-            for (int j = 0; j < C; ++j) {
-                float al, na;
-                gate_of<SIG>(to_f(gate[i].v[j]), al, na);
-                if constexpr (!BACK) {
-                    state[j] = fmaf(al, state[j], SIG ? na * to_f(value[i].v[j]) : to_f(value[i].v[j]));
-                    o.v[j] = from_f<T>(state[j]);
+        for (int j = 0; j < C; ++j) {
+            if constexpr (!BACK) {
+                state[j] = fmaf(a[j], state[j], b[j]);
+                o.v[j] = from_f<T>(state[j]);
+            } else {
+                const float g = b[j] + state[j];
+                float hb;
+                if (!last) hb = k.before[i].at(j);
+                else hb = p.h0 ? __ldg(p.h0 + seq_at + j) : 0.0f;
+                if constexpr (SIG) {
+                    const float gn = g * na[j];
+                    og.v[j] = from_f<T>(gn * a[j] * (hb - k.value[i].at(j)));
+                    o.v[j] = from_f<T>(gn);
                 } else {
-                    const float g = to_f(dh[i].v[j]) + state[j];
-                    float hb;
-                    if (t0 + i + 1 < s.len) hb = to_f(before[i].v[j]);
-                    else hb = a.h0 ? __ldg(a.h0 + (int64_t)seq * a.d + ch + j) : 0.0f;
-                    if constexpr (SIG) {
-                        og.v[j] = from_f<T>(g * (hb - to_f(value[i].v[j])) * al * na);
-                        o.v[j] = from_f<T>(g * na);
-                    } else {
-                        og.v[j] = from_f<T>(g * hb);
-                        o.v[j] = from_f<T>(g);
-                    }
-                    state[j] = al * g;
+                    og.v[j] = from_f<T>(g * hb);
+                    o.v[j] = from_f<T>(g);
                 }
+                state[j] = a[j] * g;
             }
-            if constexpr (!BACK) store_pack<T, C>(static_cast<T*>(a.h) + row * a.d + ch, o);
-            else {
-                store_pack<T, C>(static_cast<T*>(a.dgate) + row * a.d + ch, og);
-                store_pack<T, C>(static_cast<T*>(a.dvalue) + row * a.d + ch, o);
-            }
+        }
+        if constexpr (!BACK) store_pack<T, C>(static_cast<T*>(p.h) + at, o);
+        else {
+            store_pack<T, C>(static_cast<T*>(p.dgate) + at, og);
+            store_pack<T, C>(static_cast<T*>(p.dvalue) + at, o);
         }
     }
 };
@@ -195,31 +239,47 @@ __device__ __forceinline__ void put_state(const ScanArgs& a, int seq, int ch, co
 
 // Enough sequences and channels: one thread goes through a whole sequence.
 template <typename T, bool SIG, bool BACK, int C, int U>
-__global__ void __launch_bounds__(256) scan_kernel(const ScanArgs a) {
+__global__ void __launch_bounds__(256, 2) scan_kernel(const ScanArgs a) {
     const int64_t item = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (item >= a.items) return;
     const int seq = (int)(item / a.groups), ch = (int)(item % a.groups) * C;
     const Span s = span_of<BACK>(a, seq);
     float state[C];
     first_state<BACK, C>(a, seq, ch, state);
+#pragma unroll 1
     for (int64_t t = 0; t < s.len; t += U) {
         Chunk<T, SIG, BACK, C, U> k;
         k.load(a, s, t, ch);
-        k.finish(a, s, t, ch, seq, state);
+        int64_t at = (s.first + t * s.dir) * a.d + ch;
+        const int left = (int)min(s.len - t, (int64_t)(U + 1));
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (i < left) {
+                Step<SIG, BACK, C> f;
+                f.form(k, i);
+                f.take(a, k, i, i + 1 == left, at, (int64_t)seq * a.d + ch, state);
+                at += (int64_t)s.dir * a.d;
+            }
     }
     put_state<C>(a, seq, ch, state);
     clear_outside<T, BACK, C>(a, seq, ch);
 }
 
-constexpr int MAX_WARPS = 8;
+constexpr int WARPS = 8, MOST_RANKS = 8;
 
-// Few sequences and channels: 32 items per cluster, time split over the warps of its blocks.
+// The maps of a lane's C channels.
+template <int C> struct alignas(8 * C) Maps { Affine m[C]; };
+
+// Few sequences and channels: 32 items per cluster, time split over the WARPS warps of its blocks, U steps
+// a warp.  The next chunk's loads are in flight while the maps of this one go round: a block's map is
+// written straight into the shared memory of the cluster's other blocks (warp q writes to block q), so
+// after the one cluster barrier of a turn every read is local.
 template <typename T, bool SIG, bool BACK, int C, int U>
-__global__ void __launch_bounds__(32 * MAX_WARPS) scan_split_kernel(const ScanArgs a) {
+__global__ void __launch_bounds__(32 * WARPS, 2) scan_split_kernel(const ScanArgs a) {
     cg::cluster_group cluster = cg::this_cluster();
-    __shared__ Affine part[2][MAX_WARPS][C][32];      // the maps of this block's parts
-    __shared__ Affine whole[2][C][32];                // their composition, read by the cluster's other blocks
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    __shared__ Maps<C> part[2][WARPS][32];            // the maps of this block's parts
+    __shared__ Maps<C> whole[2][MOST_RANKS][32];      // the maps of the cluster's blocks
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
     const int64_t item = (int64_t)(blockIdx.x / ranks) * 32 + lane;
     const bool live = item < a.items;
@@ -231,82 +291,100 @@ __global__ void __launch_bounds__(32 * MAX_WARPS) scan_split_kernel(const ScanAr
     for (int o = 16; o > 0; o >>= 1) most = max(most, (int64_t)__shfl_xor_sync(0xffffffffu, (long long)most, o));
     float state[C];
     first_state<BACK, C>(a, seq, ch, state);
-    const int64_t stride = (int64_t)U * warps * ranks;
+    if (ranks > 1) cluster.sync();                     // every block runs before its memory is written
+    const int64_t stride = (int64_t)U * WARPS * ranks;
+    int64_t t0 = (int64_t)(rank * WARPS + w) * U;
+    Chunk<T, SIG, BACK, C, U> next;
+    next.load(a, s, t0, ch);
     int buf = 0;
-    for (int64_t base = 0; base < most; base += stride, buf ^= 1) {
-        const int64_t t0 = base + (int64_t)(rank * warps + w) * U;
-        Chunk<T, SIG, BACK, C, U> k;
-        k.load(a, s, t0, ch);
+    for (int64_t base = 0; base < most; base += stride, t0 += stride, buf ^= 1) {
+        const Chunk<T, SIG, BACK, C, U> k = next;
+        Step<SIG, BACK, C> f[BACK ? 1 : U];            // forward: kept for the second walk over the steps
+        const int left = (int)min(max(s.len - t0, (int64_t)0), (int64_t)(U + 1));
+        Maps<C> mine;
 #pragma unroll
-        for (int j = 0; j < C; ++j) {
-            Affine m{1.0f, 0.0f};
+        for (int j = 0; j < C; ++j) mine.m[j] = Affine{1.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < U; ++i) {
-                const Affine n = k.map(i, j, t0 + i < s.len);
-                m.p *= n.p;
-                m.h = fmaf(n.p, m.h, n.h);
-            }
-            part[buf][w][j][lane] = m;
+        for (int i = 0; i < U; ++i) {
+            Step<SIG, BACK, C>& g = f[BACK ? 0 : i];
+            g.form(k, i);
+            if (i < left)                              // steps beyond the end leave the state alone
+#pragma unroll
+                for (int j = 0; j < C; ++j) {
+                    Affine& m = mine.m[j];
+                    m.p *= g.a[j];
+                    m.h = BACK ? g.a[j] * (m.h + g.b[j]) : fmaf(g.a[j], m.h, g.b[j]);
+                }
         }
+        part[buf][w][lane] = mine;
         __syncthreads();
         // the map of the parts of this block before this warp's, and of all of them
-        Affine before[C], all[C];
+        Maps<C> before, all;
 #pragma unroll
-        for (int j = 0; j < C; ++j) {
-            Affine m{1.0f, 0.0f};
-            before[j] = m;
-            for (int q = 0; q < warps; ++q) {
-                if (q == w) before[j] = m;
-                const Affine n = part[buf][q][j][lane];
-                m.p *= n.p;
-                m.h = apply(n, m.h);
+        for (int j = 0; j < C; ++j) all.m[j] = before.m[j] = Affine{1.0f, 0.0f};
+#pragma unroll
+        for (int q = 0; q < WARPS; ++q) {
+            const Maps<C> n = part[buf][q][lane];
+#pragma unroll
+            for (int j = 0; j < C; ++j) {
+                if (q == w) before.m[j] = all.m[j];
+                all.m[j].h = apply(n.m[j], all.m[j].h);
+                all.m[j].p *= n.m[j].p;
             }
-            all[j] = m;
         }
         float enter[C];
         if (ranks > 1) {
-            if (w == 0)
+            if (w < ranks) *cluster.map_shared_rank(&whole[buf][rank][lane], w) = all;
+            auto token = cluster.barrier_arrive();
+            if (base + stride < most) next.load(a, s, t0 + stride, ch);
+            cluster.barrier_wait(std::move(token));
 #pragma unroll
-                for (int j = 0; j < C; ++j) whole[buf][j][lane] = all[j];
-            cluster.sync();
+            for (int j = 0; j < C; ++j) enter[j] = state[j];
 #pragma unroll
-            for (int j = 0; j < C; ++j) {
-                float x = state[j];
-                enter[j] = x;
-                for (int q = 0; q < ranks; ++q) {
-                    if (q == rank) enter[j] = x;
-                    x = apply(*cluster.map_shared_rank(&whole[buf][j][lane], q), x);
+            for (int q = 0; q < MOST_RANKS; ++q)
+                if (q < ranks) {
+                    const Maps<C> n = whole[buf][q][lane];
+#pragma unroll
+                    for (int j = 0; j < C; ++j) {
+                        if (q == rank) enter[j] = state[j];
+                        state[j] = apply(n.m[j], state[j]);
+                    }
                 }
-                state[j] = x;
-            }
         } else {
+            if (base + stride < most) next.load(a, s, t0 + stride, ch);
 #pragma unroll
             for (int j = 0; j < C; ++j) {
                 enter[j] = state[j];
-                state[j] = apply(all[j], state[j]);
+                state[j] = apply(all.m[j], state[j]);
             }
         }
 #pragma unroll
-        for (int j = 0; j < C; ++j) enter[j] = apply(before[j], enter[j]);
-        if (live) k.finish(a, s, t0, ch, seq, enter);
+        for (int j = 0; j < C; ++j) enter[j] = apply(before.m[j], enter[j]);
+        int64_t at = (s.first + t0 * s.dir) * a.d + ch;
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (i < left) {
+                if constexpr (BACK) f[0].form(k, i);   // formed again: registers are short here
+                f[BACK ? 0 : i].take(a, k, i, i + 1 == left, at, (int64_t)seq * a.d + ch, enter);
+                at += (int64_t)s.dir * a.d;
+            }
     }
     if (live && rank == 0 && w == 0) {
         put_state<C>(a, seq, ch, state);
         clear_outside<T, BACK, C>(a, seq, ch);
     }
-    if (ranks > 1) cluster.sync();                     // no block leaves while another reads its maps
+    if (ranks > 1) cluster.sync();                     // no block leaves while another writes to it
 }
 
 template <typename T, bool SIG, bool BACK, int C>
-int scan_launch(ScanArgs a, int64_t longest, cudaStream_t st) {
+int scan_launch(ScanArgs a, int64_t longest, int sms, cudaStream_t st) {
     constexpr int U = 8;
-    const int sms = op_sms();
-    if (sms <= 0) return op_fail(FFN_E_CUDA, "no CUDA device");
     a.groups = a.d / C;
     a.items = (int64_t)a.seqs * a.groups;
     const int64_t warps = (a.items + 31) / 32;
     // parts of time that are wanted for about 16 warps an SM, and that the length has
-    const int64_t parts = (longest + U - 1) / U;
+    constexpr int US = sizeof(T) == 4 && BACK ? 4 : 8;   // the split form's: four streams of fp32 pairs take its registers
+    const int64_t parts = (longest + US - 1) / US;
     int64_t want = ((int64_t)sms * 16 + warps - 1) / warps;
     want = want < parts ? want : parts;
     if (want <= 1) {
@@ -315,12 +393,12 @@ int scan_launch(ScanArgs a, int64_t longest, cudaStream_t st) {
         scan_kernel<T, SIG, BACK, C, U><<<(unsigned)blocks, 256, 0, st>>>(a);
         return op_launched("ffn_gated_scan");
     }
-    int w = 2, ranks = 1;
-    while (w < MAX_WARPS && w < want) w *= 2;
-    while (ranks < 8 && (int64_t)w * ranks < want) ranks *= 2;
+    if constexpr (C <= 2) {
+    int ranks = 1;
+    while (ranks < MOST_RANKS && (int64_t)WARPS * ranks < want) ranks *= 2;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(warps * ranks));
-    cfg.blockDim = dim3(32 * w);
+    cfg.blockDim = dim3(32 * WARPS);
     cfg.stream = st;
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeClusterDimension;
@@ -328,20 +406,43 @@ int scan_launch(ScanArgs a, int64_t longest, cudaStream_t st) {
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, scan_split_kernel<T, SIG, BACK, C, U>, a);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, scan_split_kernel<T, SIG, BACK, C, US>, a);
     return e == cudaSuccess ? FFN_OK : op_fail(FFN_E_CUDA, std::string("ffn_gated_scan: ") + cudaGetErrorString(e));
+    }
+    return op_fail(FFN_E_CONFIG, "ffn_gated_scan: no split form for this width");   // scan_width gives C = 4 enough threads
+}
+
+// Channels of a thread: as many as an 8-byte access holds, where the rows allow it and enough threads are left.
+template <typename T, bool BACK>
+int scan_width(const ScanArgs& a, int form, int width, int64_t longest, cudaStream_t st) {
+    const int sms = op_sms();
+    if (sms <= 0) return op_fail(FFN_E_CUDA, "no CUDA device");
+    const bool sig = form == FFN_SCAN_SIGMOID;
+    if constexpr (sizeof(T) == 2) {
+        if (width == 4 && (int64_t)a.seqs * (a.d / 4) >= (int64_t)sms * 16 * 32)
+            return sig ? scan_launch<T, true, BACK, 4>(a, longest, sms, st) : scan_launch<T, false, BACK, 4>(a, longest, sms, st);
+    }
+    if (width >= 2) return sig ? scan_launch<T, true, BACK, 2>(a, longest, sms, st) : scan_launch<T, false, BACK, 2>(a, longest, sms, st);
+    return sig ? scan_launch<T, true, BACK, 1>(a, longest, sms, st) : scan_launch<T, false, BACK, 1>(a, longest, sms, st);
 }
 
 template <bool BACK>
-int scan_dispatch(const ScanArgs& a, int dtype, int form, bool paired, int64_t longest, cudaStream_t st) {
-#define FFN_SCAN(T)                                                                                                     \
-    (form == FFN_SCAN_SIGMOID                                                                                           \
-         ? (paired ? scan_launch<T, true, BACK, 2>(a, longest, st) : scan_launch<T, true, BACK, 1>(a, longest, st))     \
-         : (paired ? scan_launch<T, false, BACK, 2>(a, longest, st) : scan_launch<T, false, BACK, 1>(a, longest, st)))
-    if (dtype == FFN_F32) return FFN_SCAN(float);
-    if (dtype == FFN_F16) return FFN_SCAN(__half);
-    return FFN_SCAN(__nv_bfloat16);
-#undef FFN_SCAN
+int scan_dispatch(const ScanArgs& a, int dtype, int form, int width, int64_t longest, cudaStream_t st) {
+    if (dtype == FFN_F32) return scan_width<float, BACK>(a, form, width, longest, st);
+    if (dtype == FFN_F16) return scan_width<__half, BACK>(a, form, width, longest, st);
+    return scan_width<__nv_bfloat16, BACK>(a, form, width, longest, st);
+}
+
+// The widest group of channels that every row of these matrices holds aligned: 4, 2 or 1.
+int scan_channels(int d, int dtype, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> lds) {
+    const size_t z = dtype == FFN_F32 ? 4 : 2;
+    for (int c = 4; c > 1; c /= 2) {
+        bool ok = d % c == 0;
+        for (const void* p : ptrs) ok = ok && op_aligned(p, c * z);
+        for (int64_t ld : lds) ok = ok && ld % c == 0;
+        if (ok) return c;
+    }
+    return 1;
 }
 
 int scan_check(const char* who, int64_t n_rows, int32_t n_seq, int64_t max_len, int32_t d, int dtype, int form,
@@ -369,14 +470,12 @@ int ffn_gated_scan(const void* gate, int64_t gate_ld, const void* value, int64_t
     if (n_seq == 0) return FFN_OK;
     if (n_rows > 0 && (!gate || !value || !h)) return op_fail(FFN_E_CONFIG, "ffn_gated_scan: a required pointer is NULL");
     if (gate_ld < d || value_ld < d) return op_fail(FFN_E_CONFIG, "ffn_gated_scan: a row stride is below d");
-    const size_t pair = dtype == FFN_F32 ? 8 : 4;
-    const bool paired = d % 2 == 0 && gate_ld % 2 == 0 && value_ld % 2 == 0 && op_aligned(gate, pair) &&
-                        op_aligned(value, pair) && op_aligned(h, pair);
+    const int width = scan_channels(d, dtype, {gate, value, h}, {gate_ld, value_ld});
     ScanArgs a{};
     a.gate = gate; a.value = value; a.h0 = h0; a.h = h; a.last = h_last; a.offsets = offsets;
     a.gate_ld = gate_ld; a.value_ld = value_ld; a.rows = n_rows; a.len = max_len; a.seqs = n_seq; a.d = d;
     a.reverse = reverse;
-    return scan_dispatch<false>(a, dtype, form, paired, max_len, static_cast<cudaStream_t>(stream));
+    return scan_dispatch<false>(a, dtype, form, width, max_len, static_cast<cudaStream_t>(stream));
 }
 
 int ffn_gated_scan_bwd(const void* dh, int64_t dh_ld, const float* dh_last, const void* gate, int64_t gate_ld,
@@ -389,15 +488,13 @@ int ffn_gated_scan_bwd(const void* dh, int64_t dh_ld, const float* dh_last, cons
         return op_fail(FFN_E_CONFIG, "ffn_gated_scan_bwd: a required pointer is NULL");
     if (gate_ld < d || (value && value_ld < d) || dh_ld < d || h_ld < d)
         return op_fail(FFN_E_CONFIG, "ffn_gated_scan_bwd: a row stride is below d");
-    const size_t pair = dtype == FFN_F32 ? 8 : 4;
-    const bool paired = d % 2 == 0 && gate_ld % 2 == 0 && (!value || value_ld % 2 == 0) && dh_ld % 2 == 0 && h_ld % 2 == 0 &&
-                        op_aligned(gate, pair) && op_aligned(value, pair) && op_aligned(dh, pair) && op_aligned(h, pair) &&
-                        op_aligned(dgate, pair) && op_aligned(dvalue, pair);
+    const int width = scan_channels(d, dtype, {gate, value, dh, h, dgate, dvalue},
+                                    {gate_ld, value ? value_ld : 0, dh_ld, h_ld});
     ScanArgs a{};
     a.gate = gate; a.value = value; a.dh = dh; a.h_in = h; a.h0 = h0; a.dlast = dh_last; a.dgate = dgate; a.dvalue = dvalue;
     a.last = dh0; a.offsets = offsets; a.gate_ld = gate_ld; a.value_ld = value_ld; a.dh_ld = dh_ld; a.h_ld = h_ld;
     a.rows = n_rows; a.len = max_len; a.seqs = n_seq; a.d = d; a.reverse = reverse;
-    return scan_dispatch<true>(a, dtype, form, paired, max_len, static_cast<cudaStream_t>(stream));
+    return scan_dispatch<true>(a, dtype, form, width, max_len, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"
