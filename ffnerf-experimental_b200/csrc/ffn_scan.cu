@@ -25,12 +25,13 @@
 // shared memory (within the block) and distributed shared memory (within the cluster), and each thread
 // then enters its part with the state that the maps before it give.  The elements stay in registers in
 // between, so the split costs no second read; no global memory and no waiting on flags is involved.
+#include <atomic>
 #include <initializer_list>
 #include <type_traits>
-#include <utility>
 #include <cooperative_groups.h>
 
 #include "ffn_ops.cuh"
+#include "ffn_tcgen05.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -99,6 +100,11 @@ template <typename T, int C>
 struct Word {
     typename Raw<sizeof(T) * C>::type r;
     __device__ __forceinline__ void load(const T* p) { r = __ldg(reinterpret_cast<const decltype(r)*>(p)); }
+    // Copies a word to shared memory without waiting (4 bytes or more).
+    static __device__ __forceinline__ void copy(Word* to, const T* p) {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;"
+                     :: "r"((uint32_t)__cvta_generic_to_shared(to)), "l"(p), "n"((int)sizeof(Word)) : "memory");
+    }
     __device__ __forceinline__ float at(int j) const {
         if constexpr (sizeof(T) == 4) {
             if constexpr (C == 1) return __uint_as_float(r);
@@ -122,7 +128,10 @@ template <typename T, bool SIG, bool BACK, int C, int U>
 struct Chunk {
     Word<T, C> gate[U], value[SIG || !BACK ? U : 1], dh[BACK ? U : 1], before[BACK ? U : 1];
 
-    __device__ __forceinline__ void load(const ScanArgs& a, const Span& s, int64_t t0, int ch) {
+    // Calls f(stream, step, address) for each word of the chunk that lies before the sequence's end.
+    // Streams: 0 gate, 1 value, 2 dh, 3 the state before the step.
+    template <typename F>
+    static __device__ __forceinline__ void each(const ScanArgs& a, const Span& s, int64_t t0, int ch, F&& f) {
         const int64_t row = s.first + t0 * s.dir;
         const T* pg = static_cast<const T*>(a.gate) + row * a.gate_ld + ch;
         const T* pv = static_cast<const T*>(a.value) + row * a.value_ld + ch;
@@ -133,21 +142,27 @@ struct Chunk {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             if (i < left) {
-                gate[i].load(pg);
+                f(0, i, pg);
                 pg += sg;
                 if constexpr (SIG || !BACK) {
-                    value[i].load(pv);
+                    f(1, i, pv);
                     pv += sv;
                 }
                 if constexpr (BACK) {
-                    dh[i].load(pd);
+                    f(2, i, pd);
                     pd += sd;
                     // the state before this step: the next row of this walk (the last step's is h0)
-                    if (i + 1 < left) before[i].load(pb);
+                    if (i + 1 < left) f(3, i, pb);
                     pb += sb;
                 }
             }
         }
+    }
+    __device__ __forceinline__ Word<T, C>& word(int stream, int i) {
+        return stream == 0 ? gate[i] : stream == 1 ? value[SIG || !BACK ? i : 0] : stream == 2 ? dh[BACK ? i : 0] : before[BACK ? i : 0];
+    }
+    __device__ __forceinline__ void load(const ScanArgs& a, const Span& s, int64_t t0, int ch) {
+        each(a, s, t0, ch, [&](int q, int i, const T* p) { word(q, i).load(p); });
     }
 };
 
@@ -270,15 +285,54 @@ constexpr int WARPS = 8, MOST_RANKS = 8;
 // The maps of a lane's C channels.
 template <int C> struct alignas(8 * C) Maps { Affine m[C]; };
 
+// The split form: steps of a warp's part, and the stages of its ring of chunks in shared memory.  Each
+// thread copies the words that it will use itself, so the ring needs no barrier; words of 2 bytes, which
+// have no asynchronous copy, are prefetched one chunk ahead in registers instead.
+template <typename T, bool SIG, bool BACK, int C>
+struct Split {
+    static constexpr int W = sizeof(T) * C;
+    static constexpr bool RING = W >= 4;
+    static constexpr int U = !RING ? 8 : (BACK ? 32 : 64) / W;
+    static constexpr int STREAMS = BACK ? 4 : 2;
+    static constexpr int STAGES = RING ? 3 : 0;
+    static constexpr size_t BYTES = (size_t)STAGES * STREAMS * U * W * 32 * WARPS;   // at most 96 KB: two blocks an SM
+};
+
+__device__ int g_scan_status;                         // ST_TC_TIMEOUT's bit when a wait ran out (ffn_ops_status)
+constexpr uint32_t WAIT_POLLS = 1u << 22;
+
+// Writes a lane's maps into block `rank`'s shared memory and counts their bytes on that block's mbarrier.
+template <int C>
+__device__ __forceinline__ void send_maps(const Maps<C>* to, uint64_t* bar, int rank, const Maps<C>& v) {
+    uint32_t ra, rb;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"((uint32_t)__cvta_generic_to_shared(to)), "r"(rank));
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(rb) : "r"((uint32_t)__cvta_generic_to_shared(bar)), "r"(rank));
+    if constexpr (C == 2)
+        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];"
+                     :: "r"(ra), "f"(v.m[0].p), "f"(v.m[0].h), "f"(v.m[1].p), "f"(v.m[1].h), "r"(rb) : "memory");
+    else
+        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];"
+                     :: "r"(ra), "f"(v.m[0].p), "f"(v.m[0].h), "r"(rb) : "memory");
+}
+
 // Few sequences and channels: 32 items per cluster, time split over the WARPS warps of its blocks, U steps
-// a warp.  The next chunk's loads are in flight while the maps of this one go round: a block's map is
-// written straight into the shared memory of the cluster's other blocks (warp q writes to block q), so
-// after the one cluster barrier of a turn every read is local.
-template <typename T, bool SIG, bool BACK, int C, int U>
+// a warp.  The loads of the next chunks are in flight while the maps of this one go round: a block's map is
+// written straight into the shared memory of the cluster's blocks (warp q writes to block q), and each
+// block waits on its own mbarrier for the bytes of all.  A cluster barrier in its place costs more than
+// the rest of a turn: its release waits until the results that the last turn stored have reached L2.
+// Two buffers are enough: a block sends its maps of the next turn after it has read those of this one,
+// and nobody sends those of the turn after without having them.
+template <typename T, bool SIG, bool BACK, int C>
 __global__ void __launch_bounds__(32 * WARPS, 2) scan_split_kernel(const ScanArgs a) {
+    using S = Split<T, SIG, BACK, C>;
+    constexpr int U = S::U;
+    using K = Chunk<T, SIG, BACK, C, U>;
     cg::cluster_group cluster = cg::this_cluster();
+    extern __shared__ __align__(16) unsigned char ring_bytes[];
+    [[maybe_unused]] Word<T, C>* ring = reinterpret_cast<Word<T, C>*>(ring_bytes) + threadIdx.x;   // [stage][stream][step][thread]
     __shared__ Maps<C> part[2][WARPS][32];            // the maps of this block's parts
     __shared__ Maps<C> whole[2][MOST_RANKS][32];      // the maps of the cluster's blocks
+    __shared__ uint64_t arrived[2];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
     const int64_t item = (int64_t)(blockIdx.x / ranks) * 32 + lane;
@@ -291,14 +345,44 @@ __global__ void __launch_bounds__(32 * WARPS, 2) scan_split_kernel(const ScanArg
     for (int o = 16; o > 0; o >>= 1) most = max(most, (int64_t)__shfl_xor_sync(0xffffffffu, (long long)most, o));
     float state[C];
     first_state<BACK, C>(a, seq, ch, state);
-    if (ranks > 1) cluster.sync();                     // every block runs before its memory is written
+    if (ranks > 1) {
+        if (threadIdx.x == 0) { tc::mbar_init(arrived, 1); tc::mbar_init(arrived + 1, 1); }
+        cluster.sync();                                // every block runs, its barriers ready, before it is written to
+    }
+    bool ok = true;                                    // no wait has run out (else the rest of them is left out)
     const int64_t stride = (int64_t)U * WARPS * ranks;
     int64_t t0 = (int64_t)(rank * WARPS + w) * U;
-    Chunk<T, SIG, BACK, C, U> next;
-    next.load(a, s, t0, ch);
+    K next;
+    int fill = 0, drain = 0;                           // stages of the ring
+    auto fetch = [&](int64_t t) {
+        if constexpr (S::RING) {
+            K::each(a, s, t, ch, [&](int q, int i, const T* p) {
+                Word<T, C>::copy(ring + ((fill * S::STREAMS + q) * U + i) * (32 * WARPS), p);
+            });
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            fill = fill + 1 == S::STAGES ? 0 : fill + 1;
+        } else {
+            next.load(a, s, t, ch);
+        }
+    };
+    fetch(t0);
+    if constexpr (S::RING) fetch(t0 + stride);
     int buf = 0;
-    for (int64_t base = 0; base < most; base += stride, t0 += stride, buf ^= 1) {
-        const Chunk<T, SIG, BACK, C, U> k = next;
+    uint32_t phase = 0;
+    for (int64_t base = 0; base < most; base += stride, t0 += stride, phase ^= buf, buf ^= 1) {
+        K k;
+        if constexpr (S::RING) {
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            fetch(t0 + 2 * stride);                    // into the stage that the last turn has read
+#pragma unroll
+            for (int i = 0; i < U; ++i)
+#pragma unroll
+                for (int q = 0; q < S::STREAMS; ++q)
+                    if (q != 1 || SIG || !BACK) k.word(q, i) = ring[((drain * S::STREAMS + q) * U + i) * (32 * WARPS)];
+            drain = drain + 1 == S::STAGES ? 0 : drain + 1;
+        } else {
+            k = next;
+        }
         Step<SIG, BACK, C> f[BACK ? 1 : U];            // forward: kept for the second walk over the steps
         const int left = (int)min(max(s.len - t0, (int64_t)0), (int64_t)(U + 1));
         Maps<C> mine;
@@ -334,10 +418,15 @@ __global__ void __launch_bounds__(32 * WARPS, 2) scan_split_kernel(const ScanArg
         }
         float enter[C];
         if (ranks > 1) {
-            if (w < ranks) *cluster.map_shared_rank(&whole[buf][rank][lane], w) = all;
-            auto token = cluster.barrier_arrive();
-            if (base + stride < most) next.load(a, s, t0 + stride, ch);
-            cluster.barrier_wait(std::move(token));
+            if (threadIdx.x == 0)
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
+                             :: "r"(tc::smem_u32(arrived + buf)), "r"(ranks * 32 * (int)sizeof(Maps<C>)) : "memory");
+            if (w < ranks) send_maps<C>(&whole[buf][rank][lane], arrived + buf, w, all);
+            if constexpr (!S::RING) if (base + stride < most) fetch(t0 + stride);
+            if (ok && !tc::mbar_wait(arrived + buf, phase, WAIT_POLLS)) {
+                ok = false;
+                atomicOr(&g_scan_status, 4);
+            }
 #pragma unroll
             for (int j = 0; j < C; ++j) enter[j] = state[j];
 #pragma unroll
@@ -351,7 +440,7 @@ __global__ void __launch_bounds__(32 * WARPS, 2) scan_split_kernel(const ScanArg
                     }
                 }
         } else {
-            if (base + stride < most) next.load(a, s, t0 + stride, ch);
+            if constexpr (!S::RING) if (base + stride < most) fetch(t0 + stride);
 #pragma unroll
             for (int j = 0; j < C; ++j) {
                 enter[j] = state[j];
@@ -369,6 +458,7 @@ __global__ void __launch_bounds__(32 * WARPS, 2) scan_split_kernel(const ScanArg
                 at += (int64_t)s.dir * a.d;
             }
     }
+    if constexpr (S::RING) asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (live && rank == 0 && w == 0) {
         put_state<C>(a, seq, ch, state);
         clear_outside<T, BACK, C>(a, seq, ch);
@@ -383,7 +473,7 @@ int scan_launch(ScanArgs a, int64_t longest, int sms, cudaStream_t st) {
     a.items = (int64_t)a.seqs * a.groups;
     const int64_t warps = (a.items + 31) / 32;
     // parts of time that are wanted for about 16 warps an SM, and that the length has
-    constexpr int US = sizeof(T) == 4 && BACK ? 4 : 8;   // the split form's: four streams of fp32 pairs take its registers
+    constexpr int US = Split<T, SIG, BACK, C < 4 ? C : 2>::U;
     const int64_t parts = (longest + US - 1) / US;
     int64_t want = ((int64_t)sms * 16 + warps - 1) / warps;
     want = want < parts ? want : parts;
@@ -394,20 +484,31 @@ int scan_launch(ScanArgs a, int64_t longest, int sms, cudaStream_t st) {
         return op_launched("ffn_gated_scan");
     }
     if constexpr (C <= 2) {
-    int ranks = 1;
-    while (ranks < MOST_RANKS && (int64_t)WARPS * ranks < want) ranks *= 2;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(warps * ranks));
-    cfg.blockDim = dim3(32 * WARPS);
-    cfg.stream = st;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = (unsigned)ranks;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, scan_split_kernel<T, SIG, BACK, C, US>, a);
-    return e == cudaSuccess ? FFN_OK : op_fail(FFN_E_CUDA, std::string("ffn_gated_scan: ") + cudaGetErrorString(e));
+        using S = Split<T, SIG, BACK, C>;
+        auto kernel = scan_split_kernel<T, SIG, BACK, C>;
+        static std::atomic<uint64_t> ready{0};        // devices whose limit is set
+        int dev = 0;
+        cudaGetDevice(&dev);
+        cudaError_t e = cudaSuccess;
+        if (S::BYTES > 40960 && (dev > 63 || !(ready.load(std::memory_order_acquire) >> dev & 1))) {
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::BYTES);
+            if (e == cudaSuccess && dev <= 63) ready.fetch_or(1ull << dev, std::memory_order_release);
+        }
+        int ranks = 1;
+        while (ranks < MOST_RANKS && (int64_t)WARPS * ranks < want) ranks *= 2;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)(warps * ranks));
+        cfg.blockDim = dim3(32 * WARPS);
+        cfg.dynamicSmemBytes = S::BYTES;
+        cfg.stream = st;
+        cudaLaunchAttribute at{};
+        at.id = cudaLaunchAttributeClusterDimension;
+        at.val.clusterDim.x = (unsigned)ranks;
+        at.val.clusterDim.y = at.val.clusterDim.z = 1;
+        cfg.attrs = &at;
+        cfg.numAttrs = 1;
+        if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, a);
+        return e == cudaSuccess ? FFN_OK : op_fail(FFN_E_CUDA, std::string("ffn_gated_scan: ") + cudaGetErrorString(e));
     }
     return op_fail(FFN_E_CONFIG, "ffn_gated_scan: no split form for this width");   // scan_width gives C = 4 enough threads
 }
@@ -457,6 +558,15 @@ int scan_check(const char* who, int64_t n_rows, int32_t n_seq, int64_t max_len, 
 }
 
 }  // namespace
+
+// The scan's share of the status word (ffn_ops_status): reads and clears it.
+cudaError_t scan_status(int* v) {
+    cudaError_t e = cudaMemcpyFromSymbol(v, g_scan_status, sizeof *v);
+    const int zero = 0;
+    if (e == cudaSuccess && *v) e = cudaMemcpyToSymbol(g_scan_status, &zero, sizeof zero);
+    return e;
+}
+
 }  // namespace ffn
 
 using namespace ffn;

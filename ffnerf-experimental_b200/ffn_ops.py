@@ -351,7 +351,7 @@ def expert_mm_bwd(dy, x, w, offsets, need_dx: bool = True, need_dw: bool = True,
 def status(device=None) -> int:
     """Status word of the block operators on the current (or given) device since the last call; waits for
     the device.  0 when every kernel completed normally; ``ffn_native.STATUS_TC_TIMEOUT`` when a wait of
-    an expert product ran out and its results are incomplete."""
+    an expert product or of a split recurrence ran out and its results are wrong."""
     import ctypes
     v = ctypes.c_uint32()
     with torch.cuda.device(device):

@@ -365,8 +365,8 @@ int ffn_expert_mm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld
                       void* workspace, uint64_t workspace_bytes, void* stream);
 
 /* Reads and clears the current device's status word of the block operators (waits for the device): 0
- * when every kernel completed normally; bit 2 = a wait of an expert product exceeded its bound and the
- * kernel gave up, its results incomplete. */
+ * when every kernel completed normally; bit 2 = a wait of an expert product or of a
+ * recurrence split over a cluster exceeded its bound and the kernel gave it up, its results wrong. */
 int ffn_ops_status(uint32_t* status);
 
 #ifdef __cplusplus
