@@ -25,6 +25,7 @@ struct NormArgs {
     void* h; void* y; float* scale; float* rstd;
     int64_t n, x_ld, res_ld;
     int d, group, tpr;
+    int group_log2;              // of group, where it is not 0
     float eps;
 };
 
@@ -35,117 +36,151 @@ struct NormBwdArgs {
     int d, tpr;
 };
 
+// VEC weights from column c on (aligned where VEC > 1: the host checks gamma with the rows).
+template <int VEC>
+__device__ __forceinline__ void load_gamma(const float* g, int c, float (&w)[VEC]) {
+    if constexpr (VEC >= 4) {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 4) {
+            const float4 q = __ldg(reinterpret_cast<const float4*>(g + c + j));
+            w[j] = q.x; w[j + 1] = q.y; w[j + 2] = q.z; w[j + 3] = q.w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) w[j] = __ldg(g + c + j);
+    }
+}
+
 // Sum (or NaN-keeping maximum) over the threads of one row: `tpr` lanes, or the block (BLOCK).  In a
 // block the warps' values are added in warp order, so a row's result does not depend on timing.
 template <bool BLOCK, bool MAX>
-__device__ __forceinline__ float row_reduce(float v, int tpr, float* sh) {
+__device__ __forceinline__ float row_reduce(float v, int tpr, float (&sh)[2][32], int& turn) {
     for (int o = (BLOCK ? 32 : tpr) >> 1; o > 0; o >>= 1) {
         const float w = __shfl_xor_sync(0xffffffffu, v, o);
         v = MAX ? max_nan(v, w) : v + w;
     }
     if constexpr (BLOCK) {
+        // one barrier: the buffer of the reduction before last has been read by all who passed the last one
         const int warps = blockDim.x >> 5;
-        __syncthreads();                       // the previous use of sh is over
-        if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+        float* q = sh[turn];
+        turn ^= 1;
+        if ((threadIdx.x & 31) == 0) q[threadIdx.x >> 5] = v;
         __syncthreads();
-        v = sh[0];
-        for (int w = 1; w < warps; ++w) v = MAX ? max_nan(v, sh[w]) : v + sh[w];
+        v = q[0];
+        for (int w = 1; w < warps; ++w) v = MAX ? max_nan(v, q[w]) : v + q[w];
     }
     return v;
 }
 
-// NV vectors of VEC elements per thread: vector i of a thread starts at column (lane + i * threads) * VEC.
-template <typename T, bool OUT8, int VEC, int NV, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 512 : 256) rmsnorm_kernel(const NormArgs a) {
-    __shared__ float sh[32];
+// NV vectors of VEC elements per thread and row: vector i of a thread starts at column (lane + i * tpr) * VEC.
+// Short rows go R at a time, so that a thread has four vectors of each input in flight either way.
+template <typename T, bool OUT8, int VEC, int NV, int R, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? 512 : 256, BLOCK ? 2 : 4) rmsnorm_kernel(const NormArgs a) {
+    __shared__ float sh[2][32];
+    int turn = 0;
     const int tpr = BLOCK ? (int)blockDim.x : a.tpr;
     const int lane = threadIdx.x & (tpr - 1);
-    const int rows = BLOCK ? 1 : (int)blockDim.x / tpr;          // rows of a block at a time
+    const int rows = BLOCK ? 1 : (int)blockDim.x / tpr;          // rows of a block side by side
     const int sub = BLOCK ? 0 : (int)threadIdx.x / tpr;
     const float inv_d = 1.0f / (float)a.d;
     const T* x = static_cast<const T*>(a.x);
     const T* res = static_cast<const T*>(a.res);
-    for (int64_t base = (int64_t)blockIdx.x * rows; base < a.n; base += (int64_t)gridDim.x * rows) {
-        const int64_t row = base + sub;
-        const bool live = row < a.n;
-        float v[NV][VEC];
-        float ss = 0.0f;
+    for (int64_t base = (int64_t)blockIdx.x * rows * R; base < a.n; base += (int64_t)gridDim.x * rows * R) {
+        Vec<T, VEC> p[R][NV], q[R][NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (lane + i * tpr) * VEC;
-            const bool on = live && c < a.d;
-            Pack<T, VEC> p{}, q{};
-            if (on) {
-                p = load_pack<T, VEC>(x + row * a.x_ld + c);
-                if (res) q = load_pack<T, VEC>(res + row * a.res_ld + c);
+        for (int r = 0; r < R; ++r) {
+            const int64_t row = base + r * rows + sub;
+            const T* px = x + row * a.x_ld + lane * VEC;
+            const T* pr = res + row * a.res_ld + lane * VEC;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                p[r][i].clear();
+                q[r][i].clear();
+                if (row < a.n && (lane + i * tpr) * VEC < a.d) {
+                    p[r][i].load(px + i * tpr * VEC);
+                    if (res) q[r][i].load(pr + i * tpr * VEC);
+                }
             }
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) v[i][j] = on ? to_f(p.v[j]) + (res ? to_f(q.v[j]) : 0.0f) : 0.0f;
         }
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int r = 0; r < R; ++r) {
+            const int64_t row = base + r * rows + sub;
+            const bool live = row < a.n;
+            float v[NV][VEC];
+            float ss = 0.0f;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) ss = fmaf(v[i][j], v[i][j], ss);
-        ss = row_reduce<BLOCK, false>(ss, tpr, sh);
-        const float s = rsqrtf(fmaf(ss, inv_d, a.eps));
-        if (a.rstd && live && lane == 0) a.rstd[row] = s;
-        float top = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (lane + i * tpr) * VEC;
-            if (live && c < a.d) {
-                if (a.h) {
-                    Pack<T, VEC> p;
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) p.v[j] = from_f<T>(v[i][j]);
-                    store_pack<T, VEC>(static_cast<T*>(a.h) + row * a.d + c, p);
-                }
+            for (int i = 0; i < NV; ++i) {
+                float w[VEC];
+                p[r][i].get(v[i]);
+                q[r][i].get(w);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    v[i][j] = v[i][j] * s * __ldg(a.gamma + c + j);
-                    if constexpr (OUT8) top = max_nan(top, fabsf(v[i][j]));
-                }
-                if constexpr (!OUT8) {
-                    Pack<T, VEC> p;
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) p.v[j] = from_f<T>(v[i][j]);
-                    store_pack<T, VEC>(static_cast<T*>(a.y) + row * a.d + c, p);
+                    v[i][j] += w[j];                             // zeros where there is no residual
+                    ss = fmaf(v[i][j], v[i][j], ss);
                 }
             }
-        }
-        if constexpr (OUT8) {
-            float sc = 1.0f;
-            if (!a.group) {
-                top = row_reduce<BLOCK, true>(top, tpr, sh);
-                sc = e4m3_scale(top);
-                if (live && lane == 0) a.scale[row] = sc;
-            }
+            ss = row_reduce<BLOCK, false>(ss, tpr, sh, turn);
+            const float s = rsqrtf(fmaf(ss, inv_d, a.eps));
+            if (a.rstd && live && lane == 0) a.rstd[row] = s;
+            float top = 0.0f;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int c = (lane + i * tpr) * VEC;
-                const bool on = live && c < a.d;
-                if (a.group) {   // group / VEC neighbouring lanes hold one group's columns
-                    float m = 0.0f;
+                if (live && c < a.d) {
+                    if (a.h) {
+                        Vec<T, VEC> o;
+                        o.put(v[i]);
+                        o.store(static_cast<T*>(a.h) + row * a.d + c);
+                    }
+                    float g[VEC];
+                    load_gamma<VEC>(a.gamma, c, g);
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) m = max_nan(m, on ? fabsf(v[i][j]) : 0.0f);
-                    for (int o = a.group / VEC / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-                    sc = e4m3_scale(m);
-                    if (on && c % a.group == 0) a.scale[row * (a.d / a.group) + c / a.group] = sc;
+                    for (int j = 0; j < VEC; ++j) {
+                        v[i][j] = v[i][j] * s * g[j];
+                        if constexpr (OUT8) top = max_nan(top, fabsf(v[i][j]));
+                    }
+                    if constexpr (!OUT8) {
+                        Vec<T, VEC> o;
+                        o.put(v[i]);
+                        o.store(static_cast<T*>(a.y) + row * a.d + c);
+                    }
                 }
-                if (on) {
-                    const float inv = e4m3_inverse(sc);
-                    uint8_t* q = static_cast<uint8_t*>(a.y) + row * a.d + c;
-                    if constexpr (VEC == 8) {
-                        *reinterpret_cast<uint2*>(q) =
-                            make_uint2(pack_e4m3x4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv),
-                                       pack_e4m3x4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv));
-                    } else if constexpr (VEC == 4) {
-                        *reinterpret_cast<uint32_t*>(q) =
-                            pack_e4m3x4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
-                    } else {
+            }
+            if constexpr (OUT8) {
+                float sc = 1.0f, inv = 1.0f;
+                if (!a.group) {
+                    top = row_reduce<BLOCK, true>(top, tpr, sh, turn);
+                    sc = e4m3_scale(top);
+                    inv = e4m3_inverse(sc);
+                    if (live && lane == 0) a.scale[row] = sc;
+                }
 #pragma unroll
-                        for (int j = 0; j < VEC; ++j)
-                            q[j] = (uint8_t)__nv_cvt_float_to_fp8(v[i][j] * inv, __NV_SATFINITE, __NV_E4M3);
+                for (int i = 0; i < NV; ++i) {
+                    const int c = (lane + i * tpr) * VEC;
+                    const bool on = live && c < a.d;
+                    if (a.group) {   // group / VEC neighbouring lanes hold one group's columns
+                        float m = 0.0f;
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) m = max_nan(m, on ? fabsf(v[i][j]) : 0.0f);
+                        for (int o = (a.group / VEC) >> 1; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+                        sc = e4m3_scale(m);
+                        inv = e4m3_inverse(sc);
+                        if (on && (c & (a.group - 1)) == 0) a.scale[row * (a.d >> a.group_log2) + (c >> a.group_log2)] = sc;
+                    }
+                    if (on) {
+                        uint8_t* o = static_cast<uint8_t*>(a.y) + row * a.d + c;
+                        if constexpr (VEC == 8) {
+                            *reinterpret_cast<uint2*>(o) =
+                                make_uint2(pack_e4m3x4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv),
+                                           pack_e4m3x4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv));
+                        } else if constexpr (VEC == 4) {
+                            *reinterpret_cast<uint32_t*>(o) =
+                                pack_e4m3x4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < VEC; ++j)
+                                o[j] = (uint8_t)__nv_cvt_float_to_fp8(v[i][j] * inv, __NV_SATFINITE, __NV_E4M3);
+                        }
                     }
                 }
             }
@@ -157,7 +192,8 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 256) rmsnorm_kernel(const NormAr
 // 16-byte vectors: one block per row, which reads the row again (from L2) for each pass over it.
 template <typename T, bool OUT8>
 __global__ void __launch_bounds__(256) rmsnorm_long_kernel(const NormArgs a) {
-    __shared__ float sh[32];
+    __shared__ float sh[2][32];
+    int turn = 0;
     const float inv_d = 1.0f / (float)a.d;
     for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
         const T* x = static_cast<const T*>(a.x) + row * a.x_ld;
@@ -165,7 +201,7 @@ __global__ void __launch_bounds__(256) rmsnorm_long_kernel(const NormArgs a) {
         auto at = [&](int c) { return to_f(x[c]) + (res ? to_f(res[c]) : 0.0f); };
         float ss = 0.0f;
         for (int c = threadIdx.x; c < a.d; c += blockDim.x) { const float v = at(c); ss = fmaf(v, v, ss); }
-        ss = row_reduce<true, false>(ss, 0, sh);
+        ss = row_reduce<true, false>(ss, 0, sh, turn);
         const float s = rsqrtf(fmaf(ss, inv_d, a.eps));
         if (a.rstd && threadIdx.x == 0) a.rstd[row] = s;
         if constexpr (!OUT8) {
@@ -182,7 +218,7 @@ __global__ void __launch_bounds__(256) rmsnorm_long_kernel(const NormArgs a) {
                 float top = 0.0f;
                 for (int c = g * width + lane; c < (g + 1) * width; c += step)
                     top = max_nan(top, fabsf(at(c) * s * a.gamma[c]));
-                top = a.group ? row_reduce<false, true>(top, 32, sh) : row_reduce<true, true>(top, 0, sh);
+                top = a.group ? row_reduce<false, true>(top, 32, sh, turn) : row_reduce<true, true>(top, 0, sh, turn);
                 const float sc = e4m3_scale(top), inv = e4m3_inverse(sc);
                 if (lane == 0) a.scale[row * (a.d / width) + g] = sc;
                 for (int c = g * width + lane; c < (g + 1) * width; c += step) {
@@ -200,9 +236,10 @@ __global__ void __launch_bounds__(256) rmsnorm_long_kernel(const NormArgs a) {
 // a block adds its own and writes one row of `partial`, which norm_dgamma_kernel sums in block order.
 // The gradient of gamma is therefore the same on every run.
 template <typename T, int VEC, int NV, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 512 : 256) rmsnorm_bwd_kernel(const NormBwdArgs a) {
+__global__ void __launch_bounds__(BLOCK ? 512 : 256, BLOCK ? 1 : 2) rmsnorm_bwd_kernel(const NormBwdArgs a) {
     extern __shared__ float dyn[];                               // [warps][d] (not BLOCK)
-    __shared__ float sh[32];
+    __shared__ float sh[2][32];
+    int turn = 0;
     const int tpr = BLOCK ? (int)blockDim.x : a.tpr;
     const int lane = threadIdx.x & (tpr - 1);
     const int rows = BLOCK ? 1 : (int)blockDim.x / tpr;
@@ -221,46 +258,54 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 256) rmsnorm_bwd_kernel(const No
         const int64_t row = base + sub;
         const bool live = row < a.n;
         const float s = live ? __ldg(a.rstd + row) : 0.0f;
-        Pack<T, VEC> pd[NV], pr[NV];
+        Vec<T, VEC> pd[NV], px[NV], pq[NV], pr[NV];
         float v[NV][VEC];                                        // h, then xhat
+        const T* dyr = dyp + row * a.dy_ld + lane * VEC;
+        const T* xr = xp + row * a.x_ld + lane * VEC;
+        const T* rr = rp + row * a.res_ld + lane * VEC;
+        const T* drr = drp + row * a.dres_ld + lane * VEC;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (lane + i * tpr) * VEC;
-            Pack<T, VEC> px{}, pq{};
-            pd[i] = Pack<T, VEC>{}; pr[i] = Pack<T, VEC>{};
-            if (live && c < a.d) {
-                pd[i] = load_pack<T, VEC>(dyp + row * a.dy_ld + c);
-                px = load_pack<T, VEC>(xp + row * a.x_ld + c);
-                if (rp) pq = load_pack<T, VEC>(rp + row * a.res_ld + c);
-                if (drp) pr[i] = load_pack<T, VEC>(drp + row * a.dres_ld + c);
+            pd[i].clear(); px[i].clear(); pq[i].clear(); pr[i].clear();
+            if (live && (lane + i * tpr) * VEC < a.d) {
+                pd[i].load(dyr + i * tpr * VEC);
+                px[i].load(xr + i * tpr * VEC);
+                if (rp) pq[i].load(rr + i * tpr * VEC);
+                if (drp) pr[i].load(drr + i * tpr * VEC);
             }
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) v[i][j] = (to_f(px.v[j]) + (rp ? to_f(pq.v[j]) : 0.0f)) * s;
         }
         float dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (lane + i * tpr) * VEC;
-            if (live && c < a.d)
+            if (c < a.d) {                                       // rows past the end hold zeros
+                float g[VEC], w[VEC], dy[VEC];
+                load_gamma<VEC>(a.gamma, c, g);
+                px[i].get(v[i]);
+                pq[i].get(w);
+                pd[i].get(dy);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    const float dy = to_f(pd[i].v[j]);
-                    dg[i][j] = fmaf(dy, v[i][j], dg[i][j]);
-                    dot = fmaf(dy * __ldg(a.gamma + c + j), v[i][j], dot);
+                    v[i][j] = (v[i][j] + w[j]) * s;
+                    dg[i][j] = fmaf(dy[j], v[i][j], dg[i][j]);
+                    dot = fmaf(dy[j] * g[j], v[i][j], dot);
                 }
+            }
         }
-        dot = row_reduce<BLOCK, false>(dot, tpr, sh) * inv_d;
+        dot = row_reduce<BLOCK, false>(dot, tpr, sh, turn) * inv_d;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (lane + i * tpr) * VEC;
             if (live && c < a.d) {
-                Pack<T, VEC> p;
+                Vec<T, VEC> o;
+                float g[VEC], dy[VEC], r[VEC];
+                load_gamma<VEC>(a.gamma, c, g);
+                pd[i].get(dy);
+                pr[i].get(r);                                    // zeros where there is no dresidual
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const float u = to_f(pd[i].v[j]) * __ldg(a.gamma + c + j);
-                    p.v[j] = from_f<T>(fmaf(s, fmaf(-v[i][j], dot, u), drp ? to_f(pr[i].v[j]) : 0.0f));
-                }
-                store_pack<T, VEC>(static_cast<T*>(a.dx) + row * a.d + c, p);
+                for (int j = 0; j < VEC; ++j) r[j] = fmaf(s, fmaf(-v[i][j], dot, dy[j] * g[j]), r[j]);
+                o.put(r);
+                o.store(static_cast<T*>(a.dx) + row * a.d + c);
             }
         }
     }
@@ -297,7 +342,8 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 256) rmsnorm_bwd_kernel(const No
 // row of `partial` directly (the same thread meets the same columns in every row).
 template <typename T>
 __global__ void __launch_bounds__(256) rmsnorm_bwd_long_kernel(const NormBwdArgs a) {
-    __shared__ float sh[32];
+    __shared__ float sh[2][32];
+    int turn = 0;
     const float inv_d = 1.0f / (float)a.d;
     float* out = a.partial + (int64_t)blockIdx.x * a.d;
     for (int c = threadIdx.x; c < a.d; c += blockDim.x) out[c] = 0.0f;
@@ -314,7 +360,7 @@ __global__ void __launch_bounds__(256) rmsnorm_bwd_long_kernel(const NormBwdArgs
             out[c] += t;
             dot = fmaf(t, a.gamma[c], dot);
         }
-        dot = row_reduce<true, false>(dot, 0, sh) * inv_d;
+        dot = row_reduce<true, false>(dot, 0, sh, turn) * inv_d;
         for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
             const float u = to_f(dy[c]) * a.gamma[c], xh = at(c) * s;
             static_cast<T*>(a.dx)[row * a.d + c] = from_f<T>(fmaf(s, fmaf(-xh, dot, u), dr ? to_f(dr[c]) : 0.0f));
@@ -367,8 +413,8 @@ Shape norm_shape(int d, int full_vec, bool aligned, int group) {
     return s;
 }
 
-int norm_grid(const Shape& s, int64_t n, int sms) {
-    const int64_t rows = s.block || s.loop ? 1 : s.threads / s.tpr;
+int norm_grid(const Shape& s, int64_t n, int sms, int at_once) {
+    const int64_t rows = s.block || s.loop ? 1 : (int64_t)s.threads / s.tpr * at_once;
     const int64_t want = (n + rows - 1) / rows;
     const int64_t most = (int64_t)sms * (2048 / s.threads);
     return (int)(want < most ? want : most);
@@ -382,24 +428,28 @@ int norm_launch(const NormArgs& a0, bool aligned, cudaStream_t st) {
     const int sms = op_sms();
     if (sms <= 0) return op_fail(FFN_E_CUDA, "no CUDA device");
     a.tpr = s.tpr;
-    const int grid = norm_grid(s, a.n, sms);
+    // rows at a time: only where there are enough of them to keep every SM's blocks
+    const int at_once = !s.block && !s.loop && s.vec > 1 && a.n * s.tpr >= (int64_t)sms * 2048 * 4 / s.nv ? 4 / s.nv : 1;
+    const int grid = norm_grid(s, a.n, sms, at_once);
     if (s.loop) rmsnorm_long_kernel<T, OUT8><<<grid, 256, 0, st>>>(a);
     else if (s.vec == 1) {
-        if (s.block) rmsnorm_kernel<T, OUT8, 1, 8, true><<<grid, s.threads, 0, st>>>(a);
-        else rmsnorm_kernel<T, OUT8, 1, 8, false><<<grid, s.threads, 0, st>>>(a);
+        if (s.block) rmsnorm_kernel<T, OUT8, 1, 8, 1, true><<<grid, s.threads, 0, st>>>(a);
+        else rmsnorm_kernel<T, OUT8, 1, 8, 1, false><<<grid, s.threads, 0, st>>>(a);
     } else if (s.block) {
-        if (s.nv == 1) rmsnorm_kernel<T, OUT8, VEC, 1, true><<<grid, s.threads, 0, st>>>(a);
-        else if (s.nv == 2) rmsnorm_kernel<T, OUT8, VEC, 2, true><<<grid, s.threads, 0, st>>>(a);
-        else rmsnorm_kernel<T, OUT8, VEC, 4, true><<<grid, s.threads, 0, st>>>(a);
+        if (s.nv == 1) rmsnorm_kernel<T, OUT8, VEC, 1, 1, true><<<grid, s.threads, 0, st>>>(a);
+        else if (s.nv == 2) rmsnorm_kernel<T, OUT8, VEC, 2, 1, true><<<grid, s.threads, 0, st>>>(a);
+        else rmsnorm_kernel<T, OUT8, VEC, 4, 1, true><<<grid, s.threads, 0, st>>>(a);
     } else {
-        if (s.nv == 1) rmsnorm_kernel<T, OUT8, VEC, 1, false><<<grid, s.threads, 0, st>>>(a);
-        else if (s.nv == 2) rmsnorm_kernel<T, OUT8, VEC, 2, false><<<grid, s.threads, 0, st>>>(a);
-        else rmsnorm_kernel<T, OUT8, VEC, 4, false><<<grid, s.threads, 0, st>>>(a);
+        if (s.nv == 1 && at_once > 1) rmsnorm_kernel<T, OUT8, VEC, 1, 4, false><<<grid, s.threads, 0, st>>>(a);
+        else if (s.nv == 1) rmsnorm_kernel<T, OUT8, VEC, 1, 1, false><<<grid, s.threads, 0, st>>>(a);
+        else if (s.nv == 2 && at_once > 1) rmsnorm_kernel<T, OUT8, VEC, 2, 2, false><<<grid, s.threads, 0, st>>>(a);
+        else if (s.nv == 2) rmsnorm_kernel<T, OUT8, VEC, 2, 1, false><<<grid, s.threads, 0, st>>>(a);
+        else rmsnorm_kernel<T, OUT8, VEC, 4, 1, false><<<grid, s.threads, 0, st>>>(a);
     }
     return op_launched("ffn_rmsnorm");
 }
 
-constexpr int BWD_BLOCKS_PER_SM = 4;   // rows of partial sums: bounded, they are written and read again
+constexpr int BWD_BLOCKS_PER_SM = 4;   // at most; as many as are resident: their rows of partial sums are read again
 
 template <typename T>
 int norm_bwd_launch(const NormBwdArgs& a0, float* dgamma, bool aligned, cudaStream_t st) {
@@ -409,8 +459,9 @@ int norm_bwd_launch(const NormBwdArgs& a0, float* dgamma, bool aligned, cudaStre
     const int sms = op_sms();
     if (sms <= 0) return op_fail(FFN_E_CUDA, "no CUDA device");
     a.tpr = s.tpr;
-    int grid = norm_grid(s, a.n, sms);
-    grid = grid < sms * BWD_BLOCKS_PER_SM ? grid : sms * BWD_BLOCKS_PER_SM;
+    int grid = norm_grid(s, a.n, sms, 1);
+    const int most = sms * (s.nv >= 4 ? 2 : BWD_BLOCKS_PER_SM);
+    grid = grid < most ? grid : most;
     const size_t sm = (size_t)(s.threads / 32) * a.d * sizeof(float);   // at most 8 x 1024 floats
     if (s.loop) rmsnorm_bwd_long_kernel<T><<<grid, 256, 0, st>>>(a);
     else if (s.vec == 1) {
@@ -454,8 +505,8 @@ int ffn_rmsnorm(const void* x, int64_t x_ld, const void* residual, int64_t resid
     const size_t z = dtype == FFN_F32 ? 4 : 2;
     const int vec = (int)(16 / z);
     const bool aligned = d % vec == 0 && x_ld % vec == 0 && (!residual || residual_ld % vec == 0) && op_aligned(x, 16) &&
-                         op_aligned(residual, 16) && op_aligned(h, 16) && op_aligned(y, out8 ? vec : 16);
-    NormArgs a{x, residual, gamma, h, y, scale, rstd, n, x_ld, residual_ld, d, group, 0, eps};
+                         op_aligned(residual, 16) && op_aligned(gamma, 16) && op_aligned(h, 16) && op_aligned(y, out8 ? vec : 16);
+    NormArgs a{x, residual, gamma, h, y, scale, rstd, n, x_ld, residual_ld, d, group, 0, group == 32 ? 5 : group == 64 ? 6 : 7, eps};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == FFN_F32) return out8 ? norm_launch<float, true>(a, aligned, st) : norm_launch<float, false>(a, aligned, st);
     if (dtype == FFN_F16) return out8 ? norm_launch<__half, true>(a, aligned, st) : norm_launch<__half, false>(a, aligned, st);
@@ -491,7 +542,7 @@ int ffn_rmsnorm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, 
     const int vec = dtype == FFN_F32 ? 4 : 8;
     const bool aligned = d % vec == 0 && dy_ld % vec == 0 && x_ld % vec == 0 && (!residual || residual_ld % vec == 0) &&
                          (!dresidual || dresidual_ld % vec == 0) && op_aligned(dy, 16) && op_aligned(x, 16) &&
-                         op_aligned(residual, 16) && op_aligned(dresidual, 16) && op_aligned(dx, 16);
+                         op_aligned(residual, 16) && op_aligned(dresidual, 16) && op_aligned(gamma, 16) && op_aligned(dx, 16);
     NormBwdArgs a{dy, x, residual, dresidual, gamma, rstd, dx, static_cast<float*>(workspace), n,
                   dy_ld, x_ld, residual_ld, dresidual_ld, d, 0};
     if (dtype == FFN_F32) return norm_bwd_launch<float>(a, dgamma, aligned, st);

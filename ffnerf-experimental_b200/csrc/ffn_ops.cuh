@@ -3,6 +3,7 @@
 #pragma once
 #include <cstdint>
 #include <string>
+#include <type_traits>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -43,7 +44,7 @@ template <> __device__ __forceinline__ float from_f<float>(float v) { return v; 
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// N consecutive elements as one access of N * sizeof(T) bytes (4, 8 or 16; or one element).
+// N consecutive elements as one access of N * sizeof(T) bytes (2, 4, 8 or 16).
 template <int BYTES> struct Raw;
 template <> struct Raw<2> { using type = unsigned short; };
 template <> struct Raw<4> { using type = unsigned int; };
@@ -55,16 +56,69 @@ struct alignas(sizeof(T) * N) Pack {
     T v[N];
 };
 template <typename T, int N>
-__device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
-    using R = typename Raw<sizeof(T) * N>::type;
-    const R r = __ldg(reinterpret_cast<const R*>(p));
-    return *reinterpret_cast<const Pack<T, N>*>(&r);
-}
-template <typename T, int N>
 __device__ __forceinline__ void store_pack(T* p, const Pack<T, N>& v) {
     using R = typename Raw<sizeof(T) * N>::type;
     *reinterpret_cast<R*>(p) = *reinterpret_cast<const R*>(&v);
 }
+
+// 16 bytes of a row (or one element, N = 1) that stay packed in registers until they are used: pairs of
+// 16-bit values are widened and rounded two at a time.
+template <typename T, int N>
+struct Vec {
+    static_assert(N == 1 || sizeof(T) * N == 16, "one element or 16 bytes");
+    typename Raw<sizeof(T) * N>::type r;
+
+    __device__ __forceinline__ void clear() {
+        if constexpr (N == 1) r = 0;
+        else r = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void load(const T* p) { r = __ldg(reinterpret_cast<const decltype(r)*>(p)); }
+    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<decltype(r)*>(p) = r; }
+
+    static __device__ __forceinline__ float2 widen(uint32_t w) {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+        else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    }
+    static __device__ __forceinline__ uint32_t narrow(float a, float b) {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+            return *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+            const __half2 h = __floats2half2_rn(a, b);
+            return *reinterpret_cast<const uint32_t*>(&h);
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[N]) const {
+        if constexpr (N == 1) {
+            v[0] = to_f(*reinterpret_cast<const T*>(&r));
+        } else {
+            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(w[i]);
+                else {
+                    const float2 f = widen(w[i]);
+                    v[2 * i] = f.x;
+                    v[2 * i + 1] = f.y;
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void put(const float (&v)[N]) {
+        if constexpr (N == 1) {
+            const T t = from_f<T>(v[0]);
+            r = *reinterpret_cast<const decltype(r)*>(&t);
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(v[i]);
+                else w[i] = narrow(v[2 * i], v[2 * i + 1]);
+            }
+            r = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+};
 
 // Maximum that keeps a NaN (fmaxf drops it): a row with a NaN has to get a NaN scale.
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -75,15 +129,17 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 
 constexpr float E4M3_MAX = 448.0f;
 
-// The scale of values whose largest magnitude is `top`, and the factor that applies it.  A scale that
-// would be zero is 1 (the values are then zero, or vanish); a factor that would be infinite (scales
-// below 2^-128) is the largest finite one, so that a zero stays a zero.  A NaN stays a NaN.
+// The scale of values whose largest magnitude is `top` (top / 448 to an ulp or two), and the factor that
+// applies it.  A scale that would be zero is 1 (the values are then zero, or vanish); a factor that would
+// be infinite (scales below 2^-126) is the largest finite one, so that a zero stays a zero.  A NaN stays
+// a NaN.  The approximate reciprocal is off by an ulp: what it scales is rounded to four bits.
 __device__ __forceinline__ float e4m3_scale(float top) {
-    const float s = __fdiv_rn(top, E4M3_MAX);
+    const float s = top * (1.0f / E4M3_MAX);
     return s == 0.0f ? 1.0f : s;
 }
 __device__ __forceinline__ float e4m3_inverse(float scale) {
-    const float v = __fdiv_rn(1.0f, scale);
+    float v;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(v) : "f"(scale));
     return v > 3.402823466e38f ? 3.402823466e38f : v;
 }
 
