@@ -11,8 +11,8 @@
 // tiles of all experts, which it finds from the offsets on the device (the host never reads them, so a
 // call synchronises nothing and can be captured in a graph).  Warp roles: one thread issues TMA loads
 // into a ring of shared-memory stages (128 bytes of depth each, 128-byte swizzle), one warp issues
-// tcgen05.mma into one of two accumulators in tensor memory, four warps read the other accumulator,
-// scale, convert and store it, so loads, products and stores of neighbouring tiles overlap.
+// tcgen05.mma into one of two accumulators in tensor memory, and two groups of four warps, one for each
+// accumulator, read, scale, convert and store it, so loads, products and stores of neighbouring tiles overlap.
 //
 //   forward  A = x rows,           B = W rows           both with depth k contiguous
 //   few rows A = W rows (128), B = x rows (16 to 64): the weights fill the tensor core's 128 lanes, the
@@ -37,7 +37,7 @@ enum { FORWARD = 0, INPUT_GRAD = 1, WEIGHT_GRAD = 2, FEW_ROWS = 3 };
 
 constexpr int BM = 128;                    // lanes of an accumulator
 constexpr int KB = 128;                    // bytes of depth in a stage (K-major), or 64 rows (MN-major)
-constexpr int EPI_WARPS = 4;
+constexpr int EPI_WARPS = 8;               // two groups of four, one accumulator each
 constexpr int THREADS = 32 * (EPI_WARPS + 2);
 constexpr int SLAB = 32 * 128;             // one warp's 32 rows x 128 bytes of output
 constexpr size_t SMEM_MOST = 232448;       // what a block may have
@@ -53,7 +53,15 @@ struct Args {
     int experts, cols, depth, rows_m;      // cols: width of the output; rows_m: dW's rows
     int ntiles, mtiles;                    // tiles along the output's width; dW's tiles along its rows
     int tma_out;                           // the output can be stored by TMA (16-byte rows)
+    int most;                              // tiles over the rows (dW: units) that valid offsets give at most
+    int chunk;                             // dW: stages of depth of a unit (0: an expert's depth is one unit)
 };
+
+// Units that an expert's rows make in dW: chunks of depth, one at least (its output has to be written).
+__host__ __device__ __forceinline__ int units_of(int64_t rows, int chunk) {
+    const int blocks = (int)((rows + 63) / 64);
+    return chunk == 0 || blocks <= chunk ? 1 : (blocks + chunk - 1) / chunk;
+}
 
 // An expert's rows, kept inside [0, n] whatever the offsets hold.
 __device__ __forceinline__ void expert_rows(const Args& p, int e, int64_t& b, int64_t& end) {
@@ -128,7 +136,7 @@ struct Plan {
     static constexpr int A_BYTES = BM * KB;
     static constexpr int B_BYTES = BN * KB;
     static constexpr int STAGE = A_BYTES + B_BYTES;
-    static constexpr int EPI = MODE == FEW_ROWS ? 0 : EPI_WARPS * 2 * SLAB;
+    static constexpr int EPI = MODE == FEW_ROWS ? 0 : EPI_WARPS * SLAB;
     static constexpr int MISC = 1024 + 4 * (FFN_MAX_EXPERTS + 1) + 512;   // alignment, prefix, barriers
     static constexpr int FIT = (int)((SMEM_MOST - EPI - MISC) / STAGE);
     static constexpr int STAGES = FIT > 12 ? 12 : FIT;
@@ -142,37 +150,39 @@ struct Tile {
     int e, blocks;               // expert, stages of depth
     int64_t row, end;            // first row of the tile (of the depth in dW), end of the expert's rows
     int col, mrow;               // first output column; dW: first output row
+    int plane;                   // dW: which matrix of the output
 };
 
 template <int MODE, int BN, int EB>
 __device__ __forceinline__ Tile find_tile(const Args& p, const int* prefix, int t) {
     Tile k;
     int64_t b, end;
+    const int per = MODE == WEIGHT_GRAD ? p.ntiles * p.mtiles : p.ntiles;
+    const int q = t / per;
+    int lo = 0, hi = p.experts;                        // prefix[lo] <= q < prefix[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (prefix[mid] <= q) lo = mid; else hi = mid;
+    }
+    k.e = lo;
     if constexpr (MODE == WEIGHT_GRAD) {
-        const int per = p.ntiles * p.mtiles;
-        k.e = t / per;
-        const int r = t - k.e * per;
+        const int r = t - q * per, u = q - prefix[lo];
         k.mrow = (r % p.mtiles) * BM;
         k.col = (r / p.mtiles) * BN;
-        expert_rows(p, k.e, b, end);
-        k.row = b;
+        expert_rows(p, lo, b, end);
+        k.row = b + (int64_t)u * p.chunk * 64;
         k.end = end;
-        k.blocks = (int)((end - b + 63) / 64);
+        k.blocks = (int)((end - b + 63) / 64) - u * p.chunk;
+        if (p.chunk && k.blocks > p.chunk) k.blocks = p.chunk;
+        k.plane = p.chunk ? q : lo;
     } else {
-        const int q = t / p.ntiles;
-        int lo = 0, hi = p.experts;                    // prefix[lo] <= q < prefix[hi]
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (prefix[mid] <= q) lo = mid; else hi = mid;
-        }
-        k.e = lo;
         const int tiles = prefix[lo + 1] - prefix[lo], r = t - prefix[lo] * p.ntiles;
         expert_rows(p, lo, b, end);
         // neighbouring blocks take the same weights and the expert's row tiles in turn
         k.row = b + (int64_t)(r % tiles) * (MODE == FEW_ROWS ? BN : BM);
         k.col = (r / tiles) * (MODE == FEW_ROWS ? BM : BN);
         k.end = end;
-        k.mrow = 0;
+        k.mrow = k.plane = 0;
         constexpr int D = Plan<MODE, BN, EB>::DEPTH;
         k.blocks = (p.depth + D - 1) / D;
     }
@@ -212,43 +222,38 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
         tc::tmem_alloc(tmem_at, P::TMEM_COLS);
         if (lane == 0) {
             for (int i = 0; i < S; ++i) { tc::mbar_init(full + i, 1); tc::mbar_init(empty + i, 1); }
-            for (int i = 0; i < 2; ++i) { tc::mbar_init(done + i, 1); tc::mbar_init(freed + i, EPI_WARPS); }
+            for (int i = 0; i < 2; ++i) { tc::mbar_init(done + i, 1); tc::mbar_init(freed + i, 4); }
             *gone = 0;
         }
     }
-    int total;
-    if constexpr (MODE == WEIGHT_GRAD) {
-        total = p.experts * p.ntiles * p.mtiles;
-    } else {
-        // tiles of the experts before each: counts side by side, then one warp adds them up
-        constexpr int R = MODE == FEW_ROWS ? BN : BM;
-        for (int e = threadIdx.x; e < p.experts; e += THREADS) {
-            int64_t b, end;
-            expert_rows(p, e, b, end);
-            prefix[e + 1] = (int)((end - b + R - 1) / R);
-        }
-        __syncthreads();
-        if (warp == 0) {
-            // valid offsets give at most `most` tiles; sums stop there, so that offsets that are not
-            // (decreasing ones, whose experts overlap) cannot wrap
-            const int most = (int)(p.n / R) + p.experts;
-            int sum = 0;
-            for (int e0 = 0; e0 < p.experts; e0 += 32) {
-                int v = e0 + lane < p.experts ? prefix[e0 + lane + 1] : 0;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int u = __shfl_up_sync(0xffffffffu, v, o);
-                    if (lane >= o) v = min(v + u, most);
-                }
-                v = min(sum + v, most);
-                if (e0 + lane < p.experts) prefix[e0 + lane + 1] = v;
-                sum = __shfl_sync(0xffffffffu, v, 31);
-            }
-            if (lane == 0) prefix[0] = 0;
-        }
-        __syncthreads();
-        total = prefix[p.experts] * p.ntiles;
+    // tiles (dW: units) of the experts before each: counts side by side, then one warp adds them up
+    constexpr int R = MODE == FEW_ROWS ? BN : BM;
+    for (int e = threadIdx.x; e < p.experts; e += THREADS) {
+        int64_t b, end;
+        expert_rows(p, e, b, end);
+        prefix[e + 1] = MODE == WEIGHT_GRAD ? units_of(end - b, p.chunk) : (int)((end - b + R - 1) / R);
     }
+    __syncthreads();
+    if (warp == 0) {
+        // valid offsets give at most `most` tiles; sums stop there, so that offsets that are not
+        // (decreasing ones, whose experts overlap) cannot wrap
+        const int most = p.most;
+        int sum = 0;
+        for (int e0 = 0; e0 < p.experts; e0 += 32) {
+            int v = e0 + lane < p.experts ? prefix[e0 + lane + 1] : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v = min(v + u, most);
+            }
+            v = min(sum + v, most);
+            if (e0 + lane < p.experts) prefix[e0 + lane + 1] = v;
+            sum = __shfl_sync(0xffffffffu, v, 31);
+        }
+        if (lane == 0) prefix[0] = 0;
+    }
+    __syncthreads();
+    const int total = prefix[p.experts] * (MODE == WEIGHT_GRAD ? p.ntiles * p.mtiles : p.ntiles);
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
@@ -351,23 +356,23 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
             if (++acc == 2) { acc = 0; aph ^= 1; }
         }
     } else {                                                      // ---- results
-        int acc = 0, buf = 0;
+        const int acc = warp >> 2, quarter = warp & 3;            // this group's accumulator, this warp's lanes
         uint32_t aph = 0;
         TO* out = static_cast<TO*>(p.out);
-        unsigned char* slab = slabs + warp * 2 * SLAB;
-        for (int t = blockIdx.x; t < total; t += gridDim.x) {
+        unsigned char* sl = slabs + warp * SLAB;
+        for (int t = blockIdx.x + acc * gridDim.x; t < total; t += 2 * gridDim.x) {
             const Tile k = find_tile<MODE, BN, EB>(p, prefix, t);
-            const int64_t row = (MODE == WEIGHT_GRAD ? k.mrow : k.row) + warp * 32;     // this warp's first row
+            const int64_t row = (MODE == WEIGHT_GRAD ? k.mrow : k.row) + quarter * 32;  // this warp's first row
             const int64_t end = MODE == WEIGHT_GRAD ? p.rows_m : k.end;
             float sr = 1.0f;
             if constexpr (EB == 1 && MODE == FORWARD) sr = row + lane < end ? __ldg(p.a_scale + row + lane) : 0.0f;
             if (!wait(done + acc, aph, gone)) break;
             tc::fence_after_sync();
-            const uint32_t d = tmem + acc * P::ACC_COLS + ((uint32_t)(warp * 32) << 16);
+            const uint32_t d = tmem + acc * P::ACC_COLS + ((uint32_t)(quarter * 32) << 16);
             const bool none = MODE == WEIGHT_GRAD && k.blocks == 0;
             if constexpr (MODE == FEW_ROWS) {
                 // a lane is an output column, a column of the accumulator a row
-                const int col = k.col + warp * 32 + lane;
+                const int col = k.col + quarter * 32 + lane;
                 const int rows = (int)min((int64_t)BN, k.end - k.row);
                 float sc = 1.0f;
                 if constexpr (EB == 1) sc = col < p.cols ? __ldg(p.b_scale + (int64_t)k.e * p.cols + col) : 0.0f;
@@ -414,9 +419,8 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
                             for (int j = 0; j < 32; ++j) pk[j] = 0u;
                     }
                     // the slab's previous store has been read out of shared memory
-                    if (lane == 0) bulk_wait_read<1>();
+                    if (lane == 0) bulk_wait_read<0>();
                     __syncwarp();
-                    unsigned char* sl = slab + buf * SLAB;
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                         *reinterpret_cast<uint4*>(sl + lane * 128 + ((j ^ (lane & 7)) << 4)) =
@@ -425,12 +429,13 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
                         tc::fence_proxy_async();
                         __syncwarp();
                         if (lane == 0) {
-                            if constexpr (MODE == WEIGHT_GRAD) tma_store3(&mo, col, (int)row, k.e, tc::smem_u32(sl));
+                            if constexpr (MODE == WEIGHT_GRAD) tma_store3(&mo, col, (int)row, k.plane, tc::smem_u32(sl));
                             else tma_store2(&mo, col, (int)row, tc::smem_u32(sl));
+                            bulk_commit();
                         }
                     } else {
                         __syncwarp();
-                        TO* o = out + (MODE == WEIGHT_GRAD ? (int64_t)k.e * p.rows_m * p.cols : 0) + row * p.cols + col;
+                        TO* o = out + (MODE == WEIGHT_GRAD ? (int64_t)k.plane * p.rows_m * p.cols : 0) + row * p.cols + col;
                         const int cols = min(W, p.cols - col);
                         if (p.tma_out) {                          // rows are multiples of 16 bytes
                             for (int i = lane; i < live * 8; i += 32) {
@@ -449,14 +454,12 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
                         }
                         __syncwarp();
                     }
-                    if (lane == 0) bulk_commit();
-                    buf ^= 1;
                 }
             }
             tc::fence_before_sync();
             __syncwarp();
             if (lane == 0) arrive(freed + acc);
-            if (++acc == 2) { acc = 0; aph ^= 1; }
+            aph ^= 1;
         }
         if (lane == 0) bulk_wait_read<0>();
         if constexpr (MODE != WEIGHT_GRAD) {                      // rows of no expert
@@ -549,6 +552,9 @@ Operand pad(const void* p, int64_t ld, int64_t rows, int cols, int dtype, unsign
     return o;
 }
 
+// The most units that n rows make.
+int64_t units_most(int64_t n, int experts, int chunk) { return chunk ? n / (64 * (int64_t)chunk) + experts : experts; }
+
 template <int MODE, int BN, int EB, typename TO, bool BF>
 int launch(const Args& a0, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, int sms, cudaStream_t st) {
     using P = Plan<MODE, BN, EB>;
@@ -557,8 +563,9 @@ int launch(const Args& a0, const CUtensorMap& ma, const CUtensorMap& mb, const C
     a.ntiles = (a.cols + NT - 1) / NT;
     a.mtiles = (a.rows_m + BM - 1) / BM;
     // an upper bound of the tiles: the counts are on the device
-    const int64_t tiles = MODE == WEIGHT_GRAD ? (int64_t)a.experts * a.ntiles * a.mtiles
-                                              : (a.n / RT + a.experts) * (int64_t)a.ntiles;
+    const int64_t most = MODE == WEIGHT_GRAD ? units_most(a.n, a.experts, a.chunk) : a.n / RT + a.experts;
+    const int64_t tiles = most * a.ntiles * (MODE == WEIGHT_GRAD ? a.mtiles : 1);
+    a.most = (int)most;
     if (tiles > 0x7fffffff) return op_fail(FFN_E_CAPACITY, "ffn_expert_mm: more than 2^31 output tiles");
     auto k = experts_kernel<MODE, BN, EB, TO, BF>;
     static std::atomic<uint64_t> ready{0};            // devices whose limit is set
@@ -598,7 +605,9 @@ int tile_width(int cols) { return cols > 128 ? 256 : cols > 64 ? 128 : 64; }
 // out[r] = a[r] b[e]^T (FORWARD, FEW_ROWS) or a[r] b[e] (INPUT_GRAD); depth and cols are those of the product.
 int rows_product(int mode, Operand a, Operand b, const float* a_scale, const float* b_scale, const int32_t* offsets, void* out,
                  int64_t n, int experts, int depth, int cols, int dtype, int out_dtype, int sms, cudaStream_t st) {
-    Args p{offsets, a_scale, b_scale, out, n, experts, cols, depth, 0, 0, 0, 0};
+    Args p{};
+    p.offsets = offsets; p.a_scale = a_scale; p.b_scale = b_scale; p.out = out;
+    p.n = n; p.experts = experts; p.cols = cols; p.depth = depth;
     p.tma_out = op_aligned(out, 16) && (int64_t)cols * 2 % 16 == 0;
     CUtensorMap ma, mb, mo{};
     if (mode == FEW_ROWS) {
@@ -625,17 +634,81 @@ int rows_product(int mode, Operand a, Operand b, const float* a_scale, const flo
                      : launch_typed<INPUT_GRAD, 64>(p, ma, mb, mo, dtype, out_dtype, sms, st);
 }
 
+// Sums the units of each expert in order: dw[e] = sum of part[unit], fp32 to TO.
+template <typename TO>
+__global__ void __launch_bounds__(256) units_sum_kernel(const Args p, const float* __restrict__ part, TO* __restrict__ dw,
+                                                        int64_t size) {
+    __shared__ int counts[FFN_MAX_EXPERTS];
+    __shared__ int first;
+    const int e = blockIdx.y;
+    for (int i = threadIdx.x; i <= e; i += 256) {
+        int64_t b, end;
+        expert_rows(p, i, b, end);
+        counts[i] = units_of(end - b, p.chunk);
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        int v = 0;
+        for (int i = threadIdx.x; i < e; i += 32) v = min(v + counts[i], p.most);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v = min(v + __shfl_xor_sync(0xffffffffu, v, o), p.most);
+        if (threadIdx.x == 0) first = v;
+    }
+    __syncthreads();
+    const int units = min(counts[e], p.most - first);
+    const float* src = part + (int64_t)first * size;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.x * 256) {
+        float v = 0.0f;
+        for (int u = 0; u < units; ++u) v += src[(int64_t)u * size + i];
+        dw[(int64_t)e * size + i] = from_f<TO>(v);
+    }
+}
+
+// Stages of depth in a unit of dW, or 0.  Experts share the rows unevenly and a small W has few output
+// tiles: 64 experts of 64 x 64 have 64, the largest of them several times the average depth.  Below two
+// tiles an SM the depth is cut into units, about four an SM in all and 16 stages at least, whose fp32
+// sums go through the workspace.
+int weight_chunk(int64_t n, int experts, int k, int m, int sms) {
+    const int bn = tile_width(k);
+    const int64_t per = (int64_t)((m + BM - 1) / BM) * ((k + bn - 1) / bn), blocks = n / 64 + experts;
+    if (per * experts >= 2 * (int64_t)sms) return 0;
+    const int64_t chunk = (blocks * per + 4 * sms - 1) / (4 * sms);
+    const int64_t c = chunk > 16 ? chunk : 16;
+    return blocks <= c * experts ? 0 : (int)c;
+}
+uint64_t weight_workspace(int64_t n, int experts, int k, int m, int sms) {
+    const int chunk = sms > 0 ? weight_chunk(n, experts, k, m, sms) : 0;
+    return chunk ? ((uint64_t)units_most(n, experts, chunk) * m * k * 4 + 255) / 256 * 256 : 0;
+}
+
 int weight_product(Operand dy, Operand x, const int32_t* offsets, void* dw, int64_t n, int experts, int k, int m, int dtype,
-                   int dw_dtype, int sms, cudaStream_t st) {
-    Args p{offsets, nullptr, nullptr, dw, n, experts, k, 0, m, 0, 0, 0};
-    p.tma_out = op_aligned(dw, 16) && (int64_t)k * (int64_t)type_size(dw_dtype) % 16 == 0;
+                   int dw_dtype, unsigned char* ws, int sms, cudaStream_t st) {
+    Args p{};
+    p.offsets = offsets; p.n = n; p.experts = experts; p.cols = k; p.rows_m = m;
+    p.chunk = weight_chunk(n, experts, k, m, sms);
+    const int out_type = p.chunk ? (int)FFN_F32 : dw_dtype;
+    void* out = p.chunk ? ws : dw;
+    p.out = out;
+    p.tma_out = op_aligned(out, 16) && (int64_t)k * (int64_t)type_size(out_type) % 16 == 0;
     CUtensorMap ma, mb, mo{};
-    if (p.tma_out && !make_map(&mo, dw, dw_dtype, k, m, k, experts, 32)) return bad_map();
+    if (p.tma_out && !make_map(&mo, out, out_type, k, m, k, units_most(n, experts, p.chunk), 32)) return bad_map();
     if (!make_map(&ma, dy.p, dtype, m, n, dy.ld, 0, 64) || !make_map(&mb, x.p, dtype, k, n, x.ld, 0, 64)) return bad_map();
     const int bn = tile_width(k);
-    return bn == 256 ? launch_typed<WEIGHT_GRAD, 256>(p, ma, mb, mo, dtype, dw_dtype, sms, st)
-         : bn == 128 ? launch_typed<WEIGHT_GRAD, 128>(p, ma, mb, mo, dtype, dw_dtype, sms, st)
-                     : launch_typed<WEIGHT_GRAD, 64>(p, ma, mb, mo, dtype, dw_dtype, sms, st);
+    const int rc = bn == 256 ? launch_typed<WEIGHT_GRAD, 256>(p, ma, mb, mo, dtype, out_type, sms, st)
+                 : bn == 128 ? launch_typed<WEIGHT_GRAD, 128>(p, ma, mb, mo, dtype, out_type, sms, st)
+                             : launch_typed<WEIGHT_GRAD, 64>(p, ma, mb, mo, dtype, out_type, sms, st);
+    if (rc != FFN_OK || !p.chunk) return rc;
+    const int64_t size = (int64_t)m * k;
+    p.most = (int)units_most(n, experts, p.chunk);
+    int64_t bx = (size + 255) / 256;
+    const int64_t cap = (8 * (int64_t)sms + experts - 1) / experts;
+    if (bx > cap) bx = cap;
+    const dim3 grid((unsigned)bx, (unsigned)experts);
+    const float* part = reinterpret_cast<const float*>(ws);
+    if (dw_dtype == FFN_F32) units_sum_kernel<float><<<grid, 256, 0, st>>>(p, part, static_cast<float*>(dw), size);
+    else if (dw_dtype == FFN_F16) units_sum_kernel<__half><<<grid, 256, 0, st>>>(p, part, static_cast<__half*>(dw), size);
+    else units_sum_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p, part, static_cast<__nv_bfloat16*>(dw), size);
+    return op_launched("ffn_expert_mm_bwd sums");
 }
 
 int check(const char* who, int64_t n, int32_t experts, int32_t k, int32_t m) {
@@ -684,7 +757,7 @@ int ffn_expert_mm(const void* x, int64_t x_ld, const void* w, const int32_t* off
 uint64_t ffn_expert_mm_bwd_workspace(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, const void* w, int64_t n,
                                      int32_t experts, int32_t k, int32_t m, int dtype) {
     return pad_bytes(dy, dy_ld, n, m, dtype) + pad_bytes(x, x_ld, n, k, dtype) +
-           pad_bytes(w, k, (int64_t)experts * m, k, dtype);
+           pad_bytes(w, k, (int64_t)experts * m, k, dtype) + weight_workspace(n, experts, k, m, op_sms());
 }
 
 int ffn_expert_mm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, const void* w, const int32_t* offsets,
@@ -719,7 +792,7 @@ int ffn_expert_mm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld
     }
     if (dw) {
         const Operand b = pad(x, x_ld, n, k, dtype, ws, sms, st);
-        if (int rc = weight_product(a, b, offsets, dw, n, experts, k, m, dtype, dw_dtype, sms, st)) return rc;
+        if (int rc = weight_product(a, b, offsets, dw, n, experts, k, m, dtype, dw_dtype, ws, sms, st)) return rc;
     }
     return FFN_OK;
 }

@@ -357,7 +357,8 @@ int ffn_expert_mm(const void* x, int64_t x_ld, const void* w, const int32_t* off
                   const float* w_scale, void* y, int64_t n, int32_t experts, int32_t k, int32_t m, int dtype,
                   int out_dtype, void* workspace, uint64_t workspace_bytes, void* stream);
 /* Both gradients (either may be NULL): dx[r] = dy[r] w[e] in dtype, and dw[e] = the sum over the
- * expert's rows of dy[r]^T x[r], in dtype or fp32 (dw_dtype); an expert without rows gets zeros. */
+ * expert's rows of dy[r]^T x[r], in dtype or fp32 (dw_dtype); an expert without rows gets zeros.  The
+ * sums' order is fixed.  The workspace also holds partial sums where W is small and rows are many. */
 uint64_t ffn_expert_mm_bwd_workspace(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, const void* w,
                                      int64_t n, int32_t experts, int32_t k, int32_t m, int dtype);
 int ffn_expert_mm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, const void* w, const int32_t* offsets,
