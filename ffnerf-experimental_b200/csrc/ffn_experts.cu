@@ -153,41 +153,76 @@ struct Tile {
     int plane;                   // dW: which matrix of the output
 };
 
-template <int MODE, int BN, int EB>
-__device__ __forceinline__ Tile find_tile(const Args& p, const int* prefix, int t) {
-    Tile k;
-    int64_t b, end;
-    const int per = MODE == WEIGHT_GRAD ? p.ntiles * p.mtiles : p.ntiles;
-    const int q = t / per;
-    int lo = 0, hi = p.experts;                        // prefix[lo] <= q < prefix[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (prefix[mid] <= q) lo = mid; else hi = mid;
-    }
-    k.e = lo;
-    if constexpr (MODE == WEIGHT_GRAD) {
-        const int r = t - q * per, u = q - prefix[lo];
-        k.mrow = (r % p.mtiles) * BM;
-        k.col = (r / p.mtiles) * BN;
-        expert_rows(p, lo, b, end);
-        k.row = b + (int64_t)u * p.chunk * 64;
-        k.end = end;
-        k.blocks = (int)((end - b + 63) / 64) - u * p.chunk;
-        if (p.chunk && k.blocks > p.chunk) k.blocks = p.chunk;
-        k.plane = p.chunk ? q : lo;
-    } else {
-        const int tiles = prefix[lo + 1] - prefix[lo], r = t - prefix[lo] * p.ntiles;
-        expert_rows(p, lo, b, end);
-        // neighbouring blocks take the same weights and the expert's row tiles in turn
-        k.row = b + (int64_t)(r % tiles) * (MODE == FEW_ROWS ? BN : BM);
-        k.col = (r / tiles) * (MODE == FEW_ROWS ? BM : BN);
-        k.end = end;
-        k.mrow = k.plane = 0;
-        constexpr int D = Plan<MODE, BN, EB>::DEPTH;
-        k.blocks = (p.depth + D - 1) / D;
-    }
-    return k;
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+// One lane of a converged warp, chosen so that the compiler keeps what that lane issues on the uniform path
+// (descriptors and coordinates in uniform registers: an instruction for the tensor core or the copy engine
+// costs a few cycles to issue, and about sixty when it is issued from a divergent branch).
+__device__ __forceinline__ bool elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.b32 %0, 1, 0, q;\n\t}\n" : "=r"(p));
+    return p != 0;
 }
+
+// Each role goes through this block's tiles in the same order; the walk keeps the expert it is at, so
+// that the next tile costs a comparison, and offsets are read only where the expert changes.
+template <int MODE, int BN, int EB>
+struct Walk {
+    int e = 0, start = 0, stop = 0;      // this expert's tiles are start .. stop - 1
+    int64_t b = 0, end = 0;              // its rows
+    int known = -1;                      // the expert that b and end belong to
+
+    __device__ __forceinline__ Tile at(const Args& p, const int* prefix, int t) {
+        const int per = MODE == WEIGHT_GRAD ? p.ntiles * p.mtiles : p.ntiles;
+        if (known < 0) stop = prefix[1] * per;
+        for (int i = 0; t >= stop; ++i) {
+            if (i < 4) {
+                ++e;
+            } else {                     // many experts without rows: prefix[lo] * per <= t < prefix[hi] * per
+                int lo = e, hi = p.experts;
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (prefix[mid] * per <= t) lo = mid; else hi = mid;
+                }
+                e = lo;
+            }
+            start = prefix[e] * per;
+            stop = prefix[e + 1] * per;
+        }
+        if (known != e) {
+            expert_rows(p, e, b, end);
+            known = e;
+        }
+        Tile k;
+        k.e = e;
+        k.end = end;
+        int r = t - start;
+        if constexpr (MODE == WEIGHT_GRAD) {
+            int u = r;
+            if (per > 1) { u = r / per; r -= u * per; } else r = 0;
+            const int c = p.mtiles > 1 ? r / p.mtiles : r;
+            k.mrow = (r - c * p.mtiles) * BM;
+            k.col = c * BN;
+            k.row = b + (int64_t)u * p.chunk * 64;
+            k.blocks = (int)((end - b + 63) / 64) - u * p.chunk;
+            if (p.chunk && k.blocks > p.chunk) k.blocks = p.chunk;
+            k.plane = p.chunk ? prefix[e] + u : e;
+        } else {
+            // neighbouring blocks take the same weights and the expert's row tiles in turn
+            int c = 0;
+            if (per > 1) {
+                const int tiles = prefix[e + 1] - prefix[e];
+                c = r / tiles;
+                r -= c * tiles;
+            }
+            k.row = b + (int64_t)r * (MODE == FEW_ROWS ? BN : BM);
+            k.col = c * (MODE == FEW_ROWS ? BM : BN);
+            k.mrow = k.plane = 0;
+            constexpr int D = Plan<MODE, BN, EB>::DEPTH;
+            k.blocks = (p.depth + D - 1) / D;
+        }
+        return k;
+    }
+};
 
 // Waits for a phase of an mbarrier; false when the wait ran out here or in another role of the block.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* gone) {
@@ -260,75 +295,92 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
 
     if (warp == EPI_WARPS) {                                     // ---- loads
-        if (lane == 0) {
-            int s = 0, issued = 0;
-            uint32_t ph = 1;
-            bool ok = true;
-            for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-                const Tile k = find_tile<MODE, BN, EB>(p, prefix, t);
-                for (int b = 0; b < k.blocks; ++b) {
-                    if (!(ok = wait(empty + s, ph, gone))) break;
-                    const uint32_t sa = tc::smem_u32(base + (size_t)s * P::STAGE), sb = sa + P::A_BYTES;
+        Walk<MODE, BN, EB> walk;
+        int s = 0, issued = 0;
+        uint32_t ph = 1;
+        bool ok = true;
+        for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+            const Tile k = walk.at(p, prefix, t);
+            const int blocks = uniform(k.blocks), row = uniform((int)k.row), col = uniform(k.col), e = uniform(k.e);
+            [[maybe_unused]] const int mrow = uniform(k.mrow);
+            for (int b = 0; b < blocks; ++b) {
+                if (!(ok = wait(empty + s, ph, gone))) break;
+                const uint32_t sa = tc::smem_u32(base + (size_t)s * P::STAGE), sb = sa + P::A_BYTES;
+                if (elect()) {
                     if constexpr (MODE == FORWARD) {
                         expect_tx(full + s, P::STAGE);
-                        tma_load2(sa, &ma, b * P::DEPTH, (int)k.row, full + s);
-                        tma_load3(sb, &mb, b * P::DEPTH, k.col, k.e, full + s);
+                        tma_load2(sa, &ma, b * P::DEPTH, row, full + s);
+                        tma_load3(sb, &mb, b * P::DEPTH, col, e, full + s);
                     } else if constexpr (MODE == FEW_ROWS) {
                         expect_tx(full + s, P::STAGE);
-                        tma_load3(sa, &ma, b * P::DEPTH, k.col, k.e, full + s);
-                        tma_load2(sb, &mb, b * P::DEPTH, (int)k.row, full + s);
+                        tma_load3(sa, &ma, b * P::DEPTH, col, e, full + s);
+                        tma_load2(sb, &mb, b * P::DEPTH, row, full + s);
                     } else {
                         // boxes of 64 columns; those wholly outside the matrix are left out (what is in
                         // their place reaches only outputs that are not stored)
-                        const int nb = min(BN / 64, (p.cols - k.col + 63) / 64);
+                        const int nb = min(BN / 64, (p.cols - col + 63) / 64);
                         if constexpr (MODE == INPUT_GRAD) {
                             expect_tx(full + s, P::A_BYTES + nb * 8192);
-                            tma_load2(sa, &ma, b * 64, (int)k.row, full + s);
-                            for (int j = 0; j < nb; ++j) tma_load3(sb + j * 8192, &mb, k.col + j * 64, b * 64, k.e, full + s);
+                            tma_load2(sa, &ma, b * 64, row, full + s);
+#pragma unroll
+                            for (int j = 0; j < BN / 64; ++j)
+                                if (j < nb) tma_load3(sb + j * 8192, &mb, col + j * 64, b * 64, e, full + s);
                         } else {
-                            const int na = min(BM / 64, (p.rows_m - k.mrow + 63) / 64);
+                            const int na = min(BM / 64, (p.rows_m - mrow + 63) / 64);
                             expect_tx(full + s, (na + nb) * 8192);
-                            for (int j = 0; j < na; ++j)
-                                tma_load2(sa + j * 8192, &ma, k.mrow + j * 64, (int)(k.row + b * 64), full + s);
-                            for (int j = 0; j < nb; ++j)
-                                tma_load2(sb + j * 8192, &mb, k.col + j * 64, (int)(k.row + b * 64), full + s);
+#pragma unroll
+                            for (int j = 0; j < BM / 64; ++j)
+                                if (j < na) tma_load2(sa + j * 8192, &ma, mrow + j * 64, row + b * 64, full + s);
+#pragma unroll
+                            for (int j = 0; j < BN / 64; ++j)
+                                if (j < nb) tma_load2(sb + j * 8192, &mb, col + j * 64, row + b * 64, full + s);
                         }
                     }
-                    ++issued;
-                    if (++s == S) { s = 0; ph ^= 1; }
                 }
+                __syncwarp();
+                ++issued;
+                if (++s == S) { s = 0; ph ^= 1; }
             }
-            if (!ok)                                              // let the copies in flight land
-                for (int i = 0; i < (issued < S ? issued : S); ++i) {
-                    const int q = issued - 1 - i;
-                    tc::mbar_wait(full + q % S, (uint32_t)(q / S) & 1u, 1u << 20);
-                }
         }
+        if (!ok)                                                  // let the copies in flight land
+            for (int i = 0; i < (issued < S ? issued : S); ++i) {
+                const int q = issued - 1 - i;
+                tc::mbar_wait(full + q % S, (uint32_t)(q / S) & 1u, 1u << 20);
+            }
     } else if (warp == EPI_WARPS + 1) {                           // ---- products
         constexpr bool A_MN = MODE == WEIGHT_GRAD, B_MN = MODE == INPUT_GRAD || MODE == WEIGHT_GRAD;
         constexpr uint32_t IDESC = tc::idesc_f16(BM, BN, A_MN, B_MN) |
                                    (EB == 2 && BF ? (1u << 7) | (1u << 10) : 0u);
+        Walk<MODE, BN, EB> walk;
         int s = 0, acc = 0;
         uint32_t ph = 0, aph = 1;
         bool ok = true;
         for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-            const Tile k = find_tile<MODE, BN, EB>(p, prefix, t);
+            int blocks;
+            [[maybe_unused]] int rows = 0;                        // dW: rows of depth from the tile's first on
+            if constexpr (MODE == WEIGHT_GRAD) {
+                const Tile k = walk.at(p, prefix, t);
+                blocks = uniform(k.blocks);
+                rows = uniform((int)min(k.end - k.row, (int64_t)0x7fffffff));
+            } else {
+                blocks = (p.depth + P::DEPTH - 1) / P::DEPTH;
+            }
             if (!(ok = wait(freed + acc, aph, gone))) break;
             tc::fence_after_sync();
             const uint32_t d = tmem + acc * P::ACC_COLS;
-            for (int b = 0; b < k.blocks; ++b) {
+            for (int b = 0; b < blocks; ++b) {
                 if (!(ok = wait(full + s, ph, gone))) break;
                 tc::fence_after_sync();
                 const uint32_t sa = tc::smem_u32(base + (size_t)s * P::STAGE), sb = sa + P::A_BYTES;
                 int steps = 4;
                 if constexpr (MODE == WEIGHT_GRAD) {
-                    const int64_t left = k.end - k.row - (int64_t)b * 64;
+                    const int left = rows - b * 64;
                     if (left < 64) {                              // rows of the next expert become zeros
-                        steps = ((int)left + 15) / 16;
-                        const int rows = steps * 16 - (int)left;
+                        steps = (left + 15) / 16;
+                        const int clear = steps * 16 - left;
                         constexpr int CH = (BM + BN) / 64;
-                        for (int i = lane; i < CH * rows * 8; i += 32) {
-                            const int ch = i / (rows * 8), r = (int)left + (i / 8) % rows;
+                        for (int i = lane; i < CH * clear * 8; i += 32) {
+                            const int ch = i / (clear * 8), r = left + (i / 8) % clear;
                             *reinterpret_cast<uint4*>(base + (size_t)s * P::STAGE + ch * 8192 + r * 128 + (i & 7) * 16) =
                                 make_uint4(0, 0, 0, 0);
                         }
@@ -336,7 +388,7 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
                         __syncwarp();
                     }
                 }
-                if (lane == 0) {
+                if (elect()) {
                     const uint64_t da = A_MN ? desc_sw128(sa, 8192, 1024) : desc_sw128(sa, 16, 1024);
                     const uint64_t db = B_MN ? desc_sw128(sb, 8192, 1024) : desc_sw128(sb, 16, 1024);
                     constexpr uint64_t STEP_A = (A_MN ? 2048 : 32) >> 4, STEP_B = (B_MN ? 2048 : 32) >> 4;
@@ -347,12 +399,15 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
                             else mma_16(d, da + i * STEP_A, db + i * STEP_B, IDESC, (b | i) != 0);
                         }
                     tc::commit(empty + s);
+                    if (b == blocks - 1) tc::commit(done + acc);
                 }
                 __syncwarp();
                 if (++s == S) { s = 0; ph ^= 1; }
             }
-            if (lane == 0 && ok) tc::commit(done + acc);
-            __syncwarp();
+            if (MODE == WEIGHT_GRAD && blocks == 0) {             // no rows: the output is zero
+                if (elect()) arrive(done + acc);
+                __syncwarp();
+            }
             if (++acc == 2) { acc = 0; aph ^= 1; }
         }
     } else {                                                      // ---- results
@@ -360,8 +415,9 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
         uint32_t aph = 0;
         TO* out = static_cast<TO*>(p.out);
         unsigned char* sl = slabs + warp * SLAB;
+        Walk<MODE, BN, EB> walk;
         for (int t = blockIdx.x + acc * gridDim.x; t < total; t += 2 * gridDim.x) {
-            const Tile k = find_tile<MODE, BN, EB>(p, prefix, t);
+            const Tile k = walk.at(p, prefix, t);
             const int64_t row = (MODE == WEIGHT_GRAD ? k.mrow : k.row) + quarter * 32;  // this warp's first row
             const int64_t end = MODE == WEIGHT_GRAD ? p.rows_m : k.end;
             float sr = 1.0f;
