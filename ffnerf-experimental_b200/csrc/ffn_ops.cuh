@@ -1,6 +1,7 @@
 // ffn_ops.cuh -- what the block operators (ffn_norm.cu, ffn_scan.cu, ffn_experts.cu) share: element
 // types, wide loads and stores, argument checks.  Each operator file is a translation unit of its own.
 #pragma once
+#include <atomic>
 #include <cstdint>
 #include <string>
 #include <type_traits>
@@ -24,11 +25,14 @@ inline int op_launched(const char* what) {
     return e == cudaSuccess ? FFN_OK : op_fail(FFN_E_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
 }
 
-// Streaming multiprocessors of the current device (the attribute query is cached by the runtime).
+// Streaming multiprocessors of the current device; 0 when there is none.
 inline int op_sms() {
+    static std::atomic<int> known[64];
     int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        return 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
     return n;
 }
 

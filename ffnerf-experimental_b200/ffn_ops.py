@@ -12,7 +12,6 @@ call by the caller.
 """
 from __future__ import annotations
 
-import functools
 from typing import NamedTuple
 
 import torch
@@ -24,41 +23,55 @@ SCAN_FORMS = {"linear": 0, "sigmoid": 1}
 DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3}
 _WIDE = (torch.float32, torch.float16, torch.bfloat16)
 
+# What torch.cuda.current_stream().cuda_stream and torch.cuda.current_device() return, without building a
+# Stream object: a call on a single row is bound by the host, about 10 us of it.
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_device_now = torch._C._cuda_getDevice
 
 
 def _bad(what: str):
     raise ValueError(what)
 
 
-def _rows(t, name: str, d: int | None = None, n: int | None = None, dtype=None, device=None):
-    """Checks a matrix of contiguous columns and returns its row stride in elements."""
+def _rows(t, name: str, d: int, n: int, dtype, device) -> int:
+    """Checks a matrix [n, d] of contiguous columns and returns its row stride in elements."""
+    if t.dtype is not dtype:
+        _bad(f"{name} is {t.dtype}, expected {dtype}")
+    if t.device != device:
+        _bad(f"{name} is on {t.device}, expected {device}")
+    if t.shape != (n, d):
+        _bad(f"{name} has shape {tuple(t.shape)}, expected {(n, d)}")
+    if t.is_contiguous():
+        return d
+    ld, sc = t.stride()
+    if d > 1 and sc != 1:
+        _bad(f"{name} must have contiguous columns")
+    if n <= 1:
+        return d
+    if ld < d:
+        _bad(f"{name} must not overlap itself (row stride {ld} below {d} columns)")
+    return ld
+
+
+def _matrix(t, name: str):
+    """(rows, columns, device) of the CUDA matrix that sets a call's shape."""
     if not t.is_cuda:
         _bad(f"{name} must be a CUDA tensor")
     if t.dim() != 2:
         _bad(f"{name} must be a matrix [rows, columns], got shape {tuple(t.shape)}")
-    rows, cols = t.shape
-    if (d is not None and cols != d) or (n is not None and rows != n):
-        _bad(f"{name} has shape {(rows, cols)}, expected {(rows if n is None else n, cols if d is None else d)}")
-    if dtype is not None and t.dtype is not dtype:
-        _bad(f"{name} is {t.dtype}, expected {dtype}")
-    if device is not None and t.device != device:
-        _bad(f"{name} is on {t.device}, expected {device}")
-    ld, sc = t.stride()
-    if cols > 1 and sc != 1:
-        _bad(f"{name} must have contiguous columns")
-    if rows <= 1 or ld == cols:
-        return cols
-    if ld < cols:
-        _bad(f"{name} must not overlap itself (row stride {ld} below {cols} columns)")
-    return ld
+    return *t.shape, t.device
+
+
+def _like(t):
+    """An uninitialised contiguous tensor of t's shape and type."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _plain(t, name: str, shape: tuple, dtype, device):
     """Checks a contiguous tensor of exactly this shape and type; None passes."""
     if t is None:
         return None
-    if tuple(t.shape) != shape or t.dtype is not dtype or t.device != device or not t.is_contiguous():
+    if t.shape != shape or t.dtype is not dtype or t.device != device or not t.is_contiguous():
         _bad(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {device}, got {t.dtype} "
              f"{tuple(t.shape)} on {t.device}")
     return t.data_ptr()
@@ -67,35 +80,30 @@ def _plain(t, name: str, shape: tuple, dtype, device):
 def _call(name: str, device, *args):
     """One native call on `device` and its current stream."""
     f = getattr(fn._lib or fn.load_library(), name)
-    stream = _raw_stream(device.index)
-    if torch.cuda.current_device() == device.index:
-        rc = f(*args, stream)
+    i = device.index
+    if _device_now() == i:
+        rc = f(*args, _raw_stream(i))
     else:
         with torch.cuda.device(device):
-            rc = f(*args, stream)
+            rc = f(*args, _raw_stream(i))
     if rc != fn.FFN_OK:
         msg = fn.load_library().ffn_last_error(None).decode()
         raise (ValueError if rc in (fn.FFN_E_CONFIG, fn.FFN_E_CAPACITY) else RuntimeError)(f"{name} failed ({rc}): {msg}")
 
 
-def _streamed(f):
-    """Gives an operator its ``stream`` argument: outputs and workspaces are then allocated on that
-    stream too, so the caching allocator cannot hand their memory to other work early."""
-    @functools.wraps(f)
-    def g(*args, stream=None, **kw):
-        if stream is None:
-            return f(*args, **kw)
-        if not isinstance(stream, torch.cuda.Stream):
-            stream = torch.cuda.ExternalStream(int(stream))
-        with torch.cuda.stream(stream):
-            return f(*args, **kw)
-    return g
+def _on(stream, f, *args):
+    """f(*args) with `stream` current: outputs and workspaces are then allocated on that stream too, so
+    the caching allocator cannot hand their memory to other work early."""
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(int(stream))
+    with torch.cuda.stream(stream):
+        return f(*args)
 
 
 def _workspace(device, name: str, *args):
     """(tensor or None, pointer, bytes) of the workspace that the library asks for."""
     f = getattr(fn._lib or fn.load_library(), name)
-    if torch.cuda.current_device() == device.index:
+    if _device_now() == device.index:
         need = f(*args)
     else:
         with torch.cuda.device(device):
@@ -114,8 +122,7 @@ class NormState(NamedTuple):
     residual: torch.Tensor | None
 
 
-@_streamed
-def rmsnorm(x, gamma, residual=None, eps: float = 1e-6, out: str = "same", group: int = 0):
+def rmsnorm(x, gamma, residual=None, eps: float = 1e-6, out: str = "same", group: int = 0, stream=None):
     """RMS norm of ``x + residual`` over the columns: returns ``(y, h, state, scale)``.
 
     x, residual [n, d] (float32, float16 or bfloat16; rows may be strided), gamma [d] float32.  y is in
@@ -123,34 +130,40 @@ def rmsnorm(x, gamma, residual=None, eps: float = 1e-6, out: str = "same", group
     ``group`` 32, 64 or 128; value = y * scale (scale is None for ``out="same"``).  h is the sum in x's
     type, the residual stream that goes on (x itself without a residual); state is what
     ``rmsnorm_bwd`` takes."""
-    if x.dtype not in _WIDE:
-        _bad(f"x must be float32, float16 or bfloat16, got {x.dtype}")
-    x_ld = _rows(x, "x")
-    n, d = x.shape
-    dev, dt = x.device, x.dtype
-    res_ld = 0 if residual is None else _rows(residual, "residual", d, n, dt, dev)
+    if stream is not None:
+        return _on(stream, rmsnorm, x, gamma, residual, eps, out, group)
+    dt = x.dtype
+    if dt not in _WIDE:
+        _bad(f"x must be float32, float16 or bfloat16, got {dt}")
+    n, d, dev = _matrix(x, "x")
+    x_ld = _rows(x, "x", d, n, dt, dev)
+    code = DTYPES[dt]
     g = _plain(gamma, "gamma", (d,), torch.float32, dev)
     if out == "same":
         if group:
             _bad("group needs out='e4m3'")
-        y, scale, code = torch.empty((n, d), dtype=dt, device=dev), None, DTYPES[dt]
+        y, scale, sp, out_code = _like(x), None, None, code
     elif out == "e4m3":
         if group not in (0, 32, 64, 128) or (group and d % group):
             _bad(f"group must be 0, 32, 64 or 128 and divide the {d} columns, got {group}")
-        y, code = torch.empty((n, d), dtype=torch.float8_e4m3fn, device=dev), E4M3
-        scale = torch.empty((n, d // group) if group else (n,), dtype=torch.float32, device=dev)
+        y, out_code = torch.empty((n, d), dtype=torch.float8_e4m3fn, device=dev), E4M3
+        scale = gamma.new_empty((n, d // group) if group else (n,))
+        sp = scale.data_ptr()
     else:
         _bad(f"out must be 'same' or 'e4m3', got {out!r}")
-    h = x if residual is None else torch.empty((n, d), dtype=dt, device=dev)
-    rstd = torch.empty(n, dtype=torch.float32, device=dev)
-    _call("ffn_rmsnorm", dev, x.data_ptr(), x_ld, None if residual is None else residual.data_ptr(), res_ld, g,
-          None if residual is None else h.data_ptr(), y.data_ptr(), None if scale is None else scale.data_ptr(),
-          rstd.data_ptr(), n, d, eps, DTYPES[dt], code, group)
+    rstd = gamma.new_empty((n,))
+    if residual is None:
+        h, hp, rp, res_ld = x, None, None, 0
+    else:
+        res_ld = _rows(residual, "residual", d, n, dt, dev)
+        h = _like(x)
+        hp, rp = h.data_ptr(), residual.data_ptr()
+    _call("ffn_rmsnorm", dev, x.data_ptr(), x_ld, rp, res_ld, g, hp, y.data_ptr(), sp, rstd.data_ptr(), n, d, eps, code,
+          out_code, group)
     return y, h, NormState(rstd, x, residual), scale
 
 
-@_streamed
-def rmsnorm_bwd(dy, h, gamma, state, dresidual=None):
+def rmsnorm_bwd(dy, h, gamma, state, dresidual=None, stream=None):
     """Backward pass of ``rmsnorm``: returns ``(dx, dgamma)``.  dx (the gradient of x and of the residual
     alike) includes ``dresidual``, the gradient that reaches h past the norm.
 
@@ -158,18 +171,19 @@ def rmsnorm_bwd(dy, h, gamma, state, dresidual=None):
     and h is not read.  A caller who kept only h and the row factors passes the float32 [n] tensor
     ``state.rstd`` instead: xhat then carries the rounding of h, one array less is read, and x and the
     residual need not be kept."""
-    if dy.dtype not in _WIDE:
-        _bad(f"dy must be float32, float16 or bfloat16, got {dy.dtype}")
-    dy_ld = _rows(dy, "dy")
-    n, d = dy.shape
-    dev, dt = dy.device, dy.dtype
+    if stream is not None:
+        return _on(stream, rmsnorm_bwd, dy, h, gamma, state, dresidual)
+    dt = dy.dtype
+    if dt not in _WIDE:
+        _bad(f"dy must be float32, float16 or bfloat16, got {dt}")
+    n, d, dev = _matrix(dy, "dy")
+    dy_ld = _rows(dy, "dy", d, n, dt, dev)
     rstd, x, residual = state if isinstance(state, NormState) else (state, h, None)
     x_ld = _rows(x, "x", d, n, dt, dev)
     res_ld = 0 if residual is None else _rows(residual, "residual", d, n, dt, dev)
     dr_ld = 0 if dresidual is None else _rows(dresidual, "dresidual", d, n, dt, dev)
     g, r = _plain(gamma, "gamma", (d,), torch.float32, dev), _plain(rstd, "rstd", (n,), torch.float32, dev)
-    dx = torch.empty((n, d), dtype=dt, device=dev)
-    dgamma = torch.empty(d, dtype=torch.float32, device=dev)
+    dx, dgamma = _like(dy), _like(gamma)
     ws, p, size = _workspace(dev, "ffn_rmsnorm_bwd_workspace", n, d)
     _call("ffn_rmsnorm_bwd", dev, dy.data_ptr(), dy_ld, x.data_ptr(), x_ld,
           None if residual is None else residual.data_ptr(), res_ld, g, r,
@@ -207,22 +221,20 @@ def _packed(t, name: str, like, d: int):
     """(pointer, row stride) of a [rows, d] or [sequences, steps, d] tensor."""
     if t.shape != like.shape:
         _bad(f"{name} has shape {tuple(t.shape)}, expected {tuple(like.shape)}")
+    if t.dtype is not like.dtype or t.device != like.device or not t.is_cuda:
+        _bad(f"{name} must be a {like.dtype} CUDA tensor on {like.device}, got {t.dtype} on {t.device}")
+    if t.is_contiguous():
+        return t.data_ptr(), d
     if t.dim() == 3:
         b, s, _ = t.shape
-        if t.is_contiguous():
-            if t.dtype is not like.dtype or t.device != like.device or not t.is_cuda:
-                _bad(f"{name} must be a {like.dtype} CUDA tensor on {like.device}")
-            return t.data_ptr(), d
         if s > 1 and b > 1 and t.stride(0) != s * t.stride(1):
             _bad(f"{name}: the sequences must follow one another at a constant row stride")
-        row = t.stride(1) if s > 1 else t.stride(0)
-        t = t.as_strided((b * s, d), (row, t.stride(2)))
-    return t.data_ptr(), _rows(t, name, d, None, like.dtype, like.device)
+        t = t.as_strided((b * s, d), (t.stride(1) if s > 1 else t.stride(0), t.stride(2)))
+    return t.data_ptr(), _rows(t, name, d, t.shape[0], like.dtype, like.device)
 
 
-@_streamed
 def gated_scan(gate, value, h0=None, offsets=None, max_len: int | None = None, form: str = "sigmoid",
-               reverse: bool = False):
+               reverse: bool = False, stream=None):
     """The recurrence ``h_t = a_t h_{t-1} + b_t`` per channel: returns ``(h, h_last)``.
 
     form "sigmoid": a = sigmoid(gate), b = (1 - a) value; "linear": a = gate (magnitude at most about
@@ -232,11 +244,13 @@ def gated_scan(gate, value, h0=None, offsets=None, max_len: int | None = None, f
     get (it chooses the split of the work and bounds nothing).  h0 [sequences, channels] float32 is the
     state before the first step (None: zero); h_last, float32, the state after the last.  ``reverse``
     runs every sequence from its last step to its first (back-to-front compositing)."""
+    if stream is not None:
+        return _on(stream, gated_scan, gate, value, h0, offsets, max_len, form, reverse)
     seqs, max_len, d, off, p0 = _scan_layout(gate, value, offsets, max_len, form, h0)
     gp, g_ld = _packed(gate, "gate", gate, d)
     vp, v_ld = _packed(value, "value", gate, d)
-    h = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
-    last = torch.empty((seqs, d), dtype=torch.float32, device=gate.device)
+    h = _like(gate)
+    last = torch.empty((seqs, d), dtype=torch.float32, device=gate.device) if h0 is None else torch.empty_like(h0)
     rows = seqs * max_len if off is None else gate.shape[0]
     if seqs == 0:
         return h.zero_(), last
@@ -245,11 +259,12 @@ def gated_scan(gate, value, h0=None, offsets=None, max_len: int | None = None, f
     return h, last
 
 
-@_streamed
 def gated_scan_bwd(dh, gate, value, h, h0=None, dh_last=None, offsets=None, max_len: int | None = None,
-                   form: str = "sigmoid", reverse: bool = False):
+                   form: str = "sigmoid", reverse: bool = False, stream=None):
     """Backward pass of ``gated_scan`` from its inputs and its h: returns ``(dgate, dvalue, dh0)``.
     dh_last [sequences, channels] float32 is the gradient of h_last (None: zero); dh0 is float32."""
+    if stream is not None:
+        return _on(stream, gated_scan_bwd, dh, gate, value, h, h0, dh_last, offsets, max_len, form, reverse)
     seqs, max_len, d, off, p0 = _scan_layout(gate, value, offsets, max_len, form, h0)
     dev = gate.device
     gp, g_ld = _packed(gate, "gate", gate, d)
@@ -257,8 +272,7 @@ def gated_scan_bwd(dh, gate, value, h, h0=None, dh_last=None, offsets=None, max_
     dp, d_ld = _packed(dh, "dh", gate, d)
     hp, h_ld = _packed(h, "h", gate, d)
     pl = _plain(dh_last, "dh_last", (seqs, d), torch.float32, dev)
-    dgate = torch.empty(gate.shape, dtype=gate.dtype, device=dev)
-    dvalue = torch.empty(gate.shape, dtype=gate.dtype, device=dev)
+    dgate, dvalue = _like(gate), _like(gate)
     dh0 = torch.empty((seqs, d), dtype=torch.float32, device=dev)
     rows = seqs * max_len if off is None else gate.shape[0]
     if seqs == 0:
@@ -282,8 +296,7 @@ def _experts(x, w, offsets):
     return e, m, k, _plain(offsets, "offsets", (e + 1,), torch.int32, dev)
 
 
-@_streamed
-def expert_mm(x, w, offsets, x_scale=None, w_scale=None, out_dtype=None):
+def expert_mm(x, w, offsets, x_scale=None, w_scale=None, out_dtype=None, stream=None):
     """``y[r] = x[r] w[e]^T`` for the rows r of expert e: returns y [n, out].
 
     x [n, in] holds the rows sorted by expert (rows may be strided), offsets [experts + 1] int32 on the
@@ -291,11 +304,11 @@ def expert_mm(x, w, offsets, x_scale=None, w_scale=None, out_dtype=None):
     offsets[experts] on give zeros), w [experts, out, in].  x and w are both float16 or both bfloat16
     (y the same), or both float8_e4m3fn with float32 ``x_scale`` [n] and ``w_scale`` [experts, out]
     (y bfloat16, or float16 by ``out_dtype``).  Sums are float32."""
-    x_ld = _rows(x, "x")
+    if stream is not None:
+        return _on(stream, expert_mm, x, w, offsets, x_scale, w_scale, out_dtype)
+    n, _, dev = _matrix(x, "x")
     e, m, k, off = _experts(x, w, offsets)
-    n, dev = x.shape[0], x.device
-    if x.shape[1] != k:
-        _bad(f"x has {x.shape[1]} columns, w takes {k}")
+    x_ld = _rows(x, "x", k, n, x.dtype, dev)
     xs = ws_ = None
     if x.dtype is torch.float8_e4m3fn:
         out_dtype = out_dtype or torch.bfloat16
@@ -315,24 +328,27 @@ def expert_mm(x, w, offsets, x_scale=None, w_scale=None, out_dtype=None):
         _bad(f"x must be float16, bfloat16 or float8_e4m3fn, got {x.dtype}")
     y = torch.empty((n, m), dtype=out_dtype, device=dev)
     code = DTYPES[x.dtype]
-    buf, p, size = _workspace(dev, "ffn_expert_mm_workspace", x.data_ptr(), x_ld, w.data_ptr(), n, e, k, m, code)
-    _call("ffn_expert_mm", dev, x.data_ptr(), x_ld, w.data_ptr(), off, xs, ws_, y.data_ptr(), n, e, k, m, code,
+    xp, wp, unit = x.data_ptr(), w.data_ptr(), 16 if code == E4M3 else 8
+    buf = p = None
+    size = 0
+    if (xp | wp) & 15 or x_ld % unit or k % unit:             # rows that TMA cannot read are copied
+        buf, p, size = _workspace(dev, "ffn_expert_mm_workspace", xp, x_ld, wp, n, e, k, m, code)
+    _call("ffn_expert_mm", dev, xp, x_ld, wp, off, xs, ws_, y.data_ptr(), n, e, k, m, code,
           DTYPES[out_dtype], p, size)
     return y
 
 
-@_streamed
-def expert_mm_bwd(dy, x, w, offsets, need_dx: bool = True, need_dw: bool = True, dw_dtype=None):
+def expert_mm_bwd(dy, x, w, offsets, need_dx: bool = True, need_dw: bool = True, dw_dtype=None, stream=None):
     """Gradients of ``expert_mm`` for float16 or bfloat16 operands: returns ``(dx, dw)``, each None when
     not needed.  dx [n, in] is in x's type; dw [experts, out, in] in x's type or, by ``dw_dtype``,
     float32 (what ``ffn_native.adam`` takes).  An expert without rows gets a zero gradient."""
+    if stream is not None:
+        return _on(stream, expert_mm_bwd, dy, x, w, offsets, need_dx, need_dw, dw_dtype)
     if x.dtype not in (torch.float16, torch.bfloat16):
         _bad(f"x must be float16 or bfloat16, got {x.dtype}")
-    x_ld = _rows(x, "x")
+    n, _, dev = _matrix(x, "x")
     e, m, k, off = _experts(x, w, offsets)
-    n, dev = x.shape[0], x.device
-    if x.shape[1] != k:
-        _bad(f"x has {x.shape[1]} columns, w takes {k}")
+    x_ld = _rows(x, "x", k, n, x.dtype, dev)
     dy_ld = _rows(dy, "dy", m, n, x.dtype, dev)
     dw_dtype = dw_dtype or x.dtype
     if dw_dtype not in (x.dtype, torch.float32):
