@@ -22,7 +22,7 @@ UNITS = {
     "ffn_capi.cu": ("ffn_step.cu", "ffn_common.cuh", "ffn_raymarch.cuh", "ffn_hashgrid.cuh", "ffn_tcgen05.cuh",
                     "ffn_step_tc.cu", "ffn_noalloc.cu", "ffn_dp.cu", "ffn_batch.cu", "ffn_probe.cu", "ffn_ops.cuh"),
     "ffn_norm.cu": ("ffn_ops.cuh",),
-    "ffn_scan.cu": ("ffn_ops.cuh", "ffn_tcgen05.cuh"),
+    "ffn_scan.cu": ("ffn_ops.cuh",),
     "ffn_experts.cu": ("ffn_ops.cuh", "ffn_tcgen05.cuh"),
 }
 SOURCES = [CSRC / n for n in sorted({f for u, inc in UNITS.items() for f in (u, *inc)})] + [HEADER]

@@ -860,9 +860,7 @@ int ffn_ops_status(uint32_t* status) {
     if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&v, g_status, sizeof v);
     const int zero = 0;
     if (e == cudaSuccess && v) e = cudaMemcpyToSymbol(g_status, &zero, sizeof zero);
-    int scan = 0;
-    if (e == cudaSuccess) e = scan_status(&scan);
-    *status = (uint32_t)(v | scan);
+    *status = (uint32_t)v;
     return e == cudaSuccess ? FFN_OK : op_fail(FFN_E_CUDA, std::string("ffn_ops_status: ") + cudaGetErrorString(e));
 }
 

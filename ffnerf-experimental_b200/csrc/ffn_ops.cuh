@@ -17,9 +17,6 @@ namespace ffn {
 // Records the message that ffn_last_error(NULL) returns and gives the code back (ffn_capi.cu).
 int op_fail(int code, const std::string& msg);
 
-// Reads and clears the recurrence's share of the status word (ffn_scan.cu).
-cudaError_t scan_status(int* v);
-
 inline int op_launched(const char* what) {
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? FFN_OK : op_fail(FFN_E_CUDA, std::string(what) + ": " + cudaGetErrorString(e));

@@ -20,20 +20,18 @@
 // loads are all issued before the first is used.  Threads are numbered over (sequence, channels) so
 // that narrow rows fill warps too.  Every element is read and written once: HBM is the bound, and what
 // the kernel needs is enough loads in flight.  Where sequences x channels give too few threads for
-// that, time is split: a block of W warps takes W parts of U steps each, the blocks of a cluster take
-// W parts each, every thread first composes the map of its own part, the maps are exchanged through
-// shared memory (within the block) and distributed shared memory (within the cluster), and each thread
-// then enters its part with the state that the maps before it give.  The elements stay in registers in
-// between, so the split costs no second read; no global memory and no waiting on flags is involved.
-#include <atomic>
+// that, each sequence's time is cut into parts and there are two launches: the first composes the map of
+// every part, walking it from its end to its beginning, the second goes through each part from the state
+// that the maps before it give.  That reads the gates and inputs a second time, in part from L2 (the
+// first launch ends where the second begins); in return every thread streams its own part and waits for
+// nobody.  A one-read form was built and measured: blocks of a cluster that take turns along time and
+// exchange maps through distributed shared memory (with a cluster barrier, then with st.async and
+// mbarriers).  A turn's chain -- map, exchange, composition -- took 3 us of which memory was a quarter:
+// 433 us forward and backward at 2 sequences x 32768 steps x 1024 channels in bf16.
 #include <initializer_list>
 #include <type_traits>
-#include <cooperative_groups.h>
 
 #include "ffn_ops.cuh"
-#include "ffn_tcgen05.cuh"
-
-namespace cg = cooperative_groups;
 
 namespace ffn {
 namespace {
@@ -49,6 +47,8 @@ struct ScanArgs {
     int64_t items;                            // sequences x channel groups
     int seqs, d, groups;                      // groups = d / C
     int reverse;
+    int parts;                                // of each sequence's time (1: no maps)
+    float* maps;                              // [parts - 1][2][seqs * d]: p and h of each part but the last
 };
 
 struct Affine { float p, h; };
@@ -100,11 +100,6 @@ template <typename T, int C>
 struct Word {
     typename Raw<sizeof(T) * C>::type r;
     __device__ __forceinline__ void load(const T* p) { r = __ldg(reinterpret_cast<const decltype(r)*>(p)); }
-    // Copies a word to shared memory without waiting (4 bytes or more).
-    static __device__ __forceinline__ void copy(Word* to, const T* p) {
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;"
-                     :: "r"((uint32_t)__cvta_generic_to_shared(to)), "l"(p), "n"((int)sizeof(Word)) : "memory");
-    }
     __device__ __forceinline__ float at(int j) const {
         if constexpr (sizeof(T) == 4) {
             if constexpr (C == 1) return __uint_as_float(r);
@@ -128,41 +123,34 @@ template <typename T, bool SIG, bool BACK, int C, int U>
 struct Chunk {
     Word<T, C> gate[U], value[SIG || !BACK ? U : 1], dh[BACK ? U : 1], before[BACK ? U : 1];
 
-    // Calls f(stream, step, address) for each word of the chunk that lies before the sequence's end.
-    // Streams: 0 gate, 1 value, 2 dh, 3 the state before the step.
-    template <typename F>
-    static __device__ __forceinline__ void each(const ScanArgs& a, const Span& s, int64_t t0, int ch, F&& f) {
+    // MAPS: only what the map of a part needs.
+    template <bool MAPS>
+    __device__ __forceinline__ void load(const ScanArgs& a, const Span& s, int64_t t0, int left, int ch) {
         const int64_t row = s.first + t0 * s.dir;
         const T* pg = static_cast<const T*>(a.gate) + row * a.gate_ld + ch;
         const T* pv = static_cast<const T*>(a.value) + row * a.value_ld + ch;
         const T* pd = static_cast<const T*>(a.dh) + row * a.dh_ld + ch;
         const T* pb = static_cast<const T*>(a.h_in) + (row + s.dir) * a.h_ld + ch;
         const int64_t sg = a.gate_ld * s.dir, sv = a.value_ld * s.dir, sd = a.dh_ld * s.dir, sb = a.h_ld * s.dir;
-        const int left = (int)min(max(s.len - t0, (int64_t)0), (int64_t)(U + 1));
+        const bool more = t0 + left < s.len;           // the walk goes on after this chunk
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             if (i < left) {
-                f(0, i, pg);
+                gate[i].load(pg);
                 pg += sg;
-                if constexpr (SIG || !BACK) {
-                    f(1, i, pv);
+                if constexpr (!BACK || (SIG && !MAPS)) {
+                    value[i].load(pv);
                     pv += sv;
                 }
                 if constexpr (BACK) {
-                    f(2, i, pd);
+                    dh[i].load(pd);
                     pd += sd;
                     // the state before this step: the next row of this walk (the last step's is h0)
-                    if (i + 1 < left) f(3, i, pb);
+                    if (!MAPS && (i + 1 < left || more)) before[i].load(pb);
                     pb += sb;
                 }
             }
         }
-    }
-    __device__ __forceinline__ Word<T, C>& word(int stream, int i) {
-        return stream == 0 ? gate[i] : stream == 1 ? value[SIG || !BACK ? i : 0] : stream == 2 ? dh[BACK ? i : 0] : before[BACK ? i : 0];
-    }
-    __device__ __forceinline__ void load(const ScanArgs& a, const Span& s, int64_t t0, int ch) {
-        each(a, s, t0, ch, [&](int q, int i, const T* p) { word(q, i).load(p); });
     }
 };
 
@@ -252,292 +240,175 @@ __device__ __forceinline__ void put_state(const ScanArgs& a, int seq, int ch, co
     for (int j = 0; j < C; ++j) a.last[(int64_t)seq * a.d + ch + j] = state[j];
 }
 
-// Enough sequences and channels: one thread goes through a whole sequence.
+template <int C>
+__device__ __forceinline__ void load_floats(const float* p, float (&v)[C]) {
+    using R = typename Raw<4 * C>::type;
+    const R r = __ldg(reinterpret_cast<const R*>(p));
+#pragma unroll
+    for (int j = 0; j < C; ++j) v[j] = __uint_as_float(reinterpret_cast<const uint32_t*>(&r)[j]);
+}
+
+// A thread's steps: all of its sequence's, or one of `parts` equal parts of them (multiples of U).
+template <int U>
+__device__ __forceinline__ void part_of(const ScanArgs& a, const Span& s, int part, int64_t& lo, int64_t& hi) {
+    const int64_t chunks = (s.len + U - 1) / U, each = (chunks + a.parts - 1) / a.parts * U;
+    lo = min((int64_t)part * each, s.len);
+    hi = min(lo + each, s.len);
+}
+
+// Composes the map of every part but each sequence's last, from the part's last step to its first:
+// with m the map of the steps after it, a step x -> a x + b makes it x -> (p a) x + (p b + h).
+template <typename T, bool SIG, bool BACK, int C, int U>
+__global__ void __launch_bounds__(256, 2) scan_maps_kernel(const ScanArgs a) {
+    const int64_t item = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (item >= a.items) return;
+    const int part = blockIdx.y, seq = (int)(item / a.groups), ch = (int)(item % a.groups) * C;
+    const Span s = span_of<BACK>(a, seq);
+    int64_t lo, hi;
+    part_of<U>(a, s, part, lo, hi);
+    Affine m[C];
+#pragma unroll
+    for (int j = 0; j < C; ++j) m[j] = Affine{1.0f, 0.0f};
+    const int64_t chunks = (hi - lo + U - 1) / U;
+#pragma unroll 1
+    for (int64_t q = chunks - 1; q >= 0; --q) {
+        const int64_t t = lo + q * U;
+        const int left = (int)min(hi - t, (int64_t)U);
+        Chunk<T, SIG, BACK, C, U> k;
+        k.template load<true>(a, s, t, left, ch);
+#pragma unroll
+        for (int i = U - 1; i >= 0; --i)
+            if (i < left) {
+                Step<SIG, BACK, C> f;
+                f.form(k, i);
+#pragma unroll
+                for (int j = 0; j < C; ++j) {
+                    const float p = m[j].p * f.a[j], b = f.b[j];
+                    // (a zero stays out of the product where p may have overflowed, as in apply)
+                    m[j].h = !SIG && b == 0.0f ? m[j].h : fmaf(BACK ? p : m[j].p, b, m[j].h);
+                    m[j].p = p;
+                }
+            }
+    }
+    const int64_t plane = (int64_t)a.seqs * a.d;
+    float* out = a.maps + part * 2 * plane + (int64_t)seq * a.d + ch;
+    float p[C], h[C];
+#pragma unroll
+    for (int j = 0; j < C; ++j) { p[j] = m[j].p; h[j] = m[j].h; }
+    *reinterpret_cast<Pack<float, C>*>(out) = *reinterpret_cast<const Pack<float, C>*>(p);
+    *reinterpret_cast<Pack<float, C>*>(out + plane) = *reinterpret_cast<const Pack<float, C>*>(h);
+}
+
+// Goes through each thread's steps and writes the results.
 template <typename T, bool SIG, bool BACK, int C, int U>
 __global__ void __launch_bounds__(256, 2) scan_kernel(const ScanArgs a) {
     const int64_t item = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (item >= a.items) return;
-    const int seq = (int)(item / a.groups), ch = (int)(item % a.groups) * C;
+    const int part = blockIdx.y, seq = (int)(item / a.groups), ch = (int)(item % a.groups) * C;
     const Span s = span_of<BACK>(a, seq);
     float state[C];
     first_state<BACK, C>(a, seq, ch, state);
+    const int64_t plane = (int64_t)a.seqs * a.d;
+    const float* mp = a.maps + (int64_t)seq * a.d + ch;
+#pragma unroll 8
+    for (int q = 0; q < part; ++q, mp += 2 * plane) {
+        float p[C], h[C];
+        load_floats<C>(mp, p);
+        load_floats<C>(mp + plane, h);
+#pragma unroll
+        for (int j = 0; j < C; ++j) state[j] = apply(Affine{p[j], h[j]}, state[j]);
+    }
+    int64_t lo, hi;
+    part_of<U>(a, s, part, lo, hi);
 #pragma unroll 1
-    for (int64_t t = 0; t < s.len; t += U) {
+    for (int64_t t = lo; t < hi; t += U) {
+        const int left = (int)min(hi - t, (int64_t)U);
         Chunk<T, SIG, BACK, C, U> k;
-        k.load(a, s, t, ch);
+        k.template load<false>(a, s, t, left, ch);
         int64_t at = (s.first + t * s.dir) * a.d + ch;
-        const int left = (int)min(s.len - t, (int64_t)(U + 1));
 #pragma unroll
         for (int i = 0; i < U; ++i)
             if (i < left) {
                 Step<SIG, BACK, C> f;
                 f.form(k, i);
-                f.take(a, k, i, i + 1 == left, at, (int64_t)seq * a.d + ch, state);
+                f.take(a, k, i, t + i + 1 == s.len, at, (int64_t)seq * a.d + ch, state);
                 at += (int64_t)s.dir * a.d;
             }
     }
-    put_state<C>(a, seq, ch, state);
-    clear_outside<T, BACK, C>(a, seq, ch);
+    if (part == a.parts - 1) put_state<C>(a, seq, ch, state);
+    if (part == 0) clear_outside<T, BACK, C>(a, seq, ch);
 }
 
-constexpr int WARPS = 8, MOST_RANKS = 8;
+constexpr int U = 8;                 // steps whose loads a thread issues together
+constexpr int PART_STEPS = 32;       // a part is worth its second read from about here on
 
-// The maps of a lane's C channels.
-template <int C> struct alignas(8 * C) Maps { Affine m[C]; };
+// How the work is laid out: channels of a thread, parts of time.
+struct ScanPlan { int width, parts; };
 
-// The split form: steps of a warp's part, and the stages of its ring of chunks in shared memory.  Each
-// thread copies the words that it will use itself, so the ring needs no barrier; words of 2 bytes, which
-// have no asynchronous copy, are prefetched one chunk ahead in registers instead.
-template <typename T, bool SIG, bool BACK, int C>
-struct Split {
-    static constexpr int W = sizeof(T) * C;
-    static constexpr bool RING = W >= 4;
-    static constexpr int U = !RING ? 8 : (BACK ? 32 : 64) / W;
-    static constexpr int STREAMS = BACK ? 4 : 2;
-    static constexpr int STAGES = RING ? 3 : 0;
-    static constexpr size_t BYTES = (size_t)STAGES * STREAMS * U * W * 32 * WARPS;   // at most 96 KB: two blocks an SM
-};
-
-__device__ int g_scan_status;                         // ST_TC_TIMEOUT's bit when a wait ran out (ffn_ops_status)
-constexpr uint32_t WAIT_POLLS = 1u << 22;
-
-// Writes a lane's maps into block `rank`'s shared memory and counts their bytes on that block's mbarrier.
-template <int C>
-__device__ __forceinline__ void send_maps(const Maps<C>* to, uint64_t* bar, int rank, const Maps<C>& v) {
-    uint32_t ra, rb;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"((uint32_t)__cvta_generic_to_shared(to)), "r"(rank));
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(rb) : "r"((uint32_t)__cvta_generic_to_shared(bar)), "r"(rank));
-    if constexpr (C == 2)
-        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];"
-                     :: "r"(ra), "f"(v.m[0].p), "f"(v.m[0].h), "f"(v.m[1].p), "f"(v.m[1].h), "r"(rb) : "memory");
-    else
-        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];"
-                     :: "r"(ra), "f"(v.m[0].p), "f"(v.m[0].h), "r"(rb) : "memory");
-}
-
-// Few sequences and channels: 32 items per cluster, time split over the WARPS warps of its blocks, U steps
-// a warp.  The loads of the next chunks are in flight while the maps of this one go round: a block's map is
-// written straight into the shared memory of the cluster's blocks (warp q writes to block q), and each
-// block waits on its own mbarrier for the bytes of all.  A cluster barrier in its place costs more than
-// the rest of a turn: its release waits until the results that the last turn stored have reached L2.
-// Two buffers are enough: a block sends its maps of the next turn after it has read those of this one,
-// and nobody sends those of the turn after without having them.
-template <typename T, bool SIG, bool BACK, int C>
-__global__ void __launch_bounds__(32 * WARPS, 2) scan_split_kernel(const ScanArgs a) {
-    using S = Split<T, SIG, BACK, C>;
-    constexpr int U = S::U;
-    using K = Chunk<T, SIG, BACK, C, U>;
-    cg::cluster_group cluster = cg::this_cluster();
-    extern __shared__ __align__(16) unsigned char ring_bytes[];
-    [[maybe_unused]] Word<T, C>* ring = reinterpret_cast<Word<T, C>*>(ring_bytes) + threadIdx.x;   // [stage][stream][step][thread]
-    __shared__ Maps<C> part[2][WARPS][32];            // the maps of this block's parts
-    __shared__ Maps<C> whole[2][MOST_RANKS][32];      // the maps of the cluster's blocks
-    __shared__ uint64_t arrived[2];
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
-    const int64_t item = (int64_t)(blockIdx.x / ranks) * 32 + lane;
-    const bool live = item < a.items;
-    const int seq = live ? (int)(item / a.groups) : 0, ch = live ? (int)(item % a.groups) * C : 0;
-    Span s = span_of<BACK>(a, seq);
-    if (!live) s.len = 0;
-    int64_t most = s.len;                              // the same in every warp of the cluster
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = max(most, (int64_t)__shfl_xor_sync(0xffffffffu, (long long)most, o));
-    float state[C];
-    first_state<BACK, C>(a, seq, ch, state);
-    if (ranks > 1) {
-        if (threadIdx.x == 0) { tc::mbar_init(arrived, 1); tc::mbar_init(arrived + 1, 1); }
-        cluster.sync();                                // every block runs, its barriers ready, before it is written to
-    }
-    bool ok = true;                                    // no wait has run out (else the rest of them is left out)
-    const int64_t stride = (int64_t)U * WARPS * ranks;
-    int64_t t0 = (int64_t)(rank * WARPS + w) * U;
-    K next;
-    int fill = 0, drain = 0;                           // stages of the ring
-    auto fetch = [&](int64_t t) {
-        if constexpr (S::RING) {
-            K::each(a, s, t, ch, [&](int q, int i, const T* p) {
-                Word<T, C>::copy(ring + ((fill * S::STREAMS + q) * U + i) * (32 * WARPS), p);
-            });
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            fill = fill + 1 == S::STAGES ? 0 : fill + 1;
-        } else {
-            next.load(a, s, t, ch);
-        }
-    };
-    fetch(t0);
-    if constexpr (S::RING) fetch(t0 + stride);
-    int buf = 0;
-    uint32_t phase = 0;
-    for (int64_t base = 0; base < most; base += stride, t0 += stride, phase ^= buf, buf ^= 1) {
-        K k;
-        if constexpr (S::RING) {
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-            fetch(t0 + 2 * stride);                    // into the stage that the last turn has read
-#pragma unroll
-            for (int i = 0; i < U; ++i)
-#pragma unroll
-                for (int q = 0; q < S::STREAMS; ++q)
-                    if (q != 1 || SIG || !BACK) k.word(q, i) = ring[((drain * S::STREAMS + q) * U + i) * (32 * WARPS)];
-            drain = drain + 1 == S::STAGES ? 0 : drain + 1;
-        } else {
-            k = next;
-        }
-        Step<SIG, BACK, C> f[BACK ? 1 : U];            // forward: kept for the second walk over the steps
-        const int left = (int)min(max(s.len - t0, (int64_t)0), (int64_t)(U + 1));
-        Maps<C> mine;
-#pragma unroll
-        for (int j = 0; j < C; ++j) mine.m[j] = Affine{1.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            Step<SIG, BACK, C>& g = f[BACK ? 0 : i];
-            g.form(k, i);
-            if (i < left)                              // steps beyond the end leave the state alone
-#pragma unroll
-                for (int j = 0; j < C; ++j) {
-                    Affine& m = mine.m[j];
-                    m.p *= g.a[j];
-                    m.h = BACK ? g.a[j] * (m.h + g.b[j]) : fmaf(g.a[j], m.h, g.b[j]);
-                }
-        }
-        part[buf][w][lane] = mine;
-        __syncthreads();
-        // the map of the parts of this block before this warp's, and of all of them
-        Maps<C> before, all;
-#pragma unroll
-        for (int j = 0; j < C; ++j) all.m[j] = before.m[j] = Affine{1.0f, 0.0f};
-#pragma unroll
-        for (int q = 0; q < WARPS; ++q) {
-            const Maps<C> n = part[buf][q][lane];
-#pragma unroll
-            for (int j = 0; j < C; ++j) {
-                if (q == w) before.m[j] = all.m[j];
-                all.m[j].h = apply(n.m[j], all.m[j].h);
-                all.m[j].p *= n.m[j].p;
-            }
-        }
-        float enter[C];
-        if (ranks > 1) {
-            if (threadIdx.x == 0)
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
-                             :: "r"(tc::smem_u32(arrived + buf)), "r"(ranks * 32 * (int)sizeof(Maps<C>)) : "memory");
-            if (w < ranks) send_maps<C>(&whole[buf][rank][lane], arrived + buf, w, all);
-            if constexpr (!S::RING) if (base + stride < most) fetch(t0 + stride);
-            if (ok && !tc::mbar_wait(arrived + buf, phase, WAIT_POLLS)) {
-                ok = false;
-                atomicOr(&g_scan_status, 4);
-            }
-#pragma unroll
-            for (int j = 0; j < C; ++j) enter[j] = state[j];
-#pragma unroll
-            for (int q = 0; q < MOST_RANKS; ++q)
-                if (q < ranks) {
-                    const Maps<C> n = whole[buf][q][lane];
-#pragma unroll
-                    for (int j = 0; j < C; ++j) {
-                        if (q == rank) enter[j] = state[j];
-                        state[j] = apply(n.m[j], state[j]);
-                    }
-                }
-        } else {
-            if constexpr (!S::RING) if (base + stride < most) fetch(t0 + stride);
-#pragma unroll
-            for (int j = 0; j < C; ++j) {
-                enter[j] = state[j];
-                state[j] = apply(all.m[j], state[j]);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < C; ++j) enter[j] = apply(before.m[j], enter[j]);
-        int64_t at = (s.first + t0 * s.dir) * a.d + ch;
-#pragma unroll
-        for (int i = 0; i < U; ++i)
-            if (i < left) {
-                if constexpr (BACK) f[0].form(k, i);   // formed again: registers are short here
-                f[BACK ? 0 : i].take(a, k, i, i + 1 == left, at, (int64_t)seq * a.d + ch, enter);
-                at += (int64_t)s.dir * a.d;
-            }
-    }
-    if constexpr (S::RING) asm volatile("cp.async.wait_group 0;" ::: "memory");
-    if (live && rank == 0 && w == 0) {
-        put_state<C>(a, seq, ch, state);
-        clear_outside<T, BACK, C>(a, seq, ch);
-    }
-    if (ranks > 1) cluster.sync();                     // no block leaves while another writes to it
+// About 16 warps an SM keep enough loads in flight (2^20 x 64 in fp16, forward and backward: 0.87 of the
+// measured copy rate).  With 8-byte accesses they are reached later but cost fewer instructions, so the
+// widest access that leaves that many is taken; below two thirds of them time is cut into parts.
+ScanPlan scan_plan(int64_t seqs, int d, int most_width, int64_t longest, int sms) {
+    const int64_t want = (int64_t)sms * 16;
+    auto warps = [&](int c) { return (seqs * (d / c) + 31) / 32; };
+    for (int c = most_width; c >= 1; c /= 2)
+        if (warps(c) >= want) return {c, 1};
+    int width = most_width < 2 ? most_width : 2;
+    if (warps(width) * 3 > want * 2 || longest < 4 * PART_STEPS) return {width, 1};
+    width = most_width;
+    int64_t parts = want / warps(width);
+    if (parts > longest / PART_STEPS) parts = longest / PART_STEPS;
+    return {width, (int)(parts < 65535 ? parts : 65535)};
 }
 
 template <typename T, bool SIG, bool BACK, int C>
-int scan_launch(ScanArgs a, int64_t longest, int sms, cudaStream_t st) {
-    constexpr int U = 8;
+int scan_launch(ScanArgs a, int parts, cudaStream_t st) {
     a.groups = a.d / C;
     a.items = (int64_t)a.seqs * a.groups;
-    const int64_t warps = (a.items + 31) / 32;
-    // parts of time that are wanted for about 16 warps an SM, and that the length has
-    constexpr int US = Split<T, SIG, BACK, C < 4 ? C : 2>::U;
-    const int64_t parts = (longest + US - 1) / US;
-    int64_t want = ((int64_t)sms * 16 + warps - 1) / warps;
-    want = want < parts ? want : parts;
-    if (want <= 1) {
-        const int64_t blocks = (a.items + 255) / 256;
-        if (blocks > 0x7fffffff) return op_fail(FFN_E_CAPACITY, "ffn_gated_scan: too many sequences x channels");
-        scan_kernel<T, SIG, BACK, C, U><<<(unsigned)blocks, 256, 0, st>>>(a);
-        return op_launched("ffn_gated_scan");
+    a.parts = parts;
+    const int threads = parts > 1 && a.items < 256 ? (int)((a.items + 31) / 32 * 32) : 256;
+    const int64_t blocks = (a.items + threads - 1) / threads;
+    if (blocks > 0x7fffffff) return op_fail(FFN_E_CAPACITY, "ffn_gated_scan: too many sequences x channels");
+    if (parts > 1) {
+        scan_maps_kernel<T, SIG, BACK, C, U><<<dim3((unsigned)blocks, parts - 1), threads, 0, st>>>(a);
+        if (int rc = op_launched("ffn_gated_scan maps")) return rc;
     }
-    if constexpr (C <= 2) {
-        using S = Split<T, SIG, BACK, C>;
-        auto kernel = scan_split_kernel<T, SIG, BACK, C>;
-        static std::atomic<uint64_t> ready{0};        // devices whose limit is set
-        int dev = 0;
-        cudaGetDevice(&dev);
-        cudaError_t e = cudaSuccess;
-        if (S::BYTES > 40960 && (dev > 63 || !(ready.load(std::memory_order_acquire) >> dev & 1))) {
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::BYTES);
-            if (e == cudaSuccess && dev <= 63) ready.fetch_or(1ull << dev, std::memory_order_release);
-        }
-        int ranks = 1;
-        while (ranks < MOST_RANKS && (int64_t)WARPS * ranks < want) ranks *= 2;
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3((unsigned)(warps * ranks));
-        cfg.blockDim = dim3(32 * WARPS);
-        cfg.dynamicSmemBytes = S::BYTES;
-        cfg.stream = st;
-        cudaLaunchAttribute at{};
-        at.id = cudaLaunchAttributeClusterDimension;
-        at.val.clusterDim.x = (unsigned)ranks;
-        at.val.clusterDim.y = at.val.clusterDim.z = 1;
-        cfg.attrs = &at;
-        cfg.numAttrs = 1;
-        if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, a);
-        return e == cudaSuccess ? FFN_OK : op_fail(FFN_E_CUDA, std::string("ffn_gated_scan: ") + cudaGetErrorString(e));
-    }
-    return op_fail(FFN_E_CONFIG, "ffn_gated_scan: no split form for this width");   // scan_width gives C = 4 enough threads
+    scan_kernel<T, SIG, BACK, C, U><<<dim3((unsigned)blocks, parts), threads, 0, st>>>(a);
+    return op_launched("ffn_gated_scan");
 }
 
-// Channels of a thread: as many as an 8-byte access holds, where the rows allow it and enough threads are left.
-template <typename T, bool BACK>
-int scan_width(const ScanArgs& a, int form, int width, int64_t longest, cudaStream_t st) {
-    const int sms = op_sms();
-    if (sms <= 0) return op_fail(FFN_E_CUDA, "no CUDA device");
-    const bool sig = form == FFN_SCAN_SIGMOID;
-    if constexpr (sizeof(T) == 2) {
-        if (width == 4 && (int64_t)a.seqs * (a.d / 4) >= (int64_t)sms * 16 * 32)
-            return sig ? scan_launch<T, true, BACK, 4>(a, longest, sms, st) : scan_launch<T, false, BACK, 4>(a, longest, sms, st);
-    }
-    if (width >= 2) return sig ? scan_launch<T, true, BACK, 2>(a, longest, sms, st) : scan_launch<T, false, BACK, 2>(a, longest, sms, st);
-    return sig ? scan_launch<T, true, BACK, 1>(a, longest, sms, st) : scan_launch<T, false, BACK, 1>(a, longest, sms, st);
+template <typename T, bool BACK, int C>
+int scan_form(const ScanArgs& a, int form, int parts, cudaStream_t st) {
+    return form == FFN_SCAN_SIGMOID ? scan_launch<T, true, BACK, C>(a, parts, st) : scan_launch<T, false, BACK, C>(a, parts, st);
 }
+
+template <typename T, bool BACK>
+int scan_width(const ScanArgs& a, int form, ScanPlan plan, cudaStream_t st) {
+    if constexpr (sizeof(T) == 2)
+        if (plan.width == 4) return scan_form<T, BACK, 4>(a, form, plan.parts, st);
+    return plan.width >= 2 ? scan_form<T, BACK, 2>(a, form, plan.parts, st) : scan_form<T, BACK, 1>(a, form, plan.parts, st);
+}
+
+// Bytes of a plan's maps.
+uint64_t scan_bytes(ScanPlan p, int64_t seqs, int d) { return (uint64_t)(p.parts - 1) * 2 * seqs * d * sizeof(float); }
 
 template <bool BACK>
-int scan_dispatch(const ScanArgs& a, int dtype, int form, int width, int64_t longest, cudaStream_t st) {
-    if (dtype == FFN_F32) return scan_width<float, BACK>(a, form, width, longest, st);
-    if (dtype == FFN_F16) return scan_width<__half, BACK>(a, form, width, longest, st);
-    return scan_width<__nv_bfloat16, BACK>(a, form, width, longest, st);
+int scan_dispatch(ScanArgs a, int dtype, int form, int width, int64_t longest, void* ws, uint64_t ws_bytes, cudaStream_t st) {
+    const int sms = op_sms();
+    if (sms <= 0) return op_fail(FFN_E_CUDA, "no CUDA device");
+    const ScanPlan plan = scan_plan(a.seqs, a.d, width, longest, sms);
+    if (ws_bytes < scan_bytes(plan, a.seqs, a.d) || !op_aligned(ws, 16))
+        return op_fail(FFN_E_CAPACITY, "ffn_gated_scan: the workspace is smaller than ffn_gated_scan_workspace says, or not 16-byte aligned");
+    a.maps = static_cast<float*>(ws);
+    if (dtype == FFN_F32) return scan_width<float, BACK>(a, form, plan, st);
+    if (dtype == FFN_F16) return scan_width<__half, BACK>(a, form, plan, st);
+    return scan_width<__nv_bfloat16, BACK>(a, form, plan, st);
 }
 
-// The widest group of channels that every row of these matrices holds aligned: 4, 2 or 1.
+// The widest group of channels, at most 8 bytes, that every row of these matrices holds aligned: 4, 2 or 1.
 int scan_channels(int d, int dtype, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> lds) {
     const size_t z = dtype == FFN_F32 ? 4 : 2;
-    for (int c = 4; c > 1; c /= 2) {
+    for (int c = dtype == FFN_F32 ? 2 : 4; c > 1; c /= 2) {
         bool ok = d % c == 0;
         for (const void* p : ptrs) ok = ok && op_aligned(p, c * z);
         for (int64_t ld : lds) ok = ok && ld % c == 0;
@@ -559,23 +430,28 @@ int scan_check(const char* who, int64_t n_rows, int32_t n_seq, int64_t max_len, 
 
 }  // namespace
 
-// The scan's share of the status word (ffn_ops_status): reads and clears it.
-cudaError_t scan_status(int* v) {
-    cudaError_t e = cudaMemcpyFromSymbol(v, g_scan_status, sizeof *v);
-    const int zero = 0;
-    if (e == cudaSuccess && *v) e = cudaMemcpyToSymbol(g_scan_status, &zero, sizeof zero);
-    return e;
-}
-
 }  // namespace ffn
 
 using namespace ffn;
 
 extern "C" {
 
+uint64_t ffn_gated_scan_workspace(int32_t n_seq, int64_t max_len, int32_t d) {
+    const int sms = op_sms();
+    if (sms <= 0 || n_seq < 1 || d < 1 || max_len < 0) return 0;
+    uint64_t most = 0;                                // over the widths that alignment may leave
+    for (int c = 1; c <= 4; c *= 2)
+        if (d % c == 0) {
+            const uint64_t b = scan_bytes(scan_plan(n_seq, d, c, max_len, sms), n_seq, d);
+            most = b > most ? b : most;
+        }
+    return most;
+}
+
 int ffn_gated_scan(const void* gate, int64_t gate_ld, const void* value, int64_t value_ld, const float* h0,
                    const int32_t* offsets, void* h, float* h_last, int64_t n_rows, int32_t n_seq, int64_t max_len,
-                   int32_t d, int dtype, int form, int reverse, void* stream) {
+                   int32_t d, int dtype, int form, int reverse, void* workspace, uint64_t workspace_bytes,
+                   void* stream) {
     if (int rc = scan_check("ffn_gated_scan", n_rows, n_seq, max_len, d, dtype, form, offsets)) return rc;
     if (n_seq == 0) return FFN_OK;
     if (n_rows > 0 && (!gate || !value || !h)) return op_fail(FFN_E_CONFIG, "ffn_gated_scan: a required pointer is NULL");
@@ -585,13 +461,14 @@ int ffn_gated_scan(const void* gate, int64_t gate_ld, const void* value, int64_t
     a.gate = gate; a.value = value; a.h0 = h0; a.h = h; a.last = h_last; a.offsets = offsets;
     a.gate_ld = gate_ld; a.value_ld = value_ld; a.rows = n_rows; a.len = max_len; a.seqs = n_seq; a.d = d;
     a.reverse = reverse;
-    return scan_dispatch<false>(a, dtype, form, width, max_len, static_cast<cudaStream_t>(stream));
+    return scan_dispatch<false>(a, dtype, form, width, max_len, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 int ffn_gated_scan_bwd(const void* dh, int64_t dh_ld, const float* dh_last, const void* gate, int64_t gate_ld,
                        const void* value, int64_t value_ld, const void* h, int64_t h_ld, const float* h0,
                        const int32_t* offsets, void* dgate, void* dvalue, float* dh0, int64_t n_rows, int32_t n_seq,
-                       int64_t max_len, int32_t d, int dtype, int form, int reverse, void* stream) {
+                       int64_t max_len, int32_t d, int dtype, int form, int reverse, void* workspace,
+                       uint64_t workspace_bytes, void* stream) {
     if (int rc = scan_check("ffn_gated_scan_bwd", n_rows, n_seq, max_len, d, dtype, form, offsets)) return rc;
     if (n_seq == 0) return FFN_OK;
     if (n_rows > 0 && (!dh || !gate || (!value && form == FFN_SCAN_SIGMOID) || !h || !dgate || !dvalue))
@@ -604,7 +481,7 @@ int ffn_gated_scan_bwd(const void* dh, int64_t dh_ld, const float* dh_last, cons
     a.gate = gate; a.value = value; a.dh = dh; a.h_in = h; a.h0 = h0; a.dlast = dh_last; a.dgate = dgate; a.dvalue = dvalue;
     a.last = dh0; a.offsets = offsets; a.gate_ld = gate_ld; a.value_ld = value_ld; a.dh_ld = dh_ld; a.h_ld = h_ld;
     a.rows = n_rows; a.len = max_len; a.seqs = n_seq; a.d = d; a.reverse = reverse;
-    return scan_dispatch<true>(a, dtype, form, width, max_len, static_cast<cudaStream_t>(stream));
+    return scan_dispatch<true>(a, dtype, form, width, max_len, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -95,10 +95,11 @@ _SIGS = {
     "ffn_rmsnorm_bwd_workspace": (C.c_uint64, [C.c_int64, C.c_int32]),
     "ffn_rmsnorm_bwd": (C.c_int, [_VP, C.c_int64, _VP, C.c_int64, _VP, C.c_int64, _VP, _VP, _VP, C.c_int64, _VP, _VP, _VP, C.c_uint64,
                                   C.c_int64, C.c_int32, C.c_int, _VP]),
+    "ffn_gated_scan_workspace": (C.c_uint64, [C.c_int32, C.c_int64, C.c_int32]),
     "ffn_gated_scan": (C.c_int, [_VP, C.c_int64, _VP, C.c_int64, _VP, _VP, _VP, _VP, C.c_int64, C.c_int32, C.c_int64,
-                                 C.c_int32, C.c_int, C.c_int, C.c_int, _VP]),
+                                 C.c_int32, C.c_int, C.c_int, C.c_int, _VP, C.c_uint64, _VP]),
     "ffn_gated_scan_bwd": (C.c_int, [_VP, C.c_int64, _VP, _VP, C.c_int64, _VP, C.c_int64, _VP, C.c_int64] + [_VP] * 5
-                           + [C.c_int64, C.c_int32, C.c_int64, C.c_int32, C.c_int, C.c_int, C.c_int, _VP]),
+                           + [C.c_int64, C.c_int32, C.c_int64, C.c_int32, C.c_int, C.c_int, C.c_int, _VP, C.c_uint64, _VP]),
     "ffn_expert_mm_workspace": (C.c_uint64, [_VP, C.c_int64, _VP, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int]),
     "ffn_expert_mm": (C.c_int, [_VP, C.c_int64] + [_VP] * 5 + [C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int,
                                 C.c_int, _VP, C.c_uint64, _VP]),

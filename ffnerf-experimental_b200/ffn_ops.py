@@ -254,8 +254,9 @@ def gated_scan(gate, value, h0=None, offsets=None, max_len: int | None = None, f
     rows = seqs * max_len if off is None else gate.shape[0]
     if seqs == 0:
         return h.zero_(), last
+    buf, p, size = _workspace(gate.device, "ffn_gated_scan_workspace", seqs, max_len, d)
     _call("ffn_gated_scan", gate.device, gp, g_ld, vp, v_ld, p0, off, h.data_ptr(), last.data_ptr(), rows, seqs,
-          max_len, d, DTYPES[gate.dtype], SCAN_FORMS[form], 1 if reverse else 0)
+          max_len, d, DTYPES[gate.dtype], SCAN_FORMS[form], 1 if reverse else 0, p, size)
     return h, last
 
 
@@ -277,9 +278,10 @@ def gated_scan_bwd(dh, gate, value, h, h0=None, dh_last=None, offsets=None, max_
     rows = seqs * max_len if off is None else gate.shape[0]
     if seqs == 0:
         return dgate.zero_(), dvalue.zero_(), dh0
+    buf, p, size = _workspace(dev, "ffn_gated_scan_workspace", seqs, max_len, d)
     _call("ffn_gated_scan_bwd", dev, dp, d_ld, pl, gp, g_ld, vp, v_ld, hp, h_ld, p0, off, dgate.data_ptr(),
           dvalue.data_ptr(), dh0.data_ptr(), rows, seqs, max_len, d, DTYPES[gate.dtype], SCAN_FORMS[form],
-          1 if reverse else 0)
+          1 if reverse else 0, p, size)
     return dgate, dvalue, dh0
 
 
@@ -367,7 +369,7 @@ def expert_mm_bwd(dy, x, w, offsets, need_dx: bool = True, need_dw: bool = True,
 def status(device=None) -> int:
     """Status word of the block operators on the current (or given) device since the last call; waits for
     the device.  0 when every kernel completed normally; ``ffn_native.STATUS_TC_TIMEOUT`` when a wait of
-    an expert product or of a split recurrence ran out and its results are wrong."""
+    an expert product ran out and its results are incomplete."""
     import ctypes
     v = ctypes.c_uint32()
     with torch.cuda.device(device):

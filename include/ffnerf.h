@@ -328,18 +328,22 @@ int ffn_rmsnorm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, 
  * offsets[s+1] - 1 (32-bit, on the device, non-decreasing, at most n_rows; it may be empty: h_last is
  * then h0), or max_len rows each when offsets is NULL.  With offsets max_len is how long a sequence is
  * expected to get: it chooses how the work is split and bounds nothing.  Rows of no sequence get
- * zeros.  reverse != 0 runs each sequence from its last row to its first.  State is fp32; h is dtype. */
+ * zeros.  reverse != 0 runs each sequence from its last row to its first.  State is fp32; h is dtype.
+ * workspace: ffn_gated_scan_workspace bytes, 16-byte aligned (0 where
+ * sequences and channels alone fill the device). */
 enum { FFN_SCAN_LINEAR = 0, FFN_SCAN_SIGMOID = 1 };
+uint64_t ffn_gated_scan_workspace(int32_t n_seq, int64_t max_len, int32_t d);
 int ffn_gated_scan(const void* gate, int64_t gate_ld, const void* value, int64_t value_ld, const float* h0,
                    const int32_t* offsets, void* h, float* h_last, int64_t n_rows, int32_t n_seq, int64_t max_len,
-                   int32_t d, int dtype, int form, int reverse, void* stream);
+                   int32_t d, int dtype, int form, int reverse, void* workspace, uint64_t workspace_bytes, void* stream);
 /* Its backward pass from the gradient dh of h, the gradient dh_last of h_last (fp32, may be NULL) and the
  * forward pass's inputs and h: dgate, dvalue (dtype) and dh0 (fp32, may be NULL).  value is not read
  * in the linear form (may be NULL).  form, reverse and offsets as in the forward call. */
 int ffn_gated_scan_bwd(const void* dh, int64_t dh_ld, const float* dh_last, const void* gate, int64_t gate_ld,
                        const void* value, int64_t value_ld, const void* h, int64_t h_ld, const float* h0,
                        const int32_t* offsets, void* dgate, void* dvalue, float* dh0, int64_t n_rows, int32_t n_seq,
-                       int64_t max_len, int32_t d, int dtype, int form, int reverse, void* stream);
+                       int64_t max_len, int32_t d, int dtype, int form, int reverse, void* workspace,
+                       uint64_t workspace_bytes, void* stream);
 
 /* Matrix products of rows grouped by expert.  Rows are sorted by expert; expert e has rows
  * offsets[e] .. offsets[e+1] - 1 (32-bit, on the device, experts + 1 of them, offsets[0] = 0,
@@ -366,8 +370,8 @@ int ffn_expert_mm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld
                       void* workspace, uint64_t workspace_bytes, void* stream);
 
 /* Reads and clears the current device's status word of the block operators (waits for the device): 0
- * when every kernel completed normally; bit 2 = a wait of an expert product or of a
- * recurrence split over a cluster exceeded its bound and the kernel gave it up, its results wrong. */
+ * when every kernel completed normally; bit 2 = a wait of an expert product exceeded its bound and the
+ * kernel gave up, its results incomplete. */
 int ffn_ops_status(uint32_t* status);
 
 #ifdef __cplusplus

@@ -26,11 +26,11 @@ def test_entry_points_check_their_arguments():
     refused(lib.ffn_rmsnorm(None, 8, None, 0, p, None, p, None, None, 4, 8, 1e-6, 1, 1, 0, None), lib, "NULL")
     refused(lib.ffn_rmsnorm(p, 7, None, 0, p, None, p, None, None, 4, 8, 1e-6, 1, 1, 0, None), lib, "stride")
     refused(lib.ffn_rmsnorm_bwd(p, 8, p, 8, None, 0, p, p, None, 0, p, None, p, 0, 4, 8, 1, None), lib, "NULL")
-    refused(lib.ffn_gated_scan(p, 4, p, 4, None, None, p, None, 12, 3, 5, 4, 0, 1, 0, None), lib, "n_seq * max_len")
-    refused(lib.ffn_gated_scan(p, 4, p, 4, None, None, p, None, 15, 3, 5, 4, 0, 2, 0, None), lib, "form")
-    refused(lib.ffn_gated_scan(p, 4, p, 4, None, p, p, None, 1 << 31, 3, 5, 4, 0, 0, 0, None), lib, "32 bits")
-    refused(lib.ffn_gated_scan(p, 3, p, 4, None, None, p, None, 15, 3, 5, 4, 0, 0, 0, None), lib, "stride")
-    refused(lib.ffn_gated_scan_bwd(p, 4, None, p, 4, None, 0, p, 4, None, None, p, p, None, 15, 3, 5, 4, 0, 1, 0, None), lib,
+    refused(lib.ffn_gated_scan(p, 4, p, 4, None, None, p, None, 12, 3, 5, 4, 0, 1, 0, None, 0, None), lib, "n_seq * max_len")
+    refused(lib.ffn_gated_scan(p, 4, p, 4, None, None, p, None, 15, 3, 5, 4, 0, 2, 0, None, 0, None), lib, "form")
+    refused(lib.ffn_gated_scan(p, 4, p, 4, None, p, p, None, 1 << 31, 3, 5, 4, 0, 0, 0, None, 0, None), lib, "32 bits")
+    refused(lib.ffn_gated_scan(p, 3, p, 4, None, None, p, None, 15, 3, 5, 4, 0, 0, 0, None, 0, None), lib, "stride")
+    refused(lib.ffn_gated_scan_bwd(p, 4, None, p, 4, None, 0, p, 4, None, None, p, p, None, 15, 3, 5, 4, 0, 1, 0, None, 0, None), lib,
             "NULL")
     refused(lib.ffn_expert_mm(p, 8, p, p, None, None, p, 4, 0, 8, 8, 1, 1, None, 0, None), lib, "experts")
     refused(lib.ffn_expert_mm(p, 8, p, p, None, None, p, 4, 5000, 8, 8, 1, 1, None, 0, None), lib, "experts")
