@@ -20,10 +20,10 @@
 // loads are all issued before the first is used.  Threads are numbered over (sequence, channels) so
 // that narrow rows fill warps too.  Every element is read and written once: HBM is the bound, and what
 // the kernel needs is enough loads in flight.  Where sequences x channels give too few threads for
-// that, each sequence's time is cut into parts and there are two launches: the first composes the map of
-// every part, walking it from its end to its beginning, the second goes through each part from the state
-// that the maps before it give.  That reads the gates and inputs a second time, in part from L2 (the
-// first launch ends where the second begins); in return every thread streams its own part and waits for
+// that, each sequence's time is cut into parts and there are three launches: one composes the map of
+// every part, walking it from its end to its beginning, a small one joins the maps into the states that
+// the parts begin with, and the last goes through each part.  That reads the gates and inputs a second time, in part from L2 (the
+// first launch ends where the last begins); in return every thread streams its own part and waits for
 // nobody.  A one-read form was built and measured: blocks of a cluster that take turns along time and
 // exchange maps through distributed shared memory (with a cluster barrier, then with st.async and
 // mbarriers).  A turn's chain -- map, exchange, composition -- took 3 us of which memory was a quarter:
@@ -270,12 +270,14 @@ __global__ void __launch_bounds__(256, 2) scan_maps_kernel(const ScanArgs a) {
 #pragma unroll
     for (int j = 0; j < C; ++j) m[j] = Affine{1.0f, 0.0f};
     const int64_t chunks = (hi - lo + U - 1) / U;
+    Chunk<T, SIG, BACK, C, U> next;                    // loads of the next chunk fly while this one is used
+    if (chunks > 0) next.template load<true>(a, s, lo + (chunks - 1) * U, (int)(hi - lo - (chunks - 1) * U), ch);
 #pragma unroll 1
     for (int64_t q = chunks - 1; q >= 0; --q) {
         const int64_t t = lo + q * U;
         const int left = (int)min(hi - t, (int64_t)U);
-        Chunk<T, SIG, BACK, C, U> k;
-        k.template load<true>(a, s, t, left, ch);
+        const Chunk<T, SIG, BACK, C, U> k = next;
+        if (q > 0) next.template load<true>(a, s, t - U, U, ch);
 #pragma unroll
         for (int i = U - 1; i >= 0; --i)
             if (i < left) {
@@ -299,7 +301,47 @@ __global__ void __launch_bounds__(256, 2) scan_maps_kernel(const ScanArgs a) {
     *reinterpret_cast<Pack<float, C>*>(out + plane) = *reinterpret_cast<const Pack<float, C>*>(h);
 }
 
-// Goes through each thread's steps and writes the results.
+// Turns the maps into the states that the parts begin with, in place (part q + 1's state lies where part
+// q's p was): 32 channels x 32 groups of parts a block; each group's map first, then the states before
+// the groups, then those inside them.  (Each thread composing the maps before its own part instead
+// costs an L2 latency for every few parts: 28 us at 222 parts.)
+template <bool BACK>
+__global__ void __launch_bounds__(1024) scan_join_kernel(const ScanArgs a) {
+    __shared__ Affine group[32][32];
+    __shared__ float begin[32][32];
+    const int x = threadIdx.x, y = threadIdx.y;
+    const int64_t plane = (int64_t)a.seqs * a.d, c = (int64_t)blockIdx.x * 32 + x;
+    const int maps = a.parts - 1, each = (maps + 31) / 32, lo = min(y * each, maps), hi = min(lo + each, maps);
+    float* at = a.maps + c;
+    Affine m{1.0f, 0.0f};
+    if (c < plane)
+#pragma unroll 4
+        for (int q = lo; q < hi; ++q) {
+            const Affine n{at[q * 2 * plane], at[(q * 2 + 1) * plane]};
+            m.h = apply(n, m.h);
+            m.p *= n.p;
+        }
+    group[y][x] = m;
+    __syncthreads();
+    if (y == 0 && c < plane) {
+        const float* first = BACK ? a.dlast : a.h0;
+        float s = first ? first[c] : 0.0f;
+        for (int g = 0; g < 32; ++g) {
+            begin[g][x] = s;
+            s = apply(group[g][x], s);
+        }
+    }
+    __syncthreads();
+    if (c < plane) {
+        float s = begin[y][x];
+#pragma unroll 4
+        for (int q = lo; q < hi; ++q) {
+            s = apply(Affine{at[q * 2 * plane], at[(q * 2 + 1) * plane]}, s);
+            at[q * 2 * plane] = s;
+        }
+    }
+}
+
 template <typename T, bool SIG, bool BACK, int C, int U>
 __global__ void __launch_bounds__(256, 2) scan_kernel(const ScanArgs a) {
     const int64_t item = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -307,24 +349,19 @@ __global__ void __launch_bounds__(256, 2) scan_kernel(const ScanArgs a) {
     const int part = blockIdx.y, seq = (int)(item / a.groups), ch = (int)(item % a.groups) * C;
     const Span s = span_of<BACK>(a, seq);
     float state[C];
-    first_state<BACK, C>(a, seq, ch, state);
-    const int64_t plane = (int64_t)a.seqs * a.d;
-    const float* mp = a.maps + (int64_t)seq * a.d + ch;
-#pragma unroll 8
-    for (int q = 0; q < part; ++q, mp += 2 * plane) {
-        float p[C], h[C];
-        load_floats<C>(mp, p);
-        load_floats<C>(mp + plane, h);
-#pragma unroll
-        for (int j = 0; j < C; ++j) state[j] = apply(Affine{p[j], h[j]}, state[j]);
-    }
+    if (part == 0) first_state<BACK, C>(a, seq, ch, state);
+    else load_floats<C>(a.maps + (int64_t)(part - 1) * 2 * a.seqs * a.d + (int64_t)seq * a.d + ch, state);
     int64_t lo, hi;
     part_of<U>(a, s, part, lo, hi);
+    constexpr bool AHEAD = !BACK;                      // (four streams and their successors do not fit the registers)
+    Chunk<T, SIG, BACK, C, U> next;
+    if (AHEAD && lo < hi) next.template load<false>(a, s, lo, (int)min(hi - lo, (int64_t)U), ch);
 #pragma unroll 1
     for (int64_t t = lo; t < hi; t += U) {
         const int left = (int)min(hi - t, (int64_t)U);
-        Chunk<T, SIG, BACK, C, U> k;
-        k.template load<false>(a, s, t, left, ch);
+        if (!AHEAD) next.template load<false>(a, s, t, left, ch);
+        const Chunk<T, SIG, BACK, C, U> k = next;
+        if (AHEAD && t + U < hi) next.template load<false>(a, s, t + U, (int)min(hi - t - U, (int64_t)U), ch);
         int64_t at = (s.first + t * s.dir) * a.d + ch;
 #pragma unroll
         for (int i = 0; i < U; ++i)
@@ -356,7 +393,7 @@ ScanPlan scan_plan(int64_t seqs, int d, int most_width, int64_t longest, int sms
     int width = most_width < 2 ? most_width : 2;
     if (warps(width) * 3 > want * 2 || longest < 4 * PART_STEPS) return {width, 1};
     width = most_width;
-    int64_t parts = want / warps(width);
+    int64_t parts = want / warps(width);                  // what is resident at once
     if (parts > longest / PART_STEPS) parts = longest / PART_STEPS;
     return {width, (int)(parts < 65535 ? parts : 65535)};
 }
@@ -372,6 +409,9 @@ int scan_launch(ScanArgs a, int parts, cudaStream_t st) {
     if (parts > 1) {
         scan_maps_kernel<T, SIG, BACK, C, U><<<dim3((unsigned)blocks, parts - 1), threads, 0, st>>>(a);
         if (int rc = op_launched("ffn_gated_scan maps")) return rc;
+        const int64_t joins = ((int64_t)a.seqs * a.d + 31) / 32;
+        scan_join_kernel<BACK><<<(unsigned)joins, dim3(32, 32), 0, st>>>(a);
+        if (int rc = op_launched("ffn_gated_scan join")) return rc;
     }
     scan_kernel<T, SIG, BACK, C, U><<<dim3((unsigned)blocks, parts), threads, 0, st>>>(a);
     return op_launched("ffn_gated_scan");
