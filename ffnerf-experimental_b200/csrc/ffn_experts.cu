@@ -72,23 +72,67 @@ __device__ __forceinline__ void expert_rows(const Args& p, int e, int64_t& b, in
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
     return tc::make_desc(saddr, lbo, sbo) | (2ull << 61);
 }
-__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n"
-                 :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc));
+// D (+)= A B^T, issued by one thread; PAIR: the operands' and the accumulator's halves lie in both blocks.
+template <int EB, bool PAIR>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+#define FFN_MMA(group, kind)                                                                                     \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"                                              \
+                 "tcgen05.mma." group "." kind " [%0], %1, %2, %3, p;\n\t}\n"                                   \
+                 :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc))
+    if constexpr (PAIR) {
+        if constexpr (EB == 1) FFN_MMA("cta_group::2", "kind::f8f6f4"); else FFN_MMA("cta_group::2", "kind::f16");
+    } else {
+        if constexpr (EB == 1) FFN_MMA("cta_group::1", "kind::f8f6f4"); else FFN_MMA("cta_group::1", "kind::f16");
+    }
+#undef FFN_MMA
 }
-__device__ __forceinline__ void mma_16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
-                 :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc));
+// Loads into this block's shared memory; PAIR: the bytes count on an mbarrier of the pair's first block.
+template <bool PAIR>
+__device__ __forceinline__ void tma_load2(uint32_t dst, const CUtensorMap* m, int x, int y, uint32_t bar) {
+    if constexpr (PAIR)
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+                     "[%0], [%1, {%2, %3}], [%4];" :: "r"(dst), "l"(m), "r"(x), "r"(y), "r"(bar) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes "
+                     "[%0], [%1, {%2, %3}], [%4];" :: "r"(dst), "l"(m), "r"(x), "r"(y), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void tma_load2(uint32_t dst, const CUtensorMap* m, int x, int y, uint64_t* bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                 :: "r"(dst), "l"(m), "r"(x), "r"(y), "r"(tc::smem_u32(bar)) : "memory");
+template <bool PAIR>
+__device__ __forceinline__ void tma_load3(uint32_t dst, const CUtensorMap* m, int x, int y, int z, uint32_t bar) {
+    if constexpr (PAIR)
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+                     "[%0], [%1, {%2, %3, %4}], [%5];" :: "r"(dst), "l"(m), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes "
+                     "[%0], [%1, {%2, %3, %4}], [%5];" :: "r"(dst), "l"(m), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void tma_load3(uint32_t dst, const CUtensorMap* m, int x, int y, int z, uint64_t* bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                 :: "r"(dst), "l"(m), "r"(x), "r"(y), "r"(z), "r"(tc::smem_u32(bar)) : "memory");
+// A shared address of this block as the same place in block `rank` of the cluster.
+__device__ __forceinline__ uint32_t in_block(uint32_t addr, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ int cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return (int)r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// Arrives on `bar` of both blocks of the pair when the products issued so far are done.
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 :: "r"(tc::smem_u32(bar)), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(tc::smem_u32(dst)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t at, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(at), "r"(cols) : "memory");
+}
+__device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(cluster_addr) : "memory");
 }
 __device__ __forceinline__ void tma_store2(const CUtensorMap* m, int x, int y, uint32_t src) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
@@ -131,10 +175,12 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, fl
 }
 
 // Shape of a variant: bytes of a stage, stages, and the layout of shared memory.
-template <int MODE, int BN, int EB>
+template <int MODE, int BN, int EB, bool PAIR>
 struct Plan {
+    static constexpr int ROWS = MODE == FEW_ROWS ? BN : PAIR ? 2 * BM : BM;   // of a tile
+    static constexpr int BH = PAIR ? BN / 2 : BN;                             // this block's share of B
     static constexpr int A_BYTES = BM * KB;
-    static constexpr int B_BYTES = BN * KB;
+    static constexpr int B_BYTES = BH * KB;
     static constexpr int STAGE = A_BYTES + B_BYTES;
     static constexpr int EPI = MODE == FEW_ROWS ? 0 : EPI_WARPS * SLAB;
     static constexpr int MISC = 1024 + 4 * (FFN_MAX_EXPERTS + 1) + 512;   // alignment, prefix, barriers
@@ -165,7 +211,7 @@ __device__ __forceinline__ bool elect() {
 
 // Each role goes through this block's tiles in the same order; the walk keeps the expert it is at, so
 // that the next tile costs a comparison, and offsets are read only where the expert changes.
-template <int MODE, int BN, int EB>
+template <int MODE, int BN, int EB, bool PAIR>
 struct Walk {
     int e = 0, start = 0, stop = 0;      // this expert's tiles are start .. stop - 1
     int64_t b = 0, end = 0;              // its rows
@@ -214,10 +260,10 @@ struct Walk {
                 c = r / tiles;
                 r -= c * tiles;
             }
-            k.row = b + (int64_t)r * (MODE == FEW_ROWS ? BN : BM);
+            k.row = b + (int64_t)r * Plan<MODE, BN, EB, PAIR>::ROWS;
             k.col = c * (MODE == FEW_ROWS ? BM : BN);
             k.mrow = k.plane = 0;
-            constexpr int D = Plan<MODE, BN, EB>::DEPTH;
+            constexpr int D = Plan<MODE, BN, EB, PAIR>::DEPTH;
             k.blocks = (p.depth + D - 1) / D;
         }
         return k;
@@ -235,11 +281,12 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
     return false;
 }
 
-template <int MODE, int BN, int EB, typename TO, bool BF>
+template <int MODE, int BN, int EB, typename TO, bool BF, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1)
 experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb,
                const __grid_constant__ CUtensorMap mo) {
-    using P = Plan<MODE, BN, EB>;
+    using P = Plan<MODE, BN, EB, PAIR>;
+    static_assert(!PAIR || ((MODE == FORWARD || MODE == INPUT_GRAD) && BN == 256), "pairs form 256 x 256 tiles");
     constexpr int S = P::STAGES;
     extern __shared__ unsigned char raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -252,17 +299,20 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(freed + 2);
     volatile int* gone = reinterpret_cast<volatile int*>(tmem_at + 1);
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int rank = PAIR ? uniform(cluster_rank()) : 0;                      // in the pair
+    const int first = PAIR ? (int)blockIdx.x >> 1 : (int)blockIdx.x, stride = PAIR ? (int)gridDim.x >> 1 : (int)gridDim.x;
 
     if (warp == EPI_WARPS + 1) {
-        tc::tmem_alloc(tmem_at, P::TMEM_COLS);
+        if constexpr (PAIR) tmem_alloc_pair(tmem_at, P::TMEM_COLS);
+        else tc::tmem_alloc(tmem_at, P::TMEM_COLS);
         if (lane == 0) {
             for (int i = 0; i < S; ++i) { tc::mbar_init(full + i, 1); tc::mbar_init(empty + i, 1); }
-            for (int i = 0; i < 2; ++i) { tc::mbar_init(done + i, 1); tc::mbar_init(freed + i, 4); }
+            for (int i = 0; i < 2; ++i) { tc::mbar_init(done + i, 1); tc::mbar_init(freed + i, PAIR ? 8 : 4); }
             *gone = 0;
         }
     }
     // tiles (dW: units) of the experts before each: counts side by side, then one warp adds them up
-    constexpr int R = MODE == FEW_ROWS ? BN : BM;
+    constexpr int R = P::ROWS;
     for (int e = threadIdx.x; e < p.experts; e += THREADS) {
         int64_t b, end;
         expert_rows(p, e, b, end);
@@ -290,50 +340,56 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
     __syncthreads();
     const int total = prefix[p.experts] * (MODE == WEIGHT_GRAD ? p.ntiles * p.mtiles : p.ntiles);
     tc::fence_before_sync();
-    __syncthreads();
+    if constexpr (PAIR) cluster_sync();              // both blocks' barriers are ready
+    else __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
 
     if (warp == EPI_WARPS) {                                     // ---- loads
-        Walk<MODE, BN, EB> walk;
+        Walk<MODE, BN, EB, PAIR> walk;
         int s = 0, issued = 0;
         uint32_t ph = 1;
         bool ok = true;
-        for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+        for (int t = first; t < total && ok; t += stride) {
             const Tile k = walk.at(p, prefix, t);
-            const int blocks = uniform(k.blocks), row = uniform((int)k.row), col = uniform(k.col), e = uniform(k.e);
+            const int blocks = uniform(k.blocks), row = uniform((int)k.row) + rank * BM, col = uniform(k.col) + rank * P::BH,
+                      e = uniform(k.e);
             [[maybe_unused]] const int mrow = uniform(k.mrow);
             for (int b = 0; b < blocks; ++b) {
                 if (!(ok = wait(empty + s, ph, gone))) break;
                 const uint32_t sa = tc::smem_u32(base + (size_t)s * P::STAGE), sb = sa + P::A_BYTES;
+                // PAIR: the bytes of both blocks count on the first block's barrier
+                const uint32_t bar = PAIR ? in_block(tc::smem_u32(full + s), 0) : tc::smem_u32(full + s);
                 if (elect()) {
                     if constexpr (MODE == FORWARD) {
-                        expect_tx(full + s, P::STAGE);
-                        tma_load2(sa, &ma, b * P::DEPTH, row, full + s);
-                        tma_load3(sb, &mb, b * P::DEPTH, col, e, full + s);
+                        if (rank == 0) expect_tx(full + s, PAIR ? 2 * P::STAGE : P::STAGE);
+                        tma_load2<PAIR>(sa, &ma, b * P::DEPTH, row, bar);
+                        tma_load3<PAIR>(sb, &mb, b * P::DEPTH, col, e, bar);
                     } else if constexpr (MODE == FEW_ROWS) {
                         expect_tx(full + s, P::STAGE);
-                        tma_load3(sa, &ma, b * P::DEPTH, col, e, full + s);
-                        tma_load2(sb, &mb, b * P::DEPTH, row, full + s);
+                        tma_load3<PAIR>(sa, &ma, b * P::DEPTH, col, e, bar);
+                        tma_load2<PAIR>(sb, &mb, b * P::DEPTH, row, bar);
                     } else {
                         // boxes of 64 columns; those wholly outside the matrix are left out (what is in
                         // their place reaches only outputs that are not stored)
-                        const int nb = min(BN / 64, (p.cols - col + 63) / 64);
+                        auto boxes = [&](int c) { return max(0, min(P::BH / 64, (p.cols - c + 63) / 64)); };
+                        const int nb = boxes(col);
                         if constexpr (MODE == INPUT_GRAD) {
-                            expect_tx(full + s, P::A_BYTES + nb * 8192);
-                            tma_load2(sa, &ma, b * 64, row, full + s);
+                            if (rank == 0)
+                                expect_tx(full + s, (PAIR ? 2 : 1) * P::A_BYTES + (nb + (PAIR ? boxes(col + P::BH) : 0)) * 8192);
+                            tma_load2<PAIR>(sa, &ma, b * 64, row, bar);
 #pragma unroll
-                            for (int j = 0; j < BN / 64; ++j)
-                                if (j < nb) tma_load3(sb + j * 8192, &mb, col + j * 64, b * 64, e, full + s);
+                            for (int j = 0; j < P::BH / 64; ++j)
+                                if (j < nb) tma_load3<PAIR>(sb + j * 8192, &mb, col + j * 64, b * 64, e, bar);
                         } else {
                             const int na = min(BM / 64, (p.rows_m - mrow + 63) / 64);
                             expect_tx(full + s, (na + nb) * 8192);
 #pragma unroll
                             for (int j = 0; j < BM / 64; ++j)
-                                if (j < na) tma_load2(sa + j * 8192, &ma, mrow + j * 64, row + b * 64, full + s);
+                                if (j < na) tma_load2<PAIR>(sa + j * 8192, &ma, mrow + j * 64, row + b * 64, bar);
 #pragma unroll
                             for (int j = 0; j < BN / 64; ++j)
-                                if (j < nb) tma_load2(sb + j * 8192, &mb, col + j * 64, row + b * 64, full + s);
+                                if (j < nb) tma_load2<PAIR>(sb + j * 8192, &mb, col + j * 64, row + b * 64, bar);
                         }
                     }
                 }
@@ -342,20 +398,20 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
                 if (++s == S) { s = 0; ph ^= 1; }
             }
         }
-        if (!ok)                                                  // let the copies in flight land
+        if (!ok && rank == 0)                                     // let the copies in flight land
             for (int i = 0; i < (issued < S ? issued : S); ++i) {
                 const int q = issued - 1 - i;
                 tc::mbar_wait(full + q % S, (uint32_t)(q / S) & 1u, 1u << 20);
             }
-    } else if (warp == EPI_WARPS + 1) {                           // ---- products
+    } else if (warp == EPI_WARPS + 1) {                           // ---- products (PAIR: issued by the first block)
         constexpr bool A_MN = MODE == WEIGHT_GRAD, B_MN = MODE == INPUT_GRAD || MODE == WEIGHT_GRAD;
-        constexpr uint32_t IDESC = tc::idesc_f16(BM, BN, A_MN, B_MN) |
+        constexpr uint32_t IDESC = tc::idesc_f16(PAIR ? 2 * BM : BM, BN, A_MN, B_MN) |
                                    (EB == 2 && BF ? (1u << 7) | (1u << 10) : 0u);
-        Walk<MODE, BN, EB> walk;
+        Walk<MODE, BN, EB, PAIR> walk;
         int s = 0, acc = 0;
         uint32_t ph = 0, aph = 1;
         bool ok = true;
-        for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+        for (int t = first; t < total && ok && rank == 0; t += stride) {
             int blocks;
             [[maybe_unused]] int rows = 0;                        // dW: rows of depth from the tile's first on
             if constexpr (MODE == WEIGHT_GRAD) {
@@ -395,11 +451,15 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         if (MODE != WEIGHT_GRAD || i < steps) {
-                            if constexpr (EB == 1) mma_f8(d, da + i * STEP_A, db + i * STEP_B, IDESC, (b | i) != 0);
-                            else mma_16(d, da + i * STEP_A, db + i * STEP_B, IDESC, (b | i) != 0);
+                            mma<EB, PAIR>(d, da + i * STEP_A, db + i * STEP_B, IDESC, (b | i) != 0);
                         }
-                    tc::commit(empty + s);
-                    if (b == blocks - 1) tc::commit(done + acc);
+                    if constexpr (PAIR) {
+                        commit_pair(empty + s);
+                        if (b == blocks - 1) commit_pair(done + acc);
+                    } else {
+                        tc::commit(empty + s);
+                        if (b == blocks - 1) tc::commit(done + acc);
+                    }
                 }
                 __syncwarp();
                 if (++s == S) { s = 0; ph ^= 1; }
@@ -415,10 +475,10 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
         uint32_t aph = 0;
         TO* out = static_cast<TO*>(p.out);
         unsigned char* sl = slabs + warp * SLAB;
-        Walk<MODE, BN, EB> walk;
-        for (int t = blockIdx.x + acc * gridDim.x; t < total; t += 2 * gridDim.x) {
+        Walk<MODE, BN, EB, PAIR> walk;
+        for (int t = first + acc * stride; t < total; t += 2 * stride) {
             const Tile k = walk.at(p, prefix, t);
-            const int64_t row = (MODE == WEIGHT_GRAD ? k.mrow : k.row) + quarter * 32;  // this warp's first row
+            const int64_t row = (MODE == WEIGHT_GRAD ? k.mrow : k.row + rank * BM) + quarter * 32;  // this warp's first row
             const int64_t end = MODE == WEIGHT_GRAD ? p.rows_m : k.end;
             float sr = 1.0f;
             if constexpr (EB == 1 && MODE == FORWARD) sr = row + lane < end ? __ldg(p.a_scale + row + lane) : 0.0f;
@@ -514,7 +574,10 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
             }
             tc::fence_before_sync();
             __syncwarp();
-            if (lane == 0) arrive(freed + acc);
+            if (lane == 0) {
+                if constexpr (PAIR) arrive_at(in_block(tc::smem_u32(freed + acc), 0));
+                else arrive(freed + acc);
+            }
             aph ^= 1;
         }
         if (lane == 0) bulk_wait_read<0>();
@@ -528,10 +591,12 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
         }
     }
     tc::fence_before_sync();
-    __syncthreads();
+    if constexpr (PAIR) cluster_sync();              // nothing of the other block's is on its way here any more
+    else __syncthreads();
     if (warp == EPI_WARPS + 1) {
         tc::fence_after_sync();
-        tc::tmem_dealloc(tmem, P::TMEM_COLS);
+        if constexpr (PAIR) tmem_dealloc_pair(tmem, P::TMEM_COLS);
+        else tc::tmem_dealloc(tmem, P::TMEM_COLS);
     }
 }
 
@@ -611,11 +676,11 @@ Operand pad(const void* p, int64_t ld, int64_t rows, int cols, int dtype, unsign
 // The most units that n rows make.
 int64_t units_most(int64_t n, int experts, int chunk) { return chunk ? n / (64 * (int64_t)chunk) + experts : experts; }
 
-template <int MODE, int BN, int EB, typename TO, bool BF>
+template <int MODE, int BN, int EB, typename TO, bool BF, bool PAIR>
 int launch(const Args& a0, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, int sms, cudaStream_t st) {
-    using P = Plan<MODE, BN, EB>;
+    using P = Plan<MODE, BN, EB, PAIR>;
     Args a = a0;
-    constexpr int NT = MODE == FEW_ROWS ? BM : BN, RT = MODE == FEW_ROWS ? BN : BM;
+    constexpr int NT = MODE == FEW_ROWS ? BM : BN, RT = P::ROWS;
     a.ntiles = (a.cols + NT - 1) / NT;
     a.mtiles = (a.rows_m + BM - 1) / BM;
     // an upper bound of the tiles: the counts are on the device
@@ -623,7 +688,7 @@ int launch(const Args& a0, const CUtensorMap& ma, const CUtensorMap& mb, const C
     const int64_t tiles = most * a.ntiles * (MODE == WEIGHT_GRAD ? a.mtiles : 1);
     a.most = (int)most;
     if (tiles > 0x7fffffff) return op_fail(FFN_E_CAPACITY, "ffn_expert_mm: more than 2^31 output tiles");
-    auto k = experts_kernel<MODE, BN, EB, TO, BF>;
+    auto k = experts_kernel<MODE, BN, EB, TO, BF, PAIR>;
     static std::atomic<uint64_t> ready{0};            // devices whose limit is set
     int dev = 0;
     cudaGetDevice(&dev);
@@ -632,31 +697,49 @@ int launch(const Args& a0, const CUtensorMap& ma, const CUtensorMap& mb, const C
         if (e != cudaSuccess) return op_fail(FFN_E_CUDA, std::string("ffn_expert_mm: ") + cudaGetErrorString(e));
         if (dev <= 63) ready.fetch_or(1ull << dev, std::memory_order_release);
     }
-    k<<<(unsigned)(tiles < sms ? tiles : sms), THREADS, P::BYTES, st>>>(a, ma, mb, mo);
-    return op_launched("ffn_expert_mm");
+    if constexpr (PAIR) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)(2 * (tiles < sms / 2 ? tiles : sms / 2)));
+        cfg.blockDim = dim3(THREADS);
+        cfg.dynamicSmemBytes = P::BYTES;
+        cfg.stream = st;
+        cudaLaunchAttribute at{};
+        at.id = cudaLaunchAttributeClusterDimension;
+        at.val.clusterDim.x = 2;
+        at.val.clusterDim.y = at.val.clusterDim.z = 1;
+        cfg.attrs = &at;
+        cfg.numAttrs = 1;
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, k, a, ma, mb, mo);
+        return e == cudaSuccess ? FFN_OK : op_fail(FFN_E_CUDA, std::string("ffn_expert_mm: ") + cudaGetErrorString(e));
+    } else {
+        k<<<(unsigned)(tiles < sms ? tiles : sms), THREADS, P::BYTES, st>>>(a, ma, mb, mo);
+        return op_launched("ffn_expert_mm");
+    }
 }
 
-template <int MODE, int BN>
+template <int MODE, int BN, bool PAIR = false>
 int launch_typed(const Args& a, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, int dtype, int out_dtype,
                  int sms, cudaStream_t st) {
     if constexpr (MODE == FORWARD || MODE == FEW_ROWS) {
         if (dtype == FFN_E4M3)
-            return out_dtype == FFN_F16 ? launch<MODE, BN, 1, __half, false>(a, ma, mb, mo, sms, st)
-                                        : launch<MODE, BN, 1, __nv_bfloat16, false>(a, ma, mb, mo, sms, st);
+            return out_dtype == FFN_F16 ? launch<MODE, BN, 1, __half, false, PAIR>(a, ma, mb, mo, sms, st)
+                                        : launch<MODE, BN, 1, __nv_bfloat16, false, PAIR>(a, ma, mb, mo, sms, st);
     }
     if constexpr (MODE == WEIGHT_GRAD) {
         if (out_dtype == FFN_F32)
-            return dtype == FFN_F16 ? launch<MODE, BN, 2, float, false>(a, ma, mb, mo, sms, st)
-                                    : launch<MODE, BN, 2, float, true>(a, ma, mb, mo, sms, st);
+            return dtype == FFN_F16 ? launch<MODE, BN, 2, float, false, PAIR>(a, ma, mb, mo, sms, st)
+                                    : launch<MODE, BN, 2, float, true, PAIR>(a, ma, mb, mo, sms, st);
     }
-    return dtype == FFN_F16 ? launch<MODE, BN, 2, __half, false>(a, ma, mb, mo, sms, st)
-                            : launch<MODE, BN, 2, __nv_bfloat16, true>(a, ma, mb, mo, sms, st);
+    return dtype == FFN_F16 ? launch<MODE, BN, 2, __half, false, PAIR>(a, ma, mb, mo, sms, st)
+                            : launch<MODE, BN, 2, __nv_bfloat16, true, PAIR>(a, ma, mb, mo, sms, st);
 }
 
 int bad_map() { return op_fail(FFN_E_CUDA, "ffn_expert_mm: a tensor map could not be made"); }
 
 // Width of a tile: the widest that the output's width fills.
 int tile_width(int cols) { return cols > 128 ? 256 : cols > 64 ? 128 : 64; }
+
+constexpr int PAIR_ROWS = 512;       // rows an expert has on average from which on pairs of blocks are used
 
 // out[r] = a[r] b[e]^T (FORWARD, FEW_ROWS) or a[r] b[e] (INPUT_GRAD); depth and cols are those of the product.
 int rows_product(int mode, Operand a, Operand b, const float* a_scale, const float* b_scale, const int32_t* offsets, void* out,
@@ -676,15 +759,18 @@ int rows_product(int mode, Operand a, Operand b, const float* a_scale, const flo
                         : launch_typed<FEW_ROWS, 64>(p, ma, mb, mo, dtype, out_dtype, sms, st);
     }
     const int bn = tile_width(cols);
+    const bool pair = bn == 256 && n >= (int64_t)experts * PAIR_ROWS;
     if (p.tma_out && !make_map(&mo, out, out_dtype, cols, n, cols, 0, 32)) return bad_map();
     if (!make_map(&ma, a.p, dtype, depth, n, a.ld, 0, BM)) return bad_map();
     if (mode == FORWARD) {
-        if (!make_map(&mb, b.p, dtype, depth, cols, b.ld, experts, bn)) return bad_map();
+        if (!make_map(&mb, b.p, dtype, depth, cols, b.ld, experts, pair ? bn / 2 : bn)) return bad_map();
+        if (pair) return launch_typed<FORWARD, 256, true>(p, ma, mb, mo, dtype, out_dtype, sms, st);
         return bn == 256 ? launch_typed<FORWARD, 256>(p, ma, mb, mo, dtype, out_dtype, sms, st)
              : bn == 128 ? launch_typed<FORWARD, 128>(p, ma, mb, mo, dtype, out_dtype, sms, st)
                          : launch_typed<FORWARD, 64>(p, ma, mb, mo, dtype, out_dtype, sms, st);
     }
     if (!make_map(&mb, b.p, dtype, cols, depth, b.ld, experts, 64)) return bad_map();
+    if (pair) return launch_typed<INPUT_GRAD, 256, true>(p, ma, mb, mo, dtype, out_dtype, sms, st);
     return bn == 256 ? launch_typed<INPUT_GRAD, 256>(p, ma, mb, mo, dtype, out_dtype, sms, st)
          : bn == 128 ? launch_typed<INPUT_GRAD, 128>(p, ma, mb, mo, dtype, out_dtype, sms, st)
                      : launch_typed<INPUT_GRAD, 64>(p, ma, mb, mo, dtype, out_dtype, sms, st);

@@ -293,7 +293,8 @@ EXPERT_CASES = [  # rows of each expert, rows of none, in, out
     ([1], 0, 1, 1), ([1], 0, 64, 64), ([5, 0, 3], 2, 32, 48), ([128, 1, 0, 130], 0, 64, 64), ([0, 0], 3, 64, 64),
     ([17, 300, 64], 5, 200, 136), ([33] * 8, 0, 256, 512), ([700], 1, 1000, 264), ([9, 40, 0, 21], 7, 77, 131),
     ([2, 1, 0, 0, 4, 1, 0, 8], 0, 2048, 320), ([63, 65, 127, 129, 255], 1, 72, 40), ([1024, 512], 0, 128, 256),
-    ([10], 0, 8, 8), ([3000, 17, 0, 2100], 3, 72, 56), ([5000], 0, 200, 130)]
+    ([10], 0, 8, 8), ([3000, 17, 0, 2100], 3, 72, 56), ([5000], 0, 200, 130),
+    ([700, 513, 901], 3, 192, 264), ([1100, 0, 1537], 0, 320, 512)]
 
 
 def expert_inputs(case, dtype):
