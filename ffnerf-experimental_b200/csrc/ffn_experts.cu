@@ -302,6 +302,8 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
     const int rank = PAIR ? uniform(cluster_rank()) : 0;                      // in the pair
     const int first = PAIR ? (int)blockIdx.x >> 1 : (int)blockIdx.x, stride = PAIR ? (int)gridDim.x >> 1 : (int)gridDim.x;
 
+    if (warp == EPI_WARPS && lane < 3)               // the maps are fetched while the tiles are counted
+        asm volatile("prefetch.tensormap [%0];" :: "l"(lane == 0 ? &ma : lane == 1 ? &mb : &mo) : "memory");
     if (warp == EPI_WARPS + 1) {
         if constexpr (PAIR) tmem_alloc_pair(tmem_at, P::TMEM_COLS);
         else tc::tmem_alloc(tmem_at, P::TMEM_COLS);
@@ -736,10 +738,22 @@ int launch_typed(const Args& a, const CUtensorMap& ma, const CUtensorMap& mb, co
 
 int bad_map() { return op_fail(FFN_E_CUDA, "ffn_expert_mm: a tensor map could not be made"); }
 
-// Width of a tile: the widest that the output's width fills.
-int tile_width(int cols) { return cols > 128 ? 256 : cols > 64 ? 128 : 64; }
+// Width of a tile: what the output's width fills, halved while the tiles at hand leave half the SMs idle.
+// Both sides at 16-bit operands, in us (64 / 128 / 256 wide): 8 experts of 512 x 512 with 128 rows each
+// 8.7 / 9.2 / 10.6, with 512 rows 10.6 / 10.4 / 10.8, with 4096 rows 42.7 / 28.4 / 22.8; 4 experts of
+// 4096 x 1024 with 64 rows 22.7 / 24.7 / 30.5, with 512 rows 42.4 / 27.2 / 30.9.
+int tile_width(int cols, int64_t row_tiles, int sms) {
+    int bn = cols > 128 ? 256 : cols > 64 ? 128 : 64;
+    while (bn > 64 && row_tiles * ((cols + bn - 1) / bn) * 2 <= sms) bn /= 2;
+    return bn;
+}
 
-constexpr int PAIR_ROWS = 512;       // rows an expert has on average from which on pairs of blocks are used
+// Pairs of blocks: from so many rows an expert has on average, and while a pair of SMs still gets several
+// tiles.  Their tile holds twice the rows, so an expert's last tile wastes twice as much; per tile they read
+// a third less and hold half as many stages more in flight.  Forward, 16 experts of 1024 x 4096, pair /
+// single in us: 256 rows 43 / 46, 512 67 / 69, 1024 110 / 122, 2048 197 / 230; of 4096 x 1024: 512 rows
+// 76 / 66, 768 98 / 91, 1024 109 / 119, 2048 224 / 255; 64 experts of 256 x 320: 1024 rows 37 / 31.
+constexpr int PAIR_ROWS = 1024, PAIR_WORK = 1 << 20;   // rows an expert, elements of W
 
 // out[r] = a[r] b[e]^T (FORWARD, FEW_ROWS) or a[r] b[e] (INPUT_GRAD); depth and cols are those of the product.
 int rows_product(int mode, Operand a, Operand b, const float* a_scale, const float* b_scale, const int32_t* offsets, void* out,
@@ -758,8 +772,8 @@ int rows_product(int mode, Operand a, Operand b, const float* a_scale, const flo
              : bn == 32 ? launch_typed<FEW_ROWS, 32>(p, ma, mb, mo, dtype, out_dtype, sms, st)
                         : launch_typed<FEW_ROWS, 64>(p, ma, mb, mo, dtype, out_dtype, sms, st);
     }
-    const int bn = tile_width(cols);
-    const bool pair = bn == 256 && n >= (int64_t)experts * PAIR_ROWS;
+    const int bn = tile_width(cols, n / BM + (experts + 1) / 2, sms);
+    const bool pair = bn == 256 && n >= (int64_t)experts * PAIR_ROWS && (int64_t)depth * cols >= PAIR_WORK;
     if (p.tma_out && !make_map(&mo, out, out_dtype, cols, n, cols, 0, 32)) return bad_map();
     if (!make_map(&ma, a.p, dtype, depth, n, a.ld, 0, BM)) return bad_map();
     if (mode == FORWARD) {
@@ -806,12 +820,14 @@ __global__ void __launch_bounds__(256) units_sum_kernel(const Args p, const floa
     }
 }
 
+constexpr int64_t WIDE = 1 << 20;     // dW: the depth is cut instead of the tiles
+
 // Stages of depth in a unit of dW, or 0.  Experts share the rows unevenly and a small W has few output
 // tiles: 64 experts of 64 x 64 have 64, the largest of them several times the average depth.  Below two
 // tiles an SM the depth is cut into units, about four an SM in all and 16 stages at least, whose fp32
 // sums go through the workspace.
 int weight_chunk(int64_t n, int experts, int k, int m, int sms) {
-    const int bn = tile_width(k);
+    const int bn = tile_width(k, WIDE, sms);
     const int64_t per = (int64_t)((m + BM - 1) / BM) * ((k + bn - 1) / bn), blocks = n / 64 + experts;
     if (per * experts >= 2 * (int64_t)sms) return 0;
     const int64_t chunk = (blocks * per + 4 * sms - 1) / (4 * sms);
@@ -835,7 +851,7 @@ int weight_product(Operand dy, Operand x, const int32_t* offsets, void* dw, int6
     CUtensorMap ma, mb, mo{};
     if (p.tma_out && !make_map(&mo, out, out_type, k, m, k, units_most(n, experts, p.chunk), 32)) return bad_map();
     if (!make_map(&ma, dy.p, dtype, m, n, dy.ld, 0, 64) || !make_map(&mb, x.p, dtype, k, n, x.ld, 0, 64)) return bad_map();
-    const int bn = tile_width(k);
+    const int bn = tile_width(k, WIDE, sms);
     const int rc = bn == 256 ? launch_typed<WEIGHT_GRAD, 256>(p, ma, mb, mo, dtype, out_type, sms, st)
                  : bn == 128 ? launch_typed<WEIGHT_GRAD, 128>(p, ma, mb, mo, dtype, out_type, sms, st)
                              : launch_typed<WEIGHT_GRAD, 64>(p, ma, mb, mo, dtype, out_type, sms, st);
