@@ -1,14 +1,17 @@
 """Build recipe of libffnerf.so (the C-ABI library in include/ffnerf.h) for B200 / sm_100a.
 
 Compiles csrc/ffn_capi.cu (which includes the training step's kernels) and the block operators'
-translation units with nvcc, side by side, and links them into ``libffnerf.so`` next to this file.
-A unit is compiled again only when one of its sources is newer than its object.
+translation units with nvcc, side by side, and links them into ``libffnerf.so`` next to this file, then
+compiles the Python module ``_ffn_ops.so`` (csrc/ffn_ops_torch.cpp: the block operators on torch
+tensors), which links to it.  A unit is compiled again only when one of its sources is newer than its
+object.
 """
 from __future__ import annotations
 
 import os
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -25,6 +28,8 @@ UNITS = {
     "ffn_scan.cu": ("ffn_ops.cuh",),
     "ffn_experts.cu": ("ffn_ops.cuh", "ffn_tcgen05.cuh"),
 }
+MODULE = HERE / "_ffn_ops.so"
+MODULE_SOURCE = CSRC / "ffn_ops_torch.cpp"
 SOURCES = [CSRC / n for n in sorted({f for u, inc in UNITS.items() for f in (u, *inc)})] + [HEADER]
 
 NVCC_FLAGS = [
@@ -54,6 +59,7 @@ def _compile(unit: str, force: bool, verbose: bool):
 def build(force: bool = False, verbose: bool = False) -> Path:
     newest = max(p.stat().st_mtime for p in SOURCES)
     if SO.exists() and SO.stat().st_mtime >= newest and not force:
+        build_module(force, verbose)
         return SO
     BUILD.mkdir(exist_ok=True)
     jobs = [j for j in (_compile(u, force, verbose) for u in UNITS) if j]
@@ -74,7 +80,31 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     if res.returncode != 0:
         raise RuntimeError(f"nvcc failed:\n{' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
     tmp.replace(SO)
+    build_module(force, verbose)
     return SO
+
+
+def build_module(force: bool = False, verbose: bool = False) -> Path:
+    """The Python module of the block operators, against the installed torch."""
+    import torch
+    home = Path(torch.__file__).resolve().parent
+    newest = max(p.stat().st_mtime for p in (MODULE_SOURCE, HEADER, home / "version.py"))
+    if MODULE.exists() and MODULE.stat().st_mtime >= newest and not force:
+        return MODULE
+    tmp = MODULE.with_suffix(".so.tmp")
+    cuda = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{ROOT / 'include'}",
+           f"-I{home / 'include'}", f"-I{home / 'include' / 'torch' / 'csrc' / 'api' / 'include'}", f"-I{cuda / 'include'}",
+           f"-I{sysconfig.get_paths()['include']}", str(MODULE_SOURCE), "-o", str(tmp), f"-L{HERE}", "-l:libffnerf.so",
+           f"-L{home / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed:\n{' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
+    if verbose:
+        print(res.stderr)
+    tmp.replace(MODULE)
+    return MODULE
 
 
 if __name__ == "__main__":

@@ -1,0 +1,294 @@
+// ffn_ops_torch.cpp -- the block operators of include/ffnerf.h on torch tensors (the module _ffn_ops).
+//
+// Checks a call's tensors, allocates its outputs and workspace through torch's caching allocator on the
+// current stream, and calls the C entry.  It is native because a call on a few rows is bound by the
+// host: through ctypes a one-row norm took 13 us, 4 of them the launch.  The Python functions with the
+// documentation are in ffn_ops.py.  Arguments that an operator cannot take raise ValueError.
+#include <optional>
+#include <string>
+#include <tuple>
+
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include "ffnerf.h"
+
+namespace py = pybind11;
+using at::Tensor;
+using Maybe = std::optional<Tensor>;
+
+namespace {
+
+[[noreturn]] void bad(const std::string& what) { throw py::value_error(what); }
+
+std::string shape_of(const Tensor& t) {
+    std::string s = "(";
+    for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
+    return s + ")";
+}
+std::string kind_of(const Tensor& t) { return std::string(c10::toString(t.scalar_type())) + " " + shape_of(t) + " on " + t.device().str(); }
+
+bool wide(at::ScalarType t) { return t == at::kFloat || t == at::kHalf || t == at::kBFloat16; }
+int code_of(at::ScalarType t) {
+    return t == at::kFloat ? FFN_F32 : t == at::kHalf ? FFN_F16 : t == at::kBFloat16 ? FFN_BF16 : FFN_E4M3;
+}
+
+void done(int rc, const char* what) {
+    if (rc == FFN_OK) return;
+    const std::string msg = std::string(what) + " failed (" + std::to_string(rc) + "): " + ffn_last_error(nullptr);
+    if (rc == FFN_E_CONFIG || rc == FFN_E_CAPACITY) throw py::value_error(msg);
+    throw std::runtime_error(msg);
+}
+
+// The tensor that sets a call's device, type and shape.
+void leads(const Tensor& t, const char* name, int64_t dim) {
+    if (!t.is_cuda()) bad(std::string(name) + " must be a CUDA tensor");
+    if (t.dim() != dim) bad(std::string(name) + " must have " + std::to_string(dim) + " dimensions, got shape " + shape_of(t));
+}
+
+// A matrix [n][d] of contiguous columns on `like`'s device: its row stride in elements.
+int64_t rows_of(const Tensor& t, const char* name, int64_t n, int64_t d, at::ScalarType type, const Tensor& like) {
+    if (t.scalar_type() != type || t.device() != like.device() || t.dim() != 2 || t.size(0) != n || t.size(1) != d)
+        bad(std::string(name) + " must be " + c10::toString(type) + " (" + std::to_string(n) + ", " + std::to_string(d) + ") on " +
+            like.device().str() + ", got " + kind_of(t));
+    if (t.is_contiguous()) return d;
+    if (d > 1 && t.stride(1) != 1) bad(std::string(name) + " must have contiguous columns");
+    if (n <= 1) return d;
+    if (t.stride(0) < d) bad(std::string(name) + " must not overlap itself (row stride " + std::to_string(t.stride(0)) + ")");
+    return t.stride(0);
+}
+
+// A contiguous tensor of exactly this type and shape.
+template <typename T>
+T* plain(const Tensor& t, const char* name, at::IntArrayRef shape, at::ScalarType type, const Tensor& like) {
+    if (t.scalar_type() != type || t.device() != like.device() || t.sizes() != shape || !t.is_contiguous()) {
+        std::string s = "(";
+        for (size_t i = 0; i < shape.size(); ++i) s += (i ? ", " : "") + std::to_string(shape[i]);
+        bad(std::string(name) + " must be a contiguous " + c10::toString(type) + " tensor of shape " + s + ") on " +
+            like.device().str() + ", got " + kind_of(t));
+    }
+    return static_cast<T*>(t.data_ptr());
+}
+template <typename T>
+T* plain(const Maybe& t, const char* name, at::IntArrayRef shape, at::ScalarType type, const Tensor& like) {
+    return t ? plain<T>(*t, name, shape, type, like) : nullptr;
+}
+
+void* ptr(const Maybe& t) { return t ? t->data_ptr() : nullptr; }
+Tensor make(at::IntArrayRef shape, at::ScalarType type, const Tensor& like) { return at::empty(shape, like.options().dtype(type)); }
+
+// The device and stream of a call, and its workspace.
+struct Call {
+    c10::cuda::CUDAGuard guard;
+    void* stream;
+    Tensor buffer;
+    explicit Call(const Tensor& t) : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream(t.device().index()).stream()) {}
+    void* space(uint64_t bytes, const Tensor& like) {
+        if (!bytes) return nullptr;
+        buffer = at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+        return buffer.data_ptr();
+    }
+};
+
+// ------------------------------------------------------------------------------------------- norm
+std::tuple<Tensor, Tensor, Tensor, Maybe> rmsnorm(const Tensor& x, const Tensor& gamma, const Maybe& residual, double eps,
+                                                  bool e4m3, int64_t group) {
+    leads(x, "x", 2);
+    const auto type = x.scalar_type();
+    if (!wide(type)) bad(std::string("x must be float32, float16 or bfloat16, got ") + c10::toString(type));
+    const int64_t n = x.size(0), d = x.size(1);
+    const int64_t x_ld = rows_of(x, "x", n, d, type, x);
+    const int64_t r_ld = residual ? rows_of(*residual, "residual", n, d, type, x) : 0;
+    const float* g = plain<float>(gamma, "gamma", {d}, at::kFloat, x);
+    if (group != 0 && (!e4m3 || (group != 32 && group != 64 && group != 128) || d % group))
+        bad("group must be 0, or 32, 64 or 128 with out='e4m3' and divide the " + std::to_string(d) + " columns, got " +
+            std::to_string(group));
+    if (d < 1 || d > INT32_MAX) bad("x must have between 1 and 2^31 - 1 columns");
+    Call call(x);
+    Tensor y = make({n, d}, e4m3 ? at::kFloat8_e4m3fn : type, x);
+    Tensor h = residual ? make({n, d}, type, x) : x;
+    Tensor rstd = make({n}, at::kFloat, x);
+    Maybe scale;
+    if (e4m3) scale = group ? make({n, d / group}, at::kFloat, x) : make({n}, at::kFloat, x);
+    done(ffn_rmsnorm(x.data_ptr(), x_ld, ptr(residual), r_ld, g, residual ? h.data_ptr() : nullptr, y.data_ptr(),
+                     static_cast<float*>(ptr(scale)), rstd.data_ptr<float>(), n, (int32_t)d, (float)eps, code_of(type),
+                     e4m3 ? FFN_E4M3 : code_of(type), (int32_t)group, call.stream), "ffn_rmsnorm");
+    return {y, h, rstd, scale};
+}
+
+std::tuple<Tensor, Tensor> rmsnorm_bwd(const Tensor& dy, const Tensor& x, const Maybe& residual, const Tensor& gamma,
+                                       const Tensor& rstd, const Maybe& dresidual) {
+    leads(dy, "dy", 2);
+    const auto type = dy.scalar_type();
+    if (!wide(type)) bad(std::string("dy must be float32, float16 or bfloat16, got ") + c10::toString(type));
+    const int64_t n = dy.size(0), d = dy.size(1);
+    if (d < 1 || d > INT32_MAX) bad("dy must have between 1 and 2^31 - 1 columns");
+    const int64_t dy_ld = rows_of(dy, "dy", n, d, type, dy), x_ld = rows_of(x, "x", n, d, type, dy);
+    const int64_t r_ld = residual ? rows_of(*residual, "residual", n, d, type, dy) : 0;
+    const int64_t dr_ld = dresidual ? rows_of(*dresidual, "dresidual", n, d, type, dy) : 0;
+    const float* g = plain<float>(gamma, "gamma", {d}, at::kFloat, dy);
+    const float* s = plain<float>(rstd, "rstd", {n}, at::kFloat, dy);
+    Call call(dy);
+    Tensor dx = make({n, d}, type, dy), dgamma = make({d}, at::kFloat, dy);
+    const uint64_t bytes = ffn_rmsnorm_bwd_workspace(n, (int32_t)d);
+    void* ws = call.space(bytes, dy);
+    done(ffn_rmsnorm_bwd(dy.data_ptr(), dy_ld, x.data_ptr(), x_ld, ptr(residual), r_ld, g, s, ptr(dresidual), dr_ld,
+                         dx.data_ptr(), dgamma.data_ptr<float>(), ws, bytes, n, (int32_t)d, code_of(type), call.stream),
+         "ffn_rmsnorm_bwd");
+    return {dx, dgamma};
+}
+
+// ------------------------------------------------------------------------------------------- scan
+struct Sequences {
+    int64_t seqs, rows, longest, d;
+    const int32_t* offsets;
+    const float* h0;
+    Sequences(const Tensor& gate, const Maybe& h0_, const Maybe& off, int64_t max_len) {
+        if (!wide(gate.scalar_type())) bad(std::string("gate must be float32, float16 or bfloat16, got ") + c10::toString(gate.scalar_type()));
+        if (!off) {
+            leads(gate, "gate (without offsets)", 3);
+            seqs = gate.size(0); longest = gate.size(1); d = gate.size(2);
+            rows = seqs * longest;
+            offsets = nullptr;
+        } else {
+            leads(gate, "gate (with offsets)", 2);
+            if (off->dim() != 1 || off->numel() < 1) bad("offsets must be a vector [sequences + 1]");
+            offsets = plain<int32_t>(*off, "offsets", {off->numel()}, at::kInt, gate);
+            seqs = off->numel() - 1; rows = gate.size(0); d = gate.size(1);
+            longest = max_len < 0 ? rows : max_len;
+        }
+        if (seqs > INT32_MAX || d < 1 || d > INT32_MAX) bad("gate: the sequences and the channels must be below 2^31, one channel at least");
+        h0 = plain<float>(h0_, "h0", {seqs, d}, at::kFloat, gate);
+    }
+};
+
+// Row stride of a tensor of gate's shape, [rows][d] or [sequences][steps][d].
+int64_t packed(const Tensor& t, const char* name, const Tensor& gate) {
+    if (t.sizes() != gate.sizes() || t.scalar_type() != gate.scalar_type() || t.device() != gate.device())
+        bad(std::string(name) + " must be like gate, " + kind_of(gate) + ", got " + kind_of(t));
+    const int64_t last = t.dim() - 1, d = t.size(last);
+    if (t.is_contiguous()) return d;
+    if (d > 1 && t.stride(last) != 1) bad(std::string(name) + " must have contiguous channels");
+    int64_t rows = t.size(0), ld = t.stride(0);
+    if (t.dim() == 3) {
+        const int64_t b = t.size(0), s = t.size(1);
+        if (s > 1) {
+            if (b > 1 && t.stride(0) != s * t.stride(1)) bad(std::string(name) + ": the sequences must follow one another at a constant row stride");
+            ld = t.stride(1);
+        }
+        rows = b * s;
+    }
+    if (rows <= 1) return d;
+    if (ld < d) bad(std::string(name) + " must not overlap itself (row stride " + std::to_string(ld) + ")");
+    return ld;
+}
+
+std::tuple<Tensor, Tensor> gated_scan(const Tensor& gate, const Tensor& value, const Maybe& h0, const Maybe& offsets,
+                                      int64_t max_len, int form, bool reverse) {
+    const Sequences q(gate, h0, offsets, max_len);
+    const int64_t g_ld = packed(gate, "gate", gate), v_ld = packed(value, "value", gate);
+    Call call(gate);
+    Tensor h = make(gate.sizes(), gate.scalar_type(), gate), last = make({q.seqs, q.d}, at::kFloat, gate);
+    if (q.seqs == 0) return {h.zero_(), last};
+    const uint64_t bytes = ffn_gated_scan_workspace((int32_t)q.seqs, q.longest, (int32_t)q.d);
+    void* ws = call.space(bytes, gate);
+    done(ffn_gated_scan(gate.data_ptr(), g_ld, value.data_ptr(), v_ld, q.h0, q.offsets, h.data_ptr(), last.data_ptr<float>(),
+                        q.rows, (int32_t)q.seqs, q.longest, (int32_t)q.d, code_of(gate.scalar_type()), form, reverse ? 1 : 0, ws,
+                        bytes, call.stream), "ffn_gated_scan");
+    return {h, last};
+}
+
+std::tuple<Tensor, Tensor, Tensor> gated_scan_bwd(const Tensor& dh, const Tensor& gate, const Tensor& value, const Tensor& h,
+                                                  const Maybe& h0, const Maybe& dh_last, const Maybe& offsets, int64_t max_len,
+                                                  int form, bool reverse) {
+    const Sequences q(gate, h0, offsets, max_len);
+    const int64_t g_ld = packed(gate, "gate", gate), v_ld = packed(value, "value", gate), d_ld = packed(dh, "dh", gate),
+                  h_ld = packed(h, "h", gate);
+    const float* dl = plain<float>(dh_last, "dh_last", {q.seqs, q.d}, at::kFloat, gate);
+    Call call(gate);
+    Tensor dgate = make(gate.sizes(), gate.scalar_type(), gate), dvalue = make(gate.sizes(), gate.scalar_type(), gate);
+    Tensor dh0 = make({q.seqs, q.d}, at::kFloat, gate);
+    if (q.seqs == 0) return {dgate.zero_(), dvalue.zero_(), dh0};
+    const uint64_t bytes = ffn_gated_scan_workspace((int32_t)q.seqs, q.longest, (int32_t)q.d);
+    void* ws = call.space(bytes, gate);
+    done(ffn_gated_scan_bwd(dh.data_ptr(), d_ld, dl, gate.data_ptr(), g_ld, value.data_ptr(), v_ld, h.data_ptr(), h_ld, q.h0,
+                            q.offsets, dgate.data_ptr(), dvalue.data_ptr(), dh0.data_ptr<float>(), q.rows, (int32_t)q.seqs,
+                            q.longest, (int32_t)q.d, code_of(gate.scalar_type()), form, reverse ? 1 : 0, ws, bytes, call.stream),
+         "ffn_gated_scan_bwd");
+    return {dgate, dvalue, dh0};
+}
+
+// ---------------------------------------------------------------------------------------- experts
+struct Experts {
+    int64_t n, e, m, k, x_ld;
+    const int32_t* offsets;
+    int code;
+    Experts(const Tensor& x, const Tensor& w, const Tensor& off) {
+        leads(x, "x", 2);
+        if (w.dim() != 3 || !w.is_contiguous()) bad("w must be a contiguous tensor [experts, out, in], got " + kind_of(w));
+        n = x.size(0); e = w.size(0); m = w.size(1); k = w.size(2);
+        if (e < 1 || e > FFN_MAX_EXPERTS || m < 1 || k < 1 || m > INT32_MAX || k > INT32_MAX)
+            bad("w must have 1 to " + std::to_string(FFN_MAX_EXPERTS) + " experts and at least one output and input, got shape " + shape_of(w));
+        if (w.scalar_type() != x.scalar_type() || w.device() != x.device()) bad("w is " + kind_of(w) + ", x is " + kind_of(x));
+        x_ld = rows_of(x, "x", n, k, x.scalar_type(), x);
+        offsets = plain<int32_t>(off, "offsets", {e + 1}, at::kInt, x);
+        code = code_of(x.scalar_type());
+    }
+};
+
+Tensor expert_mm(const Tensor& x, const Tensor& w, const Tensor& offsets, const Maybe& x_scale, const Maybe& w_scale,
+                 std::optional<at::ScalarType> out) {
+    const auto type = x.scalar_type();
+    const bool e4m3 = type == at::kFloat8_e4m3fn;
+    if (!e4m3 && type != at::kHalf && type != at::kBFloat16)
+        bad(std::string("x must be float16, bfloat16 or float8_e4m3fn, got ") + c10::toString(type));
+    const Experts q(x, w, offsets);
+    if (e4m3 != x_scale.has_value() || e4m3 != w_scale.has_value())
+        bad("float8_e4m3fn operands need x_scale [n] and w_scale [experts, out], others take none");
+    const float* xs = plain<float>(x_scale, "x_scale", {q.n}, at::kFloat, x);
+    const float* ws_ = plain<float>(w_scale, "w_scale", {q.e, q.m}, at::kFloat, x);
+    const auto to = out ? *out : e4m3 ? at::kBFloat16 : type;
+    if (e4m3 ? (to != at::kHalf && to != at::kBFloat16) : to != type)
+        bad(std::string("out_dtype ") + c10::toString(to) + " does not go with " + c10::toString(type) + " operands");
+    Call call(x);
+    Tensor y = make({q.n, q.m}, to, x);
+    const uint64_t bytes = ffn_expert_mm_workspace(x.data_ptr(), q.x_ld, w.data_ptr(), q.n, (int32_t)q.e, (int32_t)q.k, (int32_t)q.m, q.code);
+    void* ws = call.space(bytes, x);
+    done(ffn_expert_mm(x.data_ptr(), q.x_ld, w.data_ptr(), q.offsets, xs, ws_, y.data_ptr(), q.n, (int32_t)q.e, (int32_t)q.k,
+                       (int32_t)q.m, q.code, code_of(to), ws, bytes, call.stream), "ffn_expert_mm");
+    return y;
+}
+
+std::tuple<Maybe, Maybe> expert_mm_bwd(const Tensor& dy, const Tensor& x, const Tensor& w, const Tensor& offsets, bool need_dx,
+                                       bool need_dw, std::optional<at::ScalarType> dw_type) {
+    const auto type = x.scalar_type();
+    if (type != at::kHalf && type != at::kBFloat16) bad(std::string("x must be float16 or bfloat16, got ") + c10::toString(type));
+    const Experts q(x, w, offsets);
+    const int64_t dy_ld = rows_of(dy, "dy", q.n, q.m, type, x);
+    const auto to = dw_type ? *dw_type : type;
+    if (to != type && to != at::kFloat) bad(std::string("dw_dtype must be ") + c10::toString(type) + " or Float, got " + c10::toString(to));
+    Call call(x);
+    Maybe dx, dw;
+    if (need_dx) dx = make({q.n, q.k}, type, x);
+    if (need_dw) dw = make({q.e, q.m, q.k}, to, x);
+    const uint64_t bytes = ffn_expert_mm_bwd_workspace(dy.data_ptr(), dy_ld, x.data_ptr(), q.x_ld, w.data_ptr(), q.n, (int32_t)q.e,
+                                                       (int32_t)q.k, (int32_t)q.m, q.code);
+    void* ws = call.space(bytes, x);
+    done(ffn_expert_mm_bwd(dy.data_ptr(), dy_ld, x.data_ptr(), q.x_ld, w.data_ptr(), q.offsets, ptr(dx), ptr(dw), q.n, (int32_t)q.e,
+                           (int32_t)q.k, (int32_t)q.m, q.code, code_of(to), ws, bytes, call.stream), "ffn_expert_mm_bwd");
+    return {dx, dw};
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_ffn_ops, m) {
+    m.attr("abi_version") = FFN_ABI_VERSION;
+    m.def("rmsnorm", &rmsnorm);
+    m.def("rmsnorm_bwd", &rmsnorm_bwd);
+    m.def("gated_scan", &gated_scan);
+    m.def("gated_scan_bwd", &gated_scan_bwd);
+    m.def("expert_mm", &expert_mm);
+    m.def("expert_mm_bwd", &expert_mm_bwd);
+}

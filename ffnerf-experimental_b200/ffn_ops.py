@@ -18,77 +18,24 @@ import torch
 
 import ffn_native as fn
 
-F32, F16, BF16, E4M3 = range(4)                       # include/ffnerf.h FFN_F32 ...
-SCAN_FORMS = {"linear": 0, "sigmoid": 1}
-DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3}
-_WIDE = (torch.float32, torch.float16, torch.bfloat16)
+SCAN_FORMS = {"linear": 0, "sigmoid": 1}              # include/ffnerf.h FFN_SCAN_LINEAR, FFN_SCAN_SIGMOID
 
-# What torch.cuda.current_stream().cuda_stream and torch.cuda.current_device() return, without building a
-# Stream object: a call on a single row is bound by the host, about 10 us of it.
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_device_now = torch._C._cuda_getDevice
+_native = None
 
 
-def _bad(what: str):
-    raise ValueError(what)
-
-
-def _rows(t, name: str, d: int, n: int, dtype, device) -> int:
-    """Checks a matrix [n, d] of contiguous columns and returns its row stride in elements."""
-    if t.dtype is not dtype:
-        _bad(f"{name} is {t.dtype}, expected {dtype}")
-    if t.device != device:
-        _bad(f"{name} is on {t.device}, expected {device}")
-    if t.shape != (n, d):
-        _bad(f"{name} has shape {tuple(t.shape)}, expected {(n, d)}")
-    if t.is_contiguous():
-        return d
-    ld, sc = t.stride()
-    if d > 1 and sc != 1:
-        _bad(f"{name} must have contiguous columns")
-    if n <= 1:
-        return d
-    if ld < d:
-        _bad(f"{name} must not overlap itself (row stride {ld} below {d} columns)")
-    return ld
-
-
-def _matrix(t, name: str):
-    """(rows, columns, device) of the CUDA matrix that sets a call's shape."""
-    if not t.is_cuda:
-        _bad(f"{name} must be a CUDA tensor")
-    if t.dim() != 2:
-        _bad(f"{name} must be a matrix [rows, columns], got shape {tuple(t.shape)}")
-    return *t.shape, t.device
-
-
-def _like(t):
-    """An uninitialised contiguous tensor of t's shape and type."""
-    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
-
-
-def _plain(t, name: str, shape: tuple, dtype, device):
-    """Checks a contiguous tensor of exactly this shape and type; None passes."""
-    if t is None:
-        return None
-    if t.shape != shape or t.dtype is not dtype or t.device != device or not t.is_contiguous():
-        _bad(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {device}, got {t.dtype} "
-             f"{tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
-
-
-def _call(name: str, device, *args):
-    """One native call on `device` and its current stream."""
-    f = getattr(fn._lib or fn.load_library(), name)
-    i = device.index
-    if _device_now() == i:
-        rc = f(*args, _raw_stream(i))
-    else:
-        with torch.cuda.device(device):
-            rc = f(*args, _raw_stream(i))
-    if rc != fn.FFN_OK:
-        msg = fn.load_library().ffn_last_error(None).decode()
-        raise (ValueError if rc in (fn.FFN_E_CONFIG, fn.FFN_E_CAPACITY) else RuntimeError)(f"{name} failed ({rc}): {msg}")
+def _load():
+    """The module _ffn_ops (csrc/ffn_ops_torch.cpp), which checks tensors and calls libffnerf.so."""
+    global _native
+    fn.load_library()                                  # the missing or mismatched library is reported there
+    try:
+        import _ffn_ops
+    except ImportError as e:
+        raise RuntimeError("the module _ffn_ops must be built (python build_native.py); there is no fallback") from e
+    if _ffn_ops.abi_version != fn.ABI_VERSION:
+        raise RuntimeError(f"_ffn_ops was built for ABI version {_ffn_ops.abi_version}, this module expects "
+                           f"{fn.ABI_VERSION}: rebuild it (python build_native.py)")
+    _native = _ffn_ops
+    return _native
 
 
 def _on(stream, f, *args):
@@ -100,18 +47,16 @@ def _on(stream, f, *args):
         return f(*args)
 
 
-def _workspace(device, name: str, *args):
-    """(tensor or None, pointer, bytes) of the workspace that the library asks for."""
-    f = getattr(fn._lib or fn.load_library(), name)
-    if _device_now() == device.index:
-        need = f(*args)
-    else:
-        with torch.cuda.device(device):
-            need = f(*args)
-    if not need:
-        return None, None, 0
-    t = torch.empty(need, dtype=torch.uint8, device=device)
-    return t, t.data_ptr(), need
+def _form(form: str) -> int:
+    if form not in SCAN_FORMS:
+        raise ValueError(f"form must be one of {sorted(SCAN_FORMS)}, got {form!r}")
+    return SCAN_FORMS[form]
+
+
+def _longest(max_len) -> int:
+    if max_len is not None and max_len < 0:
+        raise ValueError(f"max_len must not be negative, got {max_len}")
+    return -1 if max_len is None else int(max_len)
 
 
 # ---------------------------------------------------------------------------------------- RMS norm
@@ -132,34 +77,9 @@ def rmsnorm(x, gamma, residual=None, eps: float = 1e-6, out: str = "same", group
     ``rmsnorm_bwd`` takes."""
     if stream is not None:
         return _on(stream, rmsnorm, x, gamma, residual, eps, out, group)
-    dt = x.dtype
-    if dt not in _WIDE:
-        _bad(f"x must be float32, float16 or bfloat16, got {dt}")
-    n, d, dev = _matrix(x, "x")
-    x_ld = _rows(x, "x", d, n, dt, dev)
-    code = DTYPES[dt]
-    g = _plain(gamma, "gamma", (d,), torch.float32, dev)
-    if out == "same":
-        if group:
-            _bad("group needs out='e4m3'")
-        y, scale, sp, out_code = _like(x), None, None, code
-    elif out == "e4m3":
-        if group not in (0, 32, 64, 128) or (group and d % group):
-            _bad(f"group must be 0, 32, 64 or 128 and divide the {d} columns, got {group}")
-        y, out_code = torch.empty((n, d), dtype=torch.float8_e4m3fn, device=dev), E4M3
-        scale = gamma.new_empty((n, d // group) if group else (n,))
-        sp = scale.data_ptr()
-    else:
-        _bad(f"out must be 'same' or 'e4m3', got {out!r}")
-    rstd = gamma.new_empty((n,))
-    if residual is None:
-        h, hp, rp, res_ld = x, None, None, 0
-    else:
-        res_ld = _rows(residual, "residual", d, n, dt, dev)
-        h = _like(x)
-        hp, rp = h.data_ptr(), residual.data_ptr()
-    _call("ffn_rmsnorm", dev, x.data_ptr(), x_ld, rp, res_ld, g, hp, y.data_ptr(), sp, rstd.data_ptr(), n, d, eps, code,
-          out_code, group)
+    if out not in ("same", "e4m3"):
+        raise ValueError(f"out must be 'same' or 'e4m3', got {out!r}")
+    y, h, rstd, scale = (_native or _load()).rmsnorm(x, gamma, residual, eps, out == "e4m3", group)
     return y, h, NormState(rstd, x, residual), scale
 
 
@@ -173,66 +93,11 @@ def rmsnorm_bwd(dy, h, gamma, state, dresidual=None, stream=None):
     residual need not be kept."""
     if stream is not None:
         return _on(stream, rmsnorm_bwd, dy, h, gamma, state, dresidual)
-    dt = dy.dtype
-    if dt not in _WIDE:
-        _bad(f"dy must be float32, float16 or bfloat16, got {dt}")
-    n, d, dev = _matrix(dy, "dy")
-    dy_ld = _rows(dy, "dy", d, n, dt, dev)
     rstd, x, residual = state if isinstance(state, NormState) else (state, h, None)
-    x_ld = _rows(x, "x", d, n, dt, dev)
-    res_ld = 0 if residual is None else _rows(residual, "residual", d, n, dt, dev)
-    dr_ld = 0 if dresidual is None else _rows(dresidual, "dresidual", d, n, dt, dev)
-    g, r = _plain(gamma, "gamma", (d,), torch.float32, dev), _plain(rstd, "rstd", (n,), torch.float32, dev)
-    dx, dgamma = _like(dy), _like(gamma)
-    ws, p, size = _workspace(dev, "ffn_rmsnorm_bwd_workspace", n, d)
-    _call("ffn_rmsnorm_bwd", dev, dy.data_ptr(), dy_ld, x.data_ptr(), x_ld,
-          None if residual is None else residual.data_ptr(), res_ld, g, r,
-          None if dresidual is None else dresidual.data_ptr(), dr_ld, dx.data_ptr(), dgamma.data_ptr(), p, size, n, d,
-          DTYPES[dt])
-    return dx, dgamma
+    return (_native or _load()).rmsnorm_bwd(dy, x, residual, gamma, rstd, dresidual)
 
 
 # -------------------------------------------------------------------------- gated linear recurrence
-def _scan_layout(gate, value, offsets, max_len, form, h0):
-    """The packed [rows, d] view of a scan's arguments and its sequences."""
-    if form not in SCAN_FORMS:
-        _bad(f"form must be one of {sorted(SCAN_FORMS)}, got {form!r}")
-    if gate.dtype not in _WIDE:
-        _bad(f"gate must be float32, float16 or bfloat16, got {gate.dtype}")
-    dev = gate.device
-    if offsets is None:
-        if gate.dim() != 3:
-            _bad("without offsets gate must be [sequences, steps, channels]")
-        seqs, max_len, d = gate.shape
-        off = None
-    else:
-        if offsets.dim() != 1 or offsets.dtype is not torch.int32 or offsets.device != dev or offsets.numel() < 1 \
-                or not offsets.is_contiguous():
-            _bad(f"offsets must be a contiguous int32 vector [sequences + 1] on {dev}")
-        if gate.dim() != 2:
-            _bad("with offsets gate must be [rows, channels]")
-        seqs, d = offsets.numel() - 1, gate.shape[1]
-        max_len = gate.shape[0] if max_len is None else int(max_len)
-        off = offsets.data_ptr()
-    return seqs, max_len, d, off, _plain(h0, "h0", (seqs, d), torch.float32, dev)
-
-
-def _packed(t, name: str, like, d: int):
-    """(pointer, row stride) of a [rows, d] or [sequences, steps, d] tensor."""
-    if t.shape != like.shape:
-        _bad(f"{name} has shape {tuple(t.shape)}, expected {tuple(like.shape)}")
-    if t.dtype is not like.dtype or t.device != like.device or not t.is_cuda:
-        _bad(f"{name} must be a {like.dtype} CUDA tensor on {like.device}, got {t.dtype} on {t.device}")
-    if t.is_contiguous():
-        return t.data_ptr(), d
-    if t.dim() == 3:
-        b, s, _ = t.shape
-        if s > 1 and b > 1 and t.stride(0) != s * t.stride(1):
-            _bad(f"{name}: the sequences must follow one another at a constant row stride")
-        t = t.as_strided((b * s, d), (t.stride(1) if s > 1 else t.stride(0), t.stride(2)))
-    return t.data_ptr(), _rows(t, name, d, t.shape[0], like.dtype, like.device)
-
-
 def gated_scan(gate, value, h0=None, offsets=None, max_len: int | None = None, form: str = "sigmoid",
                reverse: bool = False, stream=None):
     """The recurrence ``h_t = a_t h_{t-1} + b_t`` per channel: returns ``(h, h_last)``.
@@ -246,18 +111,7 @@ def gated_scan(gate, value, h0=None, offsets=None, max_len: int | None = None, f
     runs every sequence from its last step to its first (back-to-front compositing)."""
     if stream is not None:
         return _on(stream, gated_scan, gate, value, h0, offsets, max_len, form, reverse)
-    seqs, max_len, d, off, p0 = _scan_layout(gate, value, offsets, max_len, form, h0)
-    gp, g_ld = _packed(gate, "gate", gate, d)
-    vp, v_ld = _packed(value, "value", gate, d)
-    h = _like(gate)
-    last = torch.empty((seqs, d), dtype=torch.float32, device=gate.device) if h0 is None else torch.empty_like(h0)
-    rows = seqs * max_len if off is None else gate.shape[0]
-    if seqs == 0:
-        return h.zero_(), last
-    buf, p, size = _workspace(gate.device, "ffn_gated_scan_workspace", seqs, max_len, d)
-    _call("ffn_gated_scan", gate.device, gp, g_ld, vp, v_ld, p0, off, h.data_ptr(), last.data_ptr(), rows, seqs,
-          max_len, d, DTYPES[gate.dtype], SCAN_FORMS[form], 1 if reverse else 0, p, size)
-    return h, last
+    return (_native or _load()).gated_scan(gate, value, h0, offsets, _longest(max_len), _form(form), reverse)
 
 
 def gated_scan_bwd(dh, gate, value, h, h0=None, dh_last=None, offsets=None, max_len: int | None = None,
@@ -266,38 +120,11 @@ def gated_scan_bwd(dh, gate, value, h, h0=None, dh_last=None, offsets=None, max_
     dh_last [sequences, channels] float32 is the gradient of h_last (None: zero); dh0 is float32."""
     if stream is not None:
         return _on(stream, gated_scan_bwd, dh, gate, value, h, h0, dh_last, offsets, max_len, form, reverse)
-    seqs, max_len, d, off, p0 = _scan_layout(gate, value, offsets, max_len, form, h0)
-    dev = gate.device
-    gp, g_ld = _packed(gate, "gate", gate, d)
-    vp, v_ld = _packed(value, "value", gate, d)
-    dp, d_ld = _packed(dh, "dh", gate, d)
-    hp, h_ld = _packed(h, "h", gate, d)
-    pl = _plain(dh_last, "dh_last", (seqs, d), torch.float32, dev)
-    dgate, dvalue = _like(gate), _like(gate)
-    dh0 = torch.empty((seqs, d), dtype=torch.float32, device=dev)
-    rows = seqs * max_len if off is None else gate.shape[0]
-    if seqs == 0:
-        return dgate.zero_(), dvalue.zero_(), dh0
-    buf, p, size = _workspace(dev, "ffn_gated_scan_workspace", seqs, max_len, d)
-    _call("ffn_gated_scan_bwd", dev, dp, d_ld, pl, gp, g_ld, vp, v_ld, hp, h_ld, p0, off, dgate.data_ptr(),
-          dvalue.data_ptr(), dh0.data_ptr(), rows, seqs, max_len, d, DTYPES[gate.dtype], SCAN_FORMS[form],
-          1 if reverse else 0, p, size)
-    return dgate, dvalue, dh0
+    return (_native or _load()).gated_scan_bwd(dh, gate, value, h, h0, dh_last, offsets, _longest(max_len), _form(form),
+                                               reverse)
 
 
 # ------------------------------------------------------------------- matrix products by expert
-def _experts(x, w, offsets):
-    if w.dim() != 3 or not w.is_contiguous():
-        _bad(f"w must be a contiguous tensor [experts, out, in], got shape {tuple(w.shape)}")
-    e, m, k = w.shape
-    if e < 1 or m < 1 or k < 1:
-        _bad(f"w must have at least one expert, output and input, got shape {tuple(w.shape)}")
-    dev = x.device
-    if w.dtype is not x.dtype or w.device != dev:
-        _bad(f"w is {w.dtype} on {w.device}, expected {x.dtype} on {dev}")
-    return e, m, k, _plain(offsets, "offsets", (e + 1,), torch.int32, dev)
-
-
 def expert_mm(x, w, offsets, x_scale=None, w_scale=None, out_dtype=None, stream=None):
     """``y[r] = x[r] w[e]^T`` for the rows r of expert e: returns y [n, out].
 
@@ -308,36 +135,7 @@ def expert_mm(x, w, offsets, x_scale=None, w_scale=None, out_dtype=None, stream=
     (y bfloat16, or float16 by ``out_dtype``).  Sums are float32."""
     if stream is not None:
         return _on(stream, expert_mm, x, w, offsets, x_scale, w_scale, out_dtype)
-    n, _, dev = _matrix(x, "x")
-    e, m, k, off = _experts(x, w, offsets)
-    x_ld = _rows(x, "x", k, n, x.dtype, dev)
-    xs = ws_ = None
-    if x.dtype is torch.float8_e4m3fn:
-        out_dtype = out_dtype or torch.bfloat16
-        if x_scale is None or w_scale is None:
-            _bad("float8_e4m3fn rows need x_scale [n] and w_scale [experts, out]")
-        xs = _plain(x_scale, "x_scale", (n,), torch.float32, dev)
-        ws_ = _plain(w_scale, "w_scale", (e, m), torch.float32, dev)
-        if out_dtype not in (torch.float16, torch.bfloat16):
-            _bad(f"out_dtype must be float16 or bfloat16, got {out_dtype}")
-    elif x.dtype in (torch.float16, torch.bfloat16):
-        if x_scale is not None or w_scale is not None:
-            _bad("scales belong to float8_e4m3fn operands")
-        if out_dtype not in (None, x.dtype):
-            _bad(f"out_dtype must be {x.dtype} for {x.dtype} operands")
-        out_dtype = x.dtype
-    else:
-        _bad(f"x must be float16, bfloat16 or float8_e4m3fn, got {x.dtype}")
-    y = torch.empty((n, m), dtype=out_dtype, device=dev)
-    code = DTYPES[x.dtype]
-    xp, wp, unit = x.data_ptr(), w.data_ptr(), 16 if code == E4M3 else 8
-    buf = p = None
-    size = 0
-    if (xp | wp) & 15 or x_ld % unit or k % unit:             # rows that TMA cannot read are copied
-        buf, p, size = _workspace(dev, "ffn_expert_mm_workspace", xp, x_ld, wp, n, e, k, m, code)
-    _call("ffn_expert_mm", dev, xp, x_ld, wp, off, xs, ws_, y.data_ptr(), n, e, k, m, code,
-          DTYPES[out_dtype], p, size)
-    return y
+    return (_native or _load()).expert_mm(x, w, offsets, x_scale, w_scale, out_dtype)
 
 
 def expert_mm_bwd(dy, x, w, offsets, need_dx: bool = True, need_dw: bool = True, dw_dtype=None, stream=None):
@@ -346,24 +144,7 @@ def expert_mm_bwd(dy, x, w, offsets, need_dx: bool = True, need_dw: bool = True,
     float32 (what ``ffn_native.adam`` takes).  An expert without rows gets a zero gradient."""
     if stream is not None:
         return _on(stream, expert_mm_bwd, dy, x, w, offsets, need_dx, need_dw, dw_dtype)
-    if x.dtype not in (torch.float16, torch.bfloat16):
-        _bad(f"x must be float16 or bfloat16, got {x.dtype}")
-    n, _, dev = _matrix(x, "x")
-    e, m, k, off = _experts(x, w, offsets)
-    x_ld = _rows(x, "x", k, n, x.dtype, dev)
-    dy_ld = _rows(dy, "dy", m, n, x.dtype, dev)
-    dw_dtype = dw_dtype or x.dtype
-    if dw_dtype not in (x.dtype, torch.float32):
-        _bad(f"dw_dtype must be {x.dtype} or float32, got {dw_dtype}")
-    dx = torch.empty((n, k), dtype=x.dtype, device=dev) if need_dx else None
-    dw = torch.empty((e, m, k), dtype=dw_dtype, device=dev) if need_dw else None
-    code = DTYPES[x.dtype]
-    buf, p, size = _workspace(dev, "ffn_expert_mm_bwd_workspace", dy.data_ptr(), dy_ld, x.data_ptr(), x_ld, w.data_ptr(),
-                              n, e, k, m, code)
-    _call("ffn_expert_mm_bwd", dev, dy.data_ptr(), dy_ld, x.data_ptr(), x_ld, w.data_ptr(), off,
-          None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(), n, e, k, m, code,
-          DTYPES[dw_dtype], p, size)
-    return dx, dw
+    return (_native or _load()).expert_mm_bwd(dy, x, w, offsets, need_dx, need_dw, dw_dtype)
 
 
 def status(device=None) -> int:
