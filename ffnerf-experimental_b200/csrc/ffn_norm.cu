@@ -51,14 +51,16 @@ __device__ __forceinline__ void load_gamma(const float* g, int c, float (&w)[VEC
     }
 }
 
-// Sum (or NaN-keeping maximum) over the threads of one row: `tpr` lanes, or the block (BLOCK).  In a
+// Sum (or largest magnitude, its sign meaningless) over the threads of one row: `tpr` lanes, or the block (BLOCK).  In a
 // block the warps' values are added in warp order, so a row's result does not depend on timing.
 template <bool BLOCK, bool MAX>
 __device__ __forceinline__ float row_reduce(float v, int tpr, float (&sh)[2][32], int& turn) {
-    for (int o = (BLOCK ? 32 : tpr) >> 1; o > 0; o >>= 1) {
-        const float w = __shfl_xor_sync(0xffffffffu, v, o);
-        v = MAX ? max_nan(v, w) : v + w;
-    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+        if (BLOCK || o < tpr) {
+            const float w = __shfl_xor_sync(0xffffffffu, v, o);
+            v = MAX ? max_abs(v, w) : v + w;
+        }
     if constexpr (BLOCK) {
         // one barrier: the buffer of the reduction before last has been read by all who passed the last one
         const int warps = blockDim.x >> 5;
@@ -67,7 +69,7 @@ __device__ __forceinline__ float row_reduce(float v, int tpr, float (&sh)[2][32]
         if ((threadIdx.x & 31) == 0) q[threadIdx.x >> 5] = v;
         __syncthreads();
         v = q[0];
-        for (int w = 1; w < warps; ++w) v = MAX ? max_nan(v, q[w]) : v + q[w];
+        for (int w = 1; w < warps; ++w) v = MAX ? max_abs(v, q[w]) : v + q[w];
     }
     return v;
 }
@@ -95,7 +97,7 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 256, BLOCK ? 2 : 4) rmsnorm_kern
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 p[r][i].clear();
-                q[r][i].clear();
+                if (res) q[r][i].clear();
                 if (row < a.n && (lane + i * tpr) * VEC < a.d) {
                     p[r][i].load(px + i * tpr * VEC);
                     if (res) q[r][i].load(pr + i * tpr * VEC);
@@ -110,14 +112,15 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 256, BLOCK ? 2 : 4) rmsnorm_kern
             float ss = 0.0f;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                float w[VEC];
                 p[r][i].get(v[i]);
-                q[r][i].get(w);
+                if (res) {
+                    float w[VEC];
+                    q[r][i].get(w);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    v[i][j] += w[j];                             // zeros where there is no residual
-                    ss = fmaf(v[i][j], v[i][j], ss);
+                    for (int j = 0; j < VEC; ++j) v[i][j] += w[j];
                 }
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) ss = fmaf(v[i][j], v[i][j], ss);
             }
             ss = row_reduce<BLOCK, false>(ss, tpr, sh, turn);
             const float s = rsqrtf(fmaf(ss, inv_d, a.eps));
@@ -134,12 +137,15 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 256, BLOCK ? 2 : 4) rmsnorm_kern
                     }
                     float g[VEC];
                     load_gamma<VEC>(a.gamma, c, g);
+                    if constexpr (OUT8) {                        // without the row's factor, which the scale takes up
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        v[i][j] = v[i][j] * s * g[j];
-                        if constexpr (OUT8) top = max_nan(top, fabsf(v[i][j]));
-                    }
-                    if constexpr (!OUT8) {
+                        for (int j = 0; j < VEC; ++j) v[i][j] *= g[j];
+                        if (!a.group)
+#pragma unroll
+                            for (int j = 0; j < VEC; ++j) top = max_abs(top, v[i][j]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) v[i][j] *= s * g[j];
                         Vec<T, VEC> o;
                         o.put(v[i]);
                         o.store(static_cast<T*>(a.y) + row * a.d + c);
@@ -150,8 +156,8 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 256, BLOCK ? 2 : 4) rmsnorm_kern
                 float sc = 1.0f, inv = 1.0f;
                 if (!a.group) {
                     top = row_reduce<BLOCK, true>(top, tpr, sh, turn);
-                    sc = e4m3_scale(top);
-                    inv = e4m3_inverse(sc);
+                    sc = e4m3_scale(fabsf(top) * s);
+                    inv = s * e4m3_inverse(sc);
                     if (live && lane == 0) a.scale[row] = sc;
                 }
 #pragma unroll
@@ -161,10 +167,12 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 256, BLOCK ? 2 : 4) rmsnorm_kern
                     if (a.group) {   // group / VEC neighbouring lanes hold one group's columns
                         float m = 0.0f;
 #pragma unroll
-                        for (int j = 0; j < VEC; ++j) m = max_nan(m, on ? fabsf(v[i][j]) : 0.0f);
-                        for (int o = (a.group / VEC) >> 1; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-                        sc = e4m3_scale(m);
-                        inv = e4m3_inverse(sc);
+                        for (int j = 0; j < VEC; ++j) m = max_abs(m, v[i][j]);   // zeros past the row's end
+#pragma unroll
+                        for (int o = 1; o < 32; o <<= 1)
+                            if (o * VEC < a.group) m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, o));
+                        sc = e4m3_scale(fabsf(m) * s);
+                        inv = s * e4m3_inverse(sc);
                         if (on && (c & (a.group - 1)) == 0) a.scale[row * (a.d >> a.group_log2) + (c >> a.group_log2)] = sc;
                     }
                     if (on) {
@@ -217,9 +225,9 @@ __global__ void __launch_bounds__(256) rmsnorm_long_kernel(const NormArgs a) {
             for (int g = a.group ? (int)threadIdx.x >> 5 : 0; g < a.d / width; g += a.group ? (int)blockDim.x >> 5 : 1) {
                 float top = 0.0f;
                 for (int c = g * width + lane; c < (g + 1) * width; c += step)
-                    top = max_nan(top, fabsf(at(c) * s * a.gamma[c]));
+                    top = max_abs(top, at(c) * s * a.gamma[c]);
                 top = a.group ? row_reduce<false, true>(top, 32, sh, turn) : row_reduce<true, true>(top, 0, sh, turn);
-                const float sc = e4m3_scale(top), inv = e4m3_inverse(sc);
+                const float sc = e4m3_scale(fabsf(top)), inv = e4m3_inverse(sc);
                 if (lane == 0) a.scale[row * (a.d / width) + g] = sc;
                 for (int c = g * width + lane; c < (g + 1) * width; c += step) {
                     const float v = at(c);

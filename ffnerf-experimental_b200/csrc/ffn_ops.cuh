@@ -121,10 +121,11 @@ struct Vec {
     }
 };
 
-// Maximum that keeps a NaN (fmaxf drops it): a row with a NaN has to get a NaN scale.
-__device__ __forceinline__ float max_nan(float a, float b) {
+// The larger magnitude of two values, its sign meaningless, in one instruction; a NaN stays a NaN (fmaxf
+// drops it, and a row with a NaN has to get a NaN scale).
+__device__ __forceinline__ float max_abs(float a, float b) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
 
@@ -146,9 +147,12 @@ __device__ __forceinline__ float e4m3_inverse(float scale) {
 
 // Four fp32 values to four e4m3 bytes, nearest even, saturating at +-448; a NaN stays a NaN.
 __device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-    return lo | (hi << 16);
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+        "mov.b32 %0, {lo, hi};\n\t}" : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
+    return r;
 }
 
 }  // namespace ffn
