@@ -1,0 +1,141 @@
+"""A residual block over the samples of rays, made of the block operators (ffn_ops), and a small training
+run of it: ``python ffnerf-experimental_b200/ray_block.py``.
+
+The fused training step (trainer.py) evaluates one 64-wide MLP per sample and composites colours.  A
+block on top of per-sample features mixes the samples of a ray in depth order and gives each region of
+the scene a sub-network of its own:
+
+    y1 = rmsnorm(x);  gate, value = y1 W_in^T
+    s  = gated_scan(gate, value)             from the far sample to the near one: what composites colours
+    y2, h = rmsnorm(s + x)                   h is the residual stream
+    o  = relu(y2 W1_e^T) W2_e^T              e: the region that the sample lies in
+    out = h + o
+
+Parameters are float32 (updated by ``ffn_native.adam``), the products run on 16-bit copies.  ``serve``
+runs the same block with the experts' first product in 8 bits: the norm writes e4m3 rows with a scale
+each, the weights are quantised once per output channel.
+"""
+from __future__ import annotations
+
+import numpy as np
+import torch
+
+import ffn_native as fn
+import ffn_ops as ops
+
+EPS = 1e-6
+
+
+def regions(points, box_min, box_max, side: int):
+    """Region of each point [n, 3]: the cell of a side^3 grid over the box, int64 in 0 .. side^3 - 1."""
+    lo = torch.as_tensor(box_min, dtype=points.dtype, device=points.device)
+    hi = torch.as_tensor(box_max, dtype=points.dtype, device=points.device)
+    c = ((points - lo) / (hi - lo) * side).long().clamp_(0, side - 1)
+    return (c[:, 0] * side + c[:, 1]) * side + c[:, 2]
+
+
+def route(region, experts: int):
+    """(order, back, offsets): rows sorted by expert, the inverse, and where each expert's rows begin."""
+    order = torch.argsort(region, stable=True)
+    back = torch.empty_like(order)
+    back[order] = torch.arange(order.numel(), device=order.device)
+    ends = torch.bincount(region, minlength=experts).cumsum(0)
+    return order, back, torch.cat((ends.new_zeros(1), ends)).to(torch.int32)
+
+
+class RayBlock:
+    """One block of width d with ``experts`` sub-networks of hidden width m; 16-bit type ``dtype``."""
+
+    def __init__(self, d: int, hidden: int, experts: int, dtype=torch.bfloat16, device: int = 0, seed: int = 0):
+        g = torch.Generator().manual_seed(seed)
+        dev = torch.device("cuda", device)
+        w = lambda *s: (torch.randn(*s, generator=g) * s[-1] ** -0.5).to(dev)  # noqa: E731
+        self.d, self.experts, self.dtype, self.steps = d, experts, dtype, 0
+        self.params = {"g1": torch.ones(d, device=dev), "g2": torch.ones(d, device=dev), "w_in": w(1, 2 * d, d),
+                       "w1": w(experts, hidden, d), "w2": w(experts, d, hidden)}
+        self.moments = {k: (torch.zeros_like(p), torch.zeros_like(p)) for k, p in self.params.items()}
+        self._cast()
+
+    def _cast(self):
+        self.w16 = {k: self.params[k].to(self.dtype) for k in ("w_in", "w1", "w2")}
+        self._w8 = None
+
+    def forward(self, x, region):
+        """x [rays, samples, d]; region [rays * samples].  Returns the output and what backward needs."""
+        b, s, d = x.shape
+        flat = x.reshape(b * s, d)
+        one = torch.tensor([0, b * s], dtype=torch.int32, device=x.device)
+        y1, _, n1, _ = ops.rmsnorm(flat, self.params["g1"], eps=EPS)
+        p = ops.expert_mm(y1, self.w16["w_in"], one).view(b, s, 2 * d)
+        gate, value = p[..., :d], p[..., d:]
+        mix, _ = ops.gated_scan(gate, value, reverse=True)
+        y2, h, n2, _ = ops.rmsnorm(mix.view(b * s, d), self.params["g2"], flat, eps=EPS)
+        order, back, offsets = route(region, self.experts)
+        z = y2[order]
+        a = ops.expert_mm(z, self.w16["w1"], offsets).relu_()
+        out = h + ops.expert_mm(a, self.w16["w2"], offsets)[back]
+        return out.view(b, s, d), (y1, one, n1, gate, value, mix, h, n2, order, back, offsets, z, a)
+
+    def backward(self, dout, saved):
+        """Gradients of the parameters (float32) and of x for the gradient dout of the output."""
+        y1, one, n1, gate, value, mix, h, n2, order, back, offsets, z, a = saved
+        b, s, d = dout.shape
+        flat = dout.reshape(b * s, d)
+        f32 = torch.float32
+        da, dw2 = ops.expert_mm_bwd(flat[order], a, self.w16["w2"], offsets, dw_dtype=f32)
+        dz, dw1 = ops.expert_mm_bwd(da * (a > 0), z, self.w16["w1"], offsets, dw_dtype=f32)
+        dres, dg2 = ops.rmsnorm_bwd(dz[back], h, self.params["g2"], n2, flat)       # of mix and of x
+        dgate, dvalue, _ = ops.gated_scan_bwd(dres.view(b, s, d), gate, value, mix, reverse=True)
+        dp = torch.cat((dgate, dvalue), 2).view(b * s, 2 * d)
+        dy1, dw_in = ops.expert_mm_bwd(dp, y1, self.w16["w_in"], one, dw_dtype=f32)
+        dx, dg1 = ops.rmsnorm_bwd(dy1, n1.x, self.params["g1"], n1, dres)
+        return dx.view(b, s, d), {"g1": dg1, "g2": dg2, "w_in": dw_in, "w1": dw1, "w2": dw2}
+
+    def update(self, grads, lr: float = 1e-3, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8):
+        """One Adam step on the float32 parameters."""
+        self.steps += 1
+        lr_t = lr * np.sqrt(1 - beta2 ** self.steps) / (1 - beta1 ** self.steps)
+        for k, p in self.params.items():
+            m, v = self.moments[k]
+            fn.adam(p, grads[k], m, v, p.numel(), lr_t, beta1, beta2, eps)
+        self._cast()
+
+    def serve(self, x, region):
+        """The block's output with the experts' first product in 8 bits (no gradients)."""
+        b, s, d = x.shape
+        if self._w8 is None:
+            w = self.params["w1"]
+            scale = (w.abs().amax(2) / 448).clamp_min(1e-20)
+            self._w8 = (w / scale[..., None]).to(torch.float8_e4m3fn), scale
+        flat = x.reshape(b * s, d)
+        one = torch.tensor([0, b * s], dtype=torch.int32, device=x.device)
+        y1 = ops.rmsnorm(flat, self.params["g1"], eps=EPS)[0]
+        p = ops.expert_mm(y1, self.w16["w_in"], one).view(b, s, 2 * d)
+        mix, _ = ops.gated_scan(p[..., :d], p[..., d:], reverse=True)
+        y8, h, _, scale = ops.rmsnorm(mix.view(b * s, d), self.params["g2"], flat, eps=EPS, out="e4m3")
+        order, back, offsets = route(region, self.experts)
+        rows = y8.view(torch.uint8)[order].view(torch.float8_e4m3fn)
+        a = ops.expert_mm(rows, self._w8[0], offsets, scale[order], self._w8[1], out_dtype=self.dtype).relu_()
+        return (h + ops.expert_mm(a, self.w16["w2"], offsets)[back]).view(b, s, d)
+
+
+def example(rays: int = 512, samples: int = 64, d: int = 64, side: int = 2, steps: int = 100, seed: int = 0):
+    """Trains a block to reproduce another one's output on random rays; returns the losses."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    teacher, block = RayBlock(d, 2 * d, side ** 3, seed=1), RayBlock(d, 2 * d, side ** 3, seed=2)
+    losses = []
+    for _ in range(steps):
+        points = torch.rand(rays * samples, 3, generator=g, device="cuda")
+        x = torch.randn(rays, samples, d, generator=g, device="cuda").to(block.dtype)
+        region = regions(points, (0.0, 0.0, 0.0), (1.0, 1.0, 1.0), side)
+        want = teacher.forward(x, region)[0].float()
+        out, saved = block.forward(x, region)
+        diff = out.float() - want
+        losses.append(float(diff.square().mean()))
+        block.update(block.backward((diff * (2 * 4096.0 / diff.numel())).to(block.dtype), saved)[1], lr=2e-3)   # Adam ignores the loss scale
+    return losses, block
+
+
+if __name__ == "__main__":
+    losses, block = example()
+    print(f"mean squared error {losses[0]:.4f} -> {losses[-1]:.4f} in {len(losses)} steps, status {ops.status()}")
