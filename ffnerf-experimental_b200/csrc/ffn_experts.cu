@@ -41,6 +41,7 @@ constexpr int EPI_WARPS = 8;               // two groups of four, one accumulato
 constexpr int THREADS = 32 * (EPI_WARPS + 2);
 constexpr int SLAB = 32 * 128;             // one warp's 32 rows x 128 bytes of output
 constexpr size_t SMEM_MOST = 232448;       // what a block may have
+constexpr int COUNTS = (4 * (FFN_MAX_EXPERTS + 1) + 15) & ~15;
 constexpr uint32_t WAIT_ROUNDS = 1u << 12, WAIT_POLLS = 1u << 10;
 
 __device__ int g_status;                   // ST_TC_TIMEOUT when a wait ran out (ffn_ops_status)
@@ -53,7 +54,6 @@ struct Args {
     int experts, cols, depth, rows_m;      // cols: width of the output; rows_m: dW's rows
     int ntiles, mtiles;                    // tiles along the output's width; dW's tiles along its rows
     int tma_out;                           // the output can be stored by TMA (16-byte rows)
-    int most;                              // tiles over the rows (dW: units) that valid offsets give at most
     int chunk;                             // dW: stages of depth of a unit (0: an expert's depth is one unit)
 };
 
@@ -61,12 +61,6 @@ struct Args {
 __host__ __device__ __forceinline__ int units_of(int64_t rows, int chunk) {
     const int blocks = (int)((rows + 63) / 64);
     return chunk == 0 || blocks <= chunk ? 1 : (blocks + chunk - 1) / chunk;
-}
-
-// An expert's rows, kept inside [0, n] whatever the offsets hold.
-__device__ __forceinline__ void expert_rows(const Args& p, int e, int64_t& b, int64_t& end) {
-    b = e == 0 ? 0 : min(max((int64_t)__ldg(p.offsets + e), (int64_t)0), p.n);
-    end = min(max((int64_t)__ldg(p.offsets + e + 1), b), p.n);
 }
 
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
@@ -183,7 +177,7 @@ struct Plan {
     static constexpr int B_BYTES = BH * KB;
     static constexpr int STAGE = A_BYTES + B_BYTES;
     static constexpr int EPI = MODE == FEW_ROWS ? 0 : EPI_WARPS * SLAB;
-    static constexpr int MISC = 1024 + 4 * (FFN_MAX_EXPERTS + 1) + 512;   // alignment, prefix, barriers
+    static constexpr int MISC = 2 * COUNTS + 256;                          // tile counts, rows' ends, barriers
     static constexpr int FIT = (int)((SMEM_MOST - EPI - MISC) / STAGE);
     static constexpr int STAGES = FIT > 12 ? 12 : FIT;
     static constexpr size_t BYTES = (size_t)STAGE * STAGES + EPI + MISC;
@@ -215,11 +209,16 @@ template <int MODE, int BN, int EB, bool PAIR>
 struct Walk {
     int e = 0, start = 0, stop = 0;      // this expert's tiles are start .. stop - 1
     int64_t b = 0, end = 0;              // its rows
-    int known = -1;                      // the expert that b and end belong to
+    bool begun = false;
 
-    __device__ __forceinline__ Tile at(const Args& p, const int* prefix, int t) {
+    // ends[e]: the end of expert e's rows; e - 1's is where they begin
+    __device__ __forceinline__ Tile at(const Args& p, const int* prefix, const int* ends, int t) {
         const int per = MODE == WEIGHT_GRAD ? p.ntiles * p.mtiles : p.ntiles;
-        if (known < 0) stop = prefix[1] * per;
+        if (!begun) {
+            stop = prefix[1] * per;
+            end = ends[0];
+            begun = true;
+        }
         for (int i = 0; t >= stop; ++i) {
             if (i < 4) {
                 ++e;
@@ -233,10 +232,8 @@ struct Walk {
             }
             start = prefix[e] * per;
             stop = prefix[e + 1] * per;
-        }
-        if (known != e) {
-            expert_rows(p, e, b, end);
-            known = e;
+            b = ends[e - 1];
+            end = ends[e];
         }
         Tile k;
         k.e = e;
@@ -288,11 +285,15 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
     using P = Plan<MODE, BN, EB, PAIR>;
     static_assert(!PAIR || ((MODE == FORWARD || MODE == INPUT_GRAD) && BN == 256), "pairs form 256 x 256 tiles");
     constexpr int S = P::STAGES;
-    extern __shared__ unsigned char raw[];
-    unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    extern __shared__ __align__(1024) unsigned char base[];
+    if (tc::smem_u32(base) & 1023u) {                             // the swizzle goes by address bits
+        if (threadIdx.x == 0) atomicOr(&g_status, 4);
+        return;
+    }
     unsigned char* slabs = base + (size_t)P::STAGE * S;
     int* prefix = reinterpret_cast<int*>(slabs + P::EPI);
-    uint64_t* full = reinterpret_cast<uint64_t*>(slabs + P::EPI + ((4 * (FFN_MAX_EXPERTS + 1) + 15) & ~15));
+    int* ends = reinterpret_cast<int*>(slabs + P::EPI + COUNTS);
+    uint64_t* full = reinterpret_cast<uint64_t*>(slabs + P::EPI + 2 * COUNTS);
     uint64_t* empty = full + S;
     uint64_t* done = empty + S;              // accumulator filled
     uint64_t* freed = done + 2;              // accumulator read
@@ -313,29 +314,36 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
             *gone = 0;
         }
     }
-    // tiles (dW: units) of the experts before each: counts side by side, then one warp adds them up
+    // tiles (dW: units) of the experts before each, and the ends of their rows
     constexpr int R = P::ROWS;
-    for (int e = threadIdx.x; e < p.experts; e += THREADS) {
-        int64_t b, end;
-        expert_rows(p, e, b, end);
-        prefix[e + 1] = MODE == WEIGHT_GRAD ? units_of(end - b, p.chunk) : (int)((end - b + R - 1) / R);
-    }
-    __syncthreads();
     if (warp == 0) {
-        // valid offsets give at most `most` tiles; sums stop there, so that offsets that are not
-        // (decreasing ones, whose experts overlap) cannot wrap
-        const int most = p.most;
-        int sum = 0;
+        // an expert begins where the one before it ends, whatever the offsets hold: they are kept inside
+        // [0, n] and never go back, so no tile reaches outside the matrices and none is counted twice
+        int sum = 0, last = 0;
         for (int e0 = 0; e0 < p.experts; e0 += 32) {
-            int v = e0 + lane < p.experts ? prefix[e0 + lane + 1] : 0;
+            const int e = e0 + lane;
+            int end = e < p.experts ? (int)min((int64_t)max(__ldg(p.offsets + e + 1), 0), p.n) : 0;
+            end = max(end, last);
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, end, o);
+                if (lane >= o) end = max(end, u);
+            }
+            int begin = __shfl_up_sync(0xffffffffu, end, 1);
+            if (lane == 0) begin = last;
+            const int rows = end - begin;
+            int v = e >= p.experts ? 0 : MODE == WEIGHT_GRAD ? units_of(rows, p.chunk) : (rows + R - 1) / R;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int u = __shfl_up_sync(0xffffffffu, v, o);
-                if (lane >= o) v = min(v + u, most);
+                if (lane >= o) v += u;
             }
-            v = min(sum + v, most);
-            if (e0 + lane < p.experts) prefix[e0 + lane + 1] = v;
-            sum = __shfl_sync(0xffffffffu, v, 31);
+            if (e < p.experts) {
+                prefix[e + 1] = sum + v;
+                ends[e] = end;
+            }
+            sum += __shfl_sync(0xffffffffu, v, 31);
+            last = __shfl_sync(0xffffffffu, end, 31);
         }
         if (lane == 0) prefix[0] = 0;
     }
@@ -353,7 +361,7 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
         uint32_t ph = 1;
         bool ok = true;
         for (int t = first; t < total && ok; t += stride) {
-            const Tile k = walk.at(p, prefix, t);
+            const Tile k = walk.at(p, prefix, ends, t);
             const int blocks = uniform(k.blocks), row = uniform((int)k.row) + rank * BM, col = uniform(k.col) + rank * P::BH,
                       e = uniform(k.e);
             [[maybe_unused]] const int mrow = uniform(k.mrow);
@@ -417,7 +425,7 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
             int blocks;
             [[maybe_unused]] int rows = 0;                        // dW: rows of depth from the tile's first on
             if constexpr (MODE == WEIGHT_GRAD) {
-                const Tile k = walk.at(p, prefix, t);
+                const Tile k = walk.at(p, prefix, ends, t);
                 blocks = uniform(k.blocks);
                 rows = uniform((int)min(k.end - k.row, (int64_t)0x7fffffff));
             } else {
@@ -479,7 +487,7 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
         unsigned char* sl = slabs + warp * SLAB;
         Walk<MODE, BN, EB, PAIR> walk;
         for (int t = first + acc * stride; t < total; t += 2 * stride) {
-            const Tile k = walk.at(p, prefix, t);
+            const Tile k = walk.at(p, prefix, ends, t);
             const int64_t row = (MODE == WEIGHT_GRAD ? k.mrow : k.row + rank * BM) + quarter * 32;  // this warp's first row
             const int64_t end = MODE == WEIGHT_GRAD ? p.rows_m : k.end;
             float sr = 1.0f;
@@ -584,8 +592,7 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
         }
         if (lane == 0) bulk_wait_read<0>();
         if constexpr (MODE != WEIGHT_GRAD) {                      // rows of no expert
-            int64_t b, last;
-            expert_rows(p, p.experts - 1, b, last);
+            const int64_t last = ends[p.experts - 1];
             const int64_t count = (p.n - last) * p.cols;
             for (int64_t i = (int64_t)blockIdx.x * (32 * EPI_WARPS) + threadIdx.x; i < count;
                  i += (int64_t)gridDim.x * (32 * EPI_WARPS))
@@ -688,7 +695,6 @@ int launch(const Args& a0, const CUtensorMap& ma, const CUtensorMap& mb, const C
     // an upper bound of the tiles: the counts are on the device
     const int64_t most = MODE == WEIGHT_GRAD ? units_most(a.n, a.experts, a.chunk) : a.n / RT + a.experts;
     const int64_t tiles = most * a.ntiles * (MODE == WEIGHT_GRAD ? a.mtiles : 1);
-    a.most = (int)most;
     if (tiles > 0x7fffffff) return op_fail(FFN_E_CAPACITY, "ffn_expert_mm: more than 2^31 output tiles");
     auto k = experts_kernel<MODE, BN, EB, TO, BF, PAIR>;
     static std::atomic<uint64_t> ready{0};            // devices whose limit is set
@@ -794,24 +800,32 @@ int rows_product(int mode, Operand a, Operand b, const float* a_scale, const flo
 template <typename TO>
 __global__ void __launch_bounds__(256) units_sum_kernel(const Args p, const float* __restrict__ part, TO* __restrict__ dw,
                                                         int64_t size) {
-    __shared__ int counts[FFN_MAX_EXPERTS];
-    __shared__ int first;
+    __shared__ int first, units;
     const int e = blockIdx.y;
-    for (int i = threadIdx.x; i <= e; i += 256) {
-        int64_t b, end;
-        expert_rows(p, i, b, end);
-        counts[i] = units_of(end - b, p.chunk);
-    }
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        int v = 0;
-        for (int i = threadIdx.x; i < e; i += 32) v = min(v + counts[i], p.most);
+    if (threadIdx.x < 32) {                                       // as in experts_kernel
+        int sum = 0, last = 0;
+        for (int e0 = 0; e0 <= e; e0 += 32) {
+            const int i = e0 + threadIdx.x;
+            int end = i < p.experts ? (int)min((int64_t)max(__ldg(p.offsets + i + 1), 0), p.n) : 0;
+            end = max(end, last);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v = min(v + __shfl_xor_sync(0xffffffffu, v, o), p.most);
-        if (threadIdx.x == 0) first = v;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, end, o);
+                if ((int)threadIdx.x >= o) end = max(end, u);
+            }
+            int begin = __shfl_up_sync(0xffffffffu, end, 1);
+            if (threadIdx.x == 0) begin = last;
+            const int mine = units_of(end - begin, p.chunk);
+            int before = i < e ? mine : 0;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+            sum += before;
+            if (i == e) units = mine;
+            last = __shfl_sync(0xffffffffu, end, 31);
+        }
+        if (threadIdx.x == 0) first = sum;
     }
     __syncthreads();
-    const int units = min(counts[e], p.most - first);
     const float* src = part + (int64_t)first * size;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.x * 256) {
         float v = 0.0f;
@@ -857,7 +871,6 @@ int weight_product(Operand dy, Operand x, const int32_t* offsets, void* dw, int6
                              : launch_typed<WEIGHT_GRAD, 64>(p, ma, mb, mo, dtype, out_type, sms, st);
     if (rc != FFN_OK || !p.chunk) return rc;
     const int64_t size = (int64_t)m * k;
-    p.most = (int)units_most(n, experts, p.chunk);
     int64_t bx = (size + 255) / 256;
     const int64_t cap = (8 * (int64_t)sms + experts - 1) / experts;
     if (bx > cap) bx = cap;

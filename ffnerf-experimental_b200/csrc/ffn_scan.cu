@@ -51,6 +51,8 @@ struct ScanArgs {
     float* maps;                              // [parts - 1][2][seqs * d]: p and h of each part but the last
 };
 
+constexpr int THREADS = 128;         // small blocks: one lasts as long as its longest sequence
+
 struct Affine { float p, h; };
 
 // A state that is exactly zero stays out of the product: a composed p may have overflowed (linear gates
@@ -259,7 +261,7 @@ __device__ __forceinline__ void part_of(const ScanArgs& a, const Span& s, int pa
 // Composes the map of every part but each sequence's last, from the part's last step to its first:
 // with m the map of the steps after it, a step x -> a x + b makes it x -> (p a) x + (p b + h).
 template <typename T, bool SIG, bool BACK, int C, int U>
-__global__ void __launch_bounds__(256, 2) scan_maps_kernel(const ScanArgs a) {
+__global__ void __launch_bounds__(THREADS, 4) scan_maps_kernel(const ScanArgs a) {
     const int64_t item = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (item >= a.items) return;
     const int part = blockIdx.y, seq = (int)(item / a.groups), ch = (int)(item % a.groups) * C;
@@ -343,7 +345,7 @@ __global__ void __launch_bounds__(1024) scan_join_kernel(const ScanArgs a) {
 }
 
 template <typename T, bool SIG, bool BACK, int C, int U>
-__global__ void __launch_bounds__(256, 2) scan_kernel(const ScanArgs a) {
+__global__ void __launch_bounds__(THREADS, 4) scan_kernel(const ScanArgs a) {
     const int64_t item = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (item >= a.items) return;
     const int part = blockIdx.y, seq = (int)(item / a.groups), ch = (int)(item % a.groups) * C;
@@ -403,7 +405,7 @@ int scan_launch(ScanArgs a, int parts, cudaStream_t st) {
     a.groups = a.d / C;
     a.items = (int64_t)a.seqs * a.groups;
     a.parts = parts;
-    const int threads = parts > 1 && a.items < 256 ? (int)((a.items + 31) / 32 * 32) : 256;
+    const int threads = parts > 1 && a.items < THREADS ? (int)((a.items + 31) / 32 * 32) : THREADS;
     const int64_t blocks = (a.items + threads - 1) / threads;
     if (blocks > 0x7fffffff) return op_fail(FFN_E_CAPACITY, "ffn_gated_scan: too many sequences x channels");
     if (parts > 1) {

@@ -347,7 +347,8 @@ int ffn_gated_scan_bwd(const void* dh, int64_t dh_ld, const float* dh_last, cons
 
 /* Matrix products of rows grouped by expert.  Rows are sorted by expert; expert e has rows
  * offsets[e] .. offsets[e+1] - 1 (32-bit, on the device, experts + 1 of them, offsets[0] = 0,
- * non-decreasing, at most n; an expert may have none) and weights w[e], [m][k] row-major:
+ * non-decreasing, at most n -- others are read as their running maximum, cut off at n; an expert may
+ * have none) and weights w[e], [m][k] row-major:
  *   y[r] = x[r] w[e]^T.
  * Rows from offsets[experts] on belong to no expert; their results are zero.  dtype FFN_F16 or FFN_BF16
  * (out_dtype the same), or FFN_E4M3 for x and w with x_scale [n] and w_scale [experts][m] fp32 (the

@@ -395,6 +395,16 @@ def test_expert_mm_gradient_against_differences(ops):
     assert loss(x, w + vw) - loss(x, w) == float((dw.double() * vw.double()).sum())
 
 
+def test_expert_mm_keeps_offsets_inside(ops):
+    """Offsets that leave [0, n] or go back are read as their running maximum, cut off at n."""
+    x, w, dy = draw(1, 90, 64, dtype=BF16), draw(2, 5, 48, 64, dtype=BF16), draw(3, 90, 48, dtype=BF16)
+    given = torch.tensor([0, 40, 25, -7, 70, 1000], dtype=torch.int32, device="cuda")
+    meant = torch.tensor([0, 40, 40, 40, 70, 90], dtype=torch.int32, device="cuda")
+    assert torch.equal(ops.expert_mm(x, w, given), ops.expert_mm(x, w, meant))
+    for a, b in zip(ops.expert_mm_bwd(dy, x, w, given), ops.expert_mm_bwd(dy, x, w, meant)):
+        assert torch.equal(a, b)
+
+
 def test_expert_mm_is_the_same_on_every_run(ops):
     x, w, off, offsets, dy = expert_inputs(5, BF16)
     a, b = ([ops.expert_mm(x, w, offsets), *ops.expert_mm_bwd(dy, x, w, offsets)] for _ in range(2))
