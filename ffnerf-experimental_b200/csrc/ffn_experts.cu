@@ -376,9 +376,13 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
                         tma_load2<PAIR>(sa, &ma, b * P::DEPTH, row, bar);
                         tma_load3<PAIR>(sb, &mb, b * P::DEPTH, col, e, bar);
                     } else if constexpr (MODE == FEW_ROWS) {
+                        // blocks begin at different depths: all at the same one, they would read W at one
+                        // offset in each of its rows, a stride that few memory channels share
+                        int q = b + (t * 7) % blocks;
+                        if (q >= blocks) q -= blocks;
                         expect_tx(full + s, P::STAGE);
-                        tma_load3<PAIR>(sa, &ma, b * P::DEPTH, col, e, bar);
-                        tma_load2<PAIR>(sb, &mb, b * P::DEPTH, row, bar);
+                        tma_load3<PAIR>(sa, &ma, q * P::DEPTH, col, e, bar);
+                        tma_load2<PAIR>(sb, &mb, q * P::DEPTH, row, bar);
                     } else {
                         // boxes of 64 columns; those wholly outside the matrix are left out (what is in
                         // their place reaches only outputs that are not stored)
