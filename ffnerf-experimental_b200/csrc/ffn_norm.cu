@@ -460,6 +460,8 @@ int norm_launch(const NormArgs& a0, bool aligned, cudaStream_t st) {
     return op_launched("ffn_rmsnorm");
 }
 
+constexpr int MOST_D = 1 << 30;        // columns are counted in 32 bits, in steps of a block
+
 constexpr int BWD_BLOCKS_PER_SM = 4;   // at most; as many as are resident: their rows of partial sums are read again
 
 template <typename T>
@@ -502,7 +504,7 @@ extern "C" {
 int ffn_rmsnorm(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, const float* gamma, void* h,
                 void* y, float* scale, float* rstd, int64_t n, int32_t d, float eps, int dtype, int out_dtype,
                 int32_t group, void* stream) {
-    if (n < 0 || d < 1) return op_fail(FFN_E_CONFIG, "ffn_rmsnorm: n must be >= 0 and d >= 1");
+    if (n < 0 || d < 1 || d > MOST_D) return op_fail(FFN_E_CONFIG, "ffn_rmsnorm: n must be >= 0 and 1 <= d <= 2^30");
     if (dtype != FFN_F32 && dtype != FFN_F16 && dtype != FFN_BF16)
         return op_fail(FFN_E_CONFIG, "ffn_rmsnorm: dtype must be FFN_F32, FFN_F16 or FFN_BF16");
     const bool out8 = out_dtype == FFN_E4M3;
@@ -535,7 +537,7 @@ uint64_t ffn_rmsnorm_bwd_workspace(int64_t n, int32_t d) {
 int ffn_rmsnorm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, const void* residual,
                     int64_t residual_ld, const float* gamma, const float* rstd, const void* dresidual, int64_t dresidual_ld, void* dx, float* dgamma, void* workspace,
                     uint64_t workspace_bytes, int64_t n, int32_t d, int dtype, void* stream) {
-    if (n < 0 || d < 1) return op_fail(FFN_E_CONFIG, "ffn_rmsnorm_bwd: n must be >= 0 and d >= 1");
+    if (n < 0 || d < 1 || d > MOST_D) return op_fail(FFN_E_CONFIG, "ffn_rmsnorm_bwd: n must be >= 0 and 1 <= d <= 2^30");
     if (dtype != FFN_F32 && dtype != FFN_F16 && dtype != FFN_BF16)
         return op_fail(FFN_E_CONFIG, "ffn_rmsnorm_bwd: dtype must be FFN_F32, FFN_F16 or FFN_BF16");
     if (!dgamma) return op_fail(FFN_E_CONFIG, "ffn_rmsnorm_bwd: a required pointer is NULL");

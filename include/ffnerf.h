@@ -300,7 +300,7 @@ int ffn_forward_backward_noalloc(const ffn_config* cfg, const float* params, flo
  * calls come from ffn_last_error(NULL). */
 enum { FFN_F32 = 0, FFN_F16 = 1, FFN_BF16 = 2, FFN_E4M3 = 3 };
 
-/* Root-mean-square norm of x + residual (residual may be NULL), n rows of d columns:
+/* Root-mean-square norm of x + residual (residual may be NULL), n rows of d columns (at most 2^30):
  *   h = x + residual, rstd = 1 / sqrt(mean(h^2) + eps), y = h * rstd * gamma   (fp32 throughout)
  * dtype (FFN_F32, FFN_F16, FFN_BF16): type of x, residual and h.  h and rstd ([n], fp32) may be NULL
  * when they are not wanted; h is the sum rounded to dtype, y is formed from the unrounded sum.

@@ -434,6 +434,37 @@ def test_streams(ops):
     assert torch.equal(h, h2) and torch.equal(last, last2)
 
 
+def test_calls_in_a_graph(ops):
+    """Every operator can be captured: nothing synchronises or reads sizes back, and a replay on new inputs
+    and other offsets gives what a call on them gives."""
+    n, d, e = 600, 64, 4
+    x, r, w, g = draw(1, n, d, dtype=BF16), draw(2, n, d, dtype=BF16), draw(3, e, d, d, dtype=BF16), torch.ones(d, device="cuda")
+    off = torch.tensor([0, 100, 100, 450, 600], dtype=torch.int32, device="cuda")
+
+    def calls():
+        y, h, st, _ = ops.rmsnorm(x, g, r)
+        q, _, _, sc = ops.rmsnorm(x, g, r, out="e4m3")
+        s, last = ops.gated_scan(y, h, offsets=off, max_len=n)
+        z = ops.expert_mm(s, w, off)
+        dx, dw = ops.expert_mm_bwd(z, s, w, off)
+        dg, dv, d0 = ops.gated_scan_bwd(dx, y, h, s, offsets=off, max_len=n)
+        return [y, h, q.float(), sc, s, last, z, dx, dw, dg, dv, d0, *ops.rmsnorm_bwd(dg, h, g, st, dv)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        calls()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = calls()
+    x.copy_(draw(7, n, d, dtype=BF16))
+    off.copy_(torch.tensor([0, 0, 300, 310, 590], dtype=torch.int32))
+    graph.replay()
+    for a, b in zip(got, calls()):
+        assert torch.equal(a, b)
+
+
 def test_refusals_on_the_device(ops):
     x, g = draw(1, 8, 64, dtype=BF16), torch.ones(64, device="cuda")
     w = draw(2, 2, 32, 64, dtype=BF16)

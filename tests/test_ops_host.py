@@ -19,6 +19,7 @@ def test_entry_points_check_their_arguments():
     lib = fn.load_library()
     p = C.c_void_p(0x1000)   # never read: each call is refused on its sizes or types
     refused(lib.ffn_rmsnorm(p, 8, None, 0, p, None, p, None, None, -1, 8, 1e-6, 0, 0, 0, None), lib, "n must be")
+    refused(lib.ffn_rmsnorm(p, 1 << 31, None, 0, p, None, p, None, None, 1, (1 << 30) + 1, 1e-6, 1, 1, 0, None), lib, "2^30")
     refused(lib.ffn_rmsnorm(p, 8, None, 0, p, None, p, None, None, 4, 8, 1e-6, 3, 3, 0, None), lib, "dtype")
     refused(lib.ffn_rmsnorm(p, 8, None, 0, p, None, p, None, None, 4, 8, 1e-6, 1, 2, 0, None), lib, "out_dtype")
     refused(lib.ffn_rmsnorm(p, 8, None, 0, p, None, p, p, None, 4, 8, 1e-6, 1, 3, 32, None), lib, "group")
