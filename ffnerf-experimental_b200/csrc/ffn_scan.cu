@@ -48,10 +48,12 @@ struct ScanArgs {
     int seqs, d, groups;                      // groups = d / C
     int reverse;
     int parts;                                // of each sequence's time (1: no maps)
+    int joined;                               // the maps have been turned into the states that parts begin with
     float* maps;                              // [parts - 1][2][seqs * d]: p and h of each part but the last
 };
 
 constexpr int THREADS = 128;         // small blocks: one lasts as long as its longest sequence
+constexpr int STEPS = 8;             // steps whose loads a thread issues together (long sequences)
 
 struct Affine { float p, h; };
 
@@ -345,17 +347,28 @@ __global__ void __launch_bounds__(1024) scan_join_kernel(const ScanArgs a) {
 }
 
 template <typename T, bool SIG, bool BACK, int C, int U>
-__global__ void __launch_bounds__(THREADS, 4) scan_kernel(const ScanArgs a) {
+__global__ void __launch_bounds__(THREADS, U == STEPS ? 4 : BACK && sizeof(T) * C > 4 ? 5 : 8) scan_kernel(const ScanArgs a) {
     const int64_t item = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (item >= a.items) return;
     const int part = blockIdx.y, seq = (int)(item / a.groups), ch = (int)(item % a.groups) * C;
     const Span s = span_of<BACK>(a, seq);
     float state[C];
-    if (part == 0) first_state<BACK, C>(a, seq, ch, state);
-    else load_floats<C>(a.maps + (int64_t)(part - 1) * 2 * a.seqs * a.d + (int64_t)seq * a.d + ch, state);
+    const int64_t plane = (int64_t)a.seqs * a.d;
+    const float* mp = a.maps + (int64_t)seq * a.d + ch;
+    if (part == 0 || !a.joined) first_state<BACK, C>(a, seq, ch, state);
+    else load_floats<C>(mp + (int64_t)(part - 1) * 2 * plane, state);
+    if (!a.joined)
+#pragma unroll 8
+        for (int q = 0; q < part; ++q, mp += 2 * plane) {
+            float p[C], h[C];
+            load_floats<C>(mp, p);
+            load_floats<C>(mp + plane, h);
+#pragma unroll
+            for (int j = 0; j < C; ++j) state[j] = apply(Affine{p[j], h[j]}, state[j]);
+        }
     int64_t lo, hi;
     part_of<U>(a, s, part, lo, hi);
-    constexpr bool AHEAD = !BACK;                      // (four streams and their successors do not fit the registers)
+    constexpr bool AHEAD = !BACK && U == STEPS;                      // (four streams and their successors do not fit the registers)
     Chunk<T, SIG, BACK, C, U> next;
     if (AHEAD && lo < hi) next.template load<false>(a, s, lo, (int)min(hi - lo, (int64_t)U), ch);
 #pragma unroll 1
@@ -378,7 +391,8 @@ __global__ void __launch_bounds__(THREADS, 4) scan_kernel(const ScanArgs a) {
     if (part == 0) clear_outside<T, BACK, C>(a, seq, ch);
 }
 
-constexpr int U = 8;                 // steps whose loads a thread issues together
+constexpr int SHORT = 4;             // the same for sequences of at most 8 steps: fewer registers, more threads
+constexpr int FEW_PARTS = 24;        // so many maps a thread composes itself; joining them first costs a launch
 constexpr int PART_STEPS = 32;       // a part is worth its second read from about here on
 
 // How the work is laid out: channels of a thread, parts of time.
@@ -401,7 +415,7 @@ ScanPlan scan_plan(int64_t seqs, int d, int most_width, int64_t longest, int sms
 }
 
 template <typename T, bool SIG, bool BACK, int C>
-int scan_launch(ScanArgs a, int parts, cudaStream_t st) {
+int scan_launch(ScanArgs a, int parts, int64_t longest, cudaStream_t st) {
     a.groups = a.d / C;
     a.items = (int64_t)a.seqs * a.groups;
     a.parts = parts;
@@ -409,26 +423,32 @@ int scan_launch(ScanArgs a, int parts, cudaStream_t st) {
     const int64_t blocks = (a.items + threads - 1) / threads;
     if (blocks > 0x7fffffff) return op_fail(FFN_E_CAPACITY, "ffn_gated_scan: too many sequences x channels");
     if (parts > 1) {
-        scan_maps_kernel<T, SIG, BACK, C, U><<<dim3((unsigned)blocks, parts - 1), threads, 0, st>>>(a);
+        scan_maps_kernel<T, SIG, BACK, C, STEPS><<<dim3((unsigned)blocks, parts - 1), threads, 0, st>>>(a);
         if (int rc = op_launched("ffn_gated_scan maps")) return rc;
-        const int64_t joins = ((int64_t)a.seqs * a.d + 31) / 32;
-        scan_join_kernel<BACK><<<(unsigned)joins, dim3(32, 32), 0, st>>>(a);
-        if (int rc = op_launched("ffn_gated_scan join")) return rc;
+        a.joined = parts > FEW_PARTS;
+        if (a.joined) {
+            const int64_t joins = ((int64_t)a.seqs * a.d + 31) / 32;
+            scan_join_kernel<BACK><<<(unsigned)joins, dim3(32, 32), 0, st>>>(a);
+            if (int rc = op_launched("ffn_gated_scan join")) return rc;
+        }
     }
-    scan_kernel<T, SIG, BACK, C, U><<<dim3((unsigned)blocks, parts), threads, 0, st>>>(a);
+    if (parts == 1 && longest <= 2 * SHORT) scan_kernel<T, SIG, BACK, C, SHORT><<<(unsigned)blocks, threads, 0, st>>>(a);
+    else scan_kernel<T, SIG, BACK, C, STEPS><<<dim3((unsigned)blocks, parts), threads, 0, st>>>(a);
     return op_launched("ffn_gated_scan");
 }
 
 template <typename T, bool BACK, int C>
-int scan_form(const ScanArgs& a, int form, int parts, cudaStream_t st) {
-    return form == FFN_SCAN_SIGMOID ? scan_launch<T, true, BACK, C>(a, parts, st) : scan_launch<T, false, BACK, C>(a, parts, st);
+int scan_form(const ScanArgs& a, int form, int parts, int64_t longest, cudaStream_t st) {
+    return form == FFN_SCAN_SIGMOID ? scan_launch<T, true, BACK, C>(a, parts, longest, st)
+                                    : scan_launch<T, false, BACK, C>(a, parts, longest, st);
 }
 
 template <typename T, bool BACK>
-int scan_width(const ScanArgs& a, int form, ScanPlan plan, cudaStream_t st) {
+int scan_width(const ScanArgs& a, int form, ScanPlan plan, int64_t longest, cudaStream_t st) {
     if constexpr (sizeof(T) == 2)
-        if (plan.width == 4) return scan_form<T, BACK, 4>(a, form, plan.parts, st);
-    return plan.width >= 2 ? scan_form<T, BACK, 2>(a, form, plan.parts, st) : scan_form<T, BACK, 1>(a, form, plan.parts, st);
+        if (plan.width == 4) return scan_form<T, BACK, 4>(a, form, plan.parts, longest, st);
+    return plan.width >= 2 ? scan_form<T, BACK, 2>(a, form, plan.parts, longest, st)
+                           : scan_form<T, BACK, 1>(a, form, plan.parts, longest, st);
 }
 
 // Bytes of a plan's maps.
@@ -442,9 +462,9 @@ int scan_dispatch(ScanArgs a, int dtype, int form, int width, int64_t longest, v
     if (ws_bytes < scan_bytes(plan, a.seqs, a.d) || !op_aligned(ws, 16))
         return op_fail(FFN_E_CAPACITY, "ffn_gated_scan: the workspace is smaller than ffn_gated_scan_workspace says, or not 16-byte aligned");
     a.maps = static_cast<float*>(ws);
-    if (dtype == FFN_F32) return scan_width<float, BACK>(a, form, plan, st);
-    if (dtype == FFN_F16) return scan_width<__half, BACK>(a, form, plan, st);
-    return scan_width<__nv_bfloat16, BACK>(a, form, plan, st);
+    if (dtype == FFN_F32) return scan_width<float, BACK>(a, form, plan, longest, st);
+    if (dtype == FFN_F16) return scan_width<__half, BACK>(a, form, plan, longest, st);
+    return scan_width<__nv_bfloat16, BACK>(a, form, plan, longest, st);
 }
 
 // The widest group of channels, at most 8 bytes, that every row of these matrices holds aligned: 4, 2 or 1.
