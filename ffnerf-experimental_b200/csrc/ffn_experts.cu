@@ -758,12 +758,14 @@ int tile_width(int cols, int64_t row_tiles, int sms) {
     return bn;
 }
 
-// Pairs of blocks: from so many rows an expert has on average, and while a pair of SMs still gets several
-// tiles.  Their tile holds twice the rows, so an expert's last tile wastes twice as much; per tile they read
-// a third less and hold half as many stages more in flight.  Forward, 16 experts of 1024 x 4096, pair /
-// single in us: 256 rows 43 / 46, 512 67 / 69, 1024 110 / 122, 2048 197 / 230; of 4096 x 1024: 512 rows
-// 76 / 66, 768 98 / 91, 1024 109 / 119, 2048 224 / 255; 64 experts of 256 x 320: 1024 rows 37 / 31.
-constexpr int PAIR_ROWS = 1024, PAIR_WORK = 1 << 20;   // rows an expert, elements of W
+// Pairs of blocks: from so many rows an expert has on average and so many bytes of depth (eight stages).
+// Their tile holds twice the rows, so an expert's last tile wastes twice as much; per tile they read a
+// third less and hold half as many stages more in flight.  Forward, 16-bit operands, pair / single in us:
+// 16 experts of 1024 x 4096 with 512 rows each 67 / 69, 1024 110 / 122, 2048 197 / 230; of 4096 x 1024 with
+// 768 rows 98 / 91, 1024 109 / 119; 24 of 2048 x 240 with 2500 rows 63 / 69; 8 of 512 x 1024 with 6250 rows
+// 52 / 54; 16 of 512 x 512 with 3100 rows 37 / 37; 16 of 256 x 1024 with 6250 rows 82 / 74; 64 of 256 x 320
+// with 1024 rows 37 / 31; 4 of 128 x 256 with 75,000 rows 55 / 45.
+constexpr int PAIR_ROWS = 1024, PAIR_DEPTH = 1024;
 
 // out[r] = a[r] b[e]^T (FORWARD, FEW_ROWS) or a[r] b[e] (INPUT_GRAD); depth and cols are those of the product.
 int rows_product(int mode, Operand a, Operand b, const float* a_scale, const float* b_scale, const int32_t* offsets, void* out,
@@ -783,7 +785,7 @@ int rows_product(int mode, Operand a, Operand b, const float* a_scale, const flo
                         : launch_typed<FEW_ROWS, 64>(p, ma, mb, mo, dtype, out_dtype, sms, st);
     }
     const int bn = tile_width(cols, n / BM + (experts + 1) / 2, sms);
-    const bool pair = bn == 256 && n >= (int64_t)experts * PAIR_ROWS && (int64_t)depth * cols >= PAIR_WORK;
+    const bool pair = bn == 256 && n >= (int64_t)experts * PAIR_ROWS && (int64_t)depth * (int64_t)type_size(dtype) >= PAIR_DEPTH;
     if (p.tma_out && !make_map(&mo, out, out_dtype, cols, n, cols, 0, 32)) return bad_map();
     if (!make_map(&ma, a.p, dtype, depth, n, a.ld, 0, BM)) return bad_map();
     if (mode == FORWARD) {
@@ -842,14 +844,18 @@ constexpr int64_t WIDE = 1 << 20;     // dW: the depth is cut instead of the til
 
 // Stages of depth in a unit of dW, or 0.  Experts share the rows unevenly and a small W has few output
 // tiles: 64 experts of 64 x 64 have 64, the largest of them several times the average depth.  Below two
-// tiles an SM the depth is cut into units, about four an SM in all and 16 stages at least, whose fp32
-// sums go through the workspace.
+// tiles an SM the depth is cut into units, whose fp32 sums go through the workspace: as many as make two
+// full rounds of the SMs (four where the experts alone come near two), of 16 stages at least.  More units
+// balance no better and write and read more sums: 200,000 rows, 8 experts of 256 x 512, took 89 us with
+// 600 tiles (158 MB of sums).
 int weight_chunk(int64_t n, int experts, int k, int m, int sms) {
     const int bn = tile_width(k, WIDE, sms);
     const int64_t per = (int64_t)((m + BM - 1) / BM) * ((k + bn - 1) / bn), blocks = n / 64 + experts;
-    if (per * experts >= 2 * (int64_t)sms) return 0;
-    const int64_t chunk = (blocks * per + 4 * sms - 1) / (4 * sms);
-    const int64_t c = chunk > 16 ? chunk : 16;
+    const int64_t least = per * experts;                          // every expert has a unit
+    if (least >= 2 * (int64_t)sms) return 0;
+    const int64_t room = (least > sms ? 4 : 2) * (int64_t)sms - least;
+    int64_t c = (blocks * per + room - 1) / room;
+    c = c > 16 ? c : 16;
     return blocks <= c * experts ? 0 : (int)c;
 }
 uint64_t weight_workspace(int64_t n, int experts, int k, int m, int sms) {
