@@ -24,6 +24,16 @@
 // stored (a row's products depend on that row only).  In dW the rows are the depth: there the stage that
 // reaches past the expert's last row has the rest of its rows cleared in shared memory, in both
 // operands, since a NaN times zero would not be zero.
+//
+// Where rows are many, two blocks form one 256 x 256 tile (cta_group::2): each loads and holds half of both
+// operands and half of the accumulator, and the first issues the products of both.  That reads 32 KB a
+// block and stage where a single block's 128 x 256 tile reads 48, so six stages fit in place of four.
+//
+// What bounds it: on wide matrices the tensor cores under the power limit (16384 rows, 16 experts of
+// 1024 x 4096, bf16: forward 111 us = 1.24 PFLOP/s of useful products, 0.74 of the measured library rate,
+// and one row in nine of the tiles is unused; dx 110, dW 124; e4m3, 30011 rows, 8 x 4096 x 2048: 181 us =
+// 2.8 PFLOP/s), on narrow ones HBM (2^20 rows, 64 x 64 x 64: forward 52 us = 0.81 of the copy rate), with
+// a few rows W's bytes (16 rows, 8 x 4096 x 4096: 47 us = 0.88).
 #include <atomic>
 #include <cuda.h>
 
@@ -243,7 +253,7 @@ struct Walk {
             int u = r;
             if (per > 1) { u = r / per; r -= u * per; } else r = 0;
             const int c = p.mtiles > 1 ? r / p.mtiles : r;
-            k.mrow = (r - c * p.mtiles) * BM;
+            k.mrow = (r - c * p.mtiles) * (PAIR ? 2 * BM : BM);
             k.col = c * BN;
             k.row = b + (int64_t)u * p.chunk * 64;
             k.blocks = (int)((end - b + 63) / 64) - u * p.chunk;
@@ -267,10 +277,25 @@ struct Walk {
     }
 };
 
+// One round of polls; CLUSTER: what the other block wrote before its arrival is visible afterwards.
+template <bool CLUSTER>
+__device__ __forceinline__ bool poll(uint64_t* bar, uint32_t parity) {
+    if constexpr (!CLUSTER) return tc::mbar_wait(bar, parity, WAIT_POLLS);
+    for (uint32_t i = 0; i < WAIT_POLLS; ++i) {
+        uint32_t done;
+        asm volatile("{\n\t.reg .pred p;\n\t"
+                     "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+                     "selp.b32 %0, 1, 0, p;\n\t}\n" : "=r"(done) : "r"(tc::smem_u32(bar)), "r"(parity) : "memory");
+        if (done) return true;
+    }
+    return false;
+}
+
 // Waits for a phase of an mbarrier; false when the wait ran out here or in another role of the block.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* gone) {
     for (uint32_t i = 0; i < WAIT_ROUNDS; ++i) {
-        if (tc::mbar_wait(bar, parity, WAIT_POLLS)) return true;
+        if (poll<CLUSTER>(bar, parity)) return true;
         if (*gone) return false;
     }
     *gone = 1;
@@ -278,12 +303,25 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
     return false;
 }
 
+// dW: zeros in the rows of a stage from `left` to the next multiple of 16, in both operands; one warp.
+template <int MODE, int BN, int EB, bool PAIR>
+__device__ __forceinline__ void clear_rows(unsigned char* stage, int left, int lane) {
+    const int rows = (left + 15) / 16 * 16 - left;
+    constexpr int CH = (BM + Plan<MODE, BN, EB, PAIR>::BH) / 64;
+    for (int i = lane; i < CH * rows * 8; i += 32) {
+        const int ch = i / (rows * 8), r = left + (i / 8) % rows;
+        *reinterpret_cast<uint4*>(stage + ch * 8192 + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+    }
+    tc::fence_proxy_async();
+    __syncwarp();
+}
+
 template <int MODE, int BN, int EB, typename TO, bool BF, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1)
 experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb,
                const __grid_constant__ CUtensorMap mo) {
     using P = Plan<MODE, BN, EB, PAIR>;
-    static_assert(!PAIR || ((MODE == FORWARD || MODE == INPUT_GRAD) && BN == 256), "pairs form 256 x 256 tiles");
+    static_assert(!PAIR || (MODE != FEW_ROWS && BN == 256), "pairs form 256 x 256 tiles");
     constexpr int S = P::STAGES;
     extern __shared__ __align__(1024) unsigned char base[];
     if (tc::smem_u32(base) & 1023u) {                             // the swizzle goes by address bits
@@ -297,7 +335,9 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
     uint64_t* empty = full + S;
     uint64_t* done = empty + S;              // accumulator filled
     uint64_t* freed = done + 2;              // accumulator read
-    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(freed + 2);
+    uint64_t* tail = freed + 2;              // dW by a pair: the second block may clear the last stage's spare rows
+    uint64_t* clean = tail + 1;              // and has done so (on the first block)
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(clean + 1);
     volatile int* gone = reinterpret_cast<volatile int*>(tmem_at + 1);
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = PAIR ? uniform(cluster_rank()) : 0;                      // in the pair
@@ -311,6 +351,8 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
         if (lane == 0) {
             for (int i = 0; i < S; ++i) { tc::mbar_init(full + i, 1); tc::mbar_init(empty + i, 1); }
             for (int i = 0; i < 2; ++i) { tc::mbar_init(done + i, 1); tc::mbar_init(freed + i, PAIR ? 8 : 4); }
+            tc::mbar_init(tail, 1);
+            tc::mbar_init(clean, 1);
             *gone = 0;
         }
     }
@@ -362,9 +404,9 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
         bool ok = true;
         for (int t = first; t < total && ok; t += stride) {
             const Tile k = walk.at(p, prefix, ends, t);
-            const int blocks = uniform(k.blocks), row = uniform((int)k.row) + rank * BM, col = uniform(k.col) + rank * P::BH,
+            const int blocks = uniform(k.blocks), row = uniform((int)k.row) + (MODE == WEIGHT_GRAD ? 0 : rank * BM), col = uniform(k.col) + rank * P::BH,
                       e = uniform(k.e);
-            [[maybe_unused]] const int mrow = uniform(k.mrow);
+            [[maybe_unused]] const int mrow = uniform(k.mrow) + rank * BM;
             for (int b = 0; b < blocks; ++b) {
                 if (!(ok = wait(empty + s, ph, gone))) break;
                 const uint32_t sa = tc::smem_u32(base + (size_t)s * P::STAGE), sb = sa + P::A_BYTES;
@@ -396,13 +438,15 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
                             for (int j = 0; j < P::BH / 64; ++j)
                                 if (j < nb) tma_load3<PAIR>(sb + j * 8192, &mb, col + j * 64, b * 64, e, bar);
                         } else {
-                            const int na = min(BM / 64, (p.rows_m - mrow + 63) / 64);
-                            expect_tx(full + s, (na + nb) * 8192);
+                            auto strips = [&](int r) { return max(0, min(BM / 64, (p.rows_m - r + 63) / 64)); };
+                            const int na = strips(mrow);
+                            if (rank == 0)
+                                expect_tx(full + s, (na + nb + (PAIR ? strips(mrow + BM) + boxes(col + P::BH) : 0)) * 8192);
 #pragma unroll
                             for (int j = 0; j < BM / 64; ++j)
                                 if (j < na) tma_load2<PAIR>(sa + j * 8192, &ma, mrow + j * 64, row + b * 64, bar);
 #pragma unroll
-                            for (int j = 0; j < BN / 64; ++j)
+                            for (int j = 0; j < P::BH / 64; ++j)
                                 if (j < nb) tma_load2<PAIR>(sb + j * 8192, &mb, col + j * 64, row + b * 64, bar);
                         }
                     }
@@ -424,7 +468,23 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
         Walk<MODE, BN, EB, PAIR> walk;
         int s = 0, acc = 0;
         uint32_t ph = 0, aph = 1;
+        [[maybe_unused]] uint32_t cph = 0;
         bool ok = true;
+        if constexpr (PAIR && MODE == WEIGHT_GRAD) {              // the second block clears its share when told to
+            for (int t = first; t < total && ok && rank == 1; t += stride) {
+                const Tile k = walk.at(p, prefix, ends, t);
+                if (k.blocks == 0) continue;
+                const int left = (int)min(k.end - k.row, (int64_t)0x7fffffff) - (k.blocks - 1) * 64;
+                s = (s + k.blocks - 1) % S;
+                if (left < 64 && left % 16) {
+                    if (!(ok = wait<true>(tail, cph, gone))) break;
+                    cph ^= 1;
+                    clear_rows<MODE, BN, EB, PAIR>(base + (size_t)s * P::STAGE, left, lane);
+                    if (lane == 0) arrive_at(in_block(tc::smem_u32(clean), 0));
+                }
+                s = (s + 1) % S;
+            }
+        }
         for (int t = first; t < total && ok && rank == 0; t += stride) {
             int blocks;
             [[maybe_unused]] int rows = 0;                        // dW: rows of depth from the tile's first on
@@ -447,15 +507,17 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
                     const int left = rows - b * 64;
                     if (left < 64) {                              // rows of the next expert become zeros
                         steps = (left + 15) / 16;
-                        const int clear = steps * 16 - left;
-                        constexpr int CH = (BM + BN) / 64;
-                        for (int i = lane; i < CH * clear * 8; i += 32) {
-                            const int ch = i / (clear * 8), r = left + (i / 8) % clear;
-                            *reinterpret_cast<uint4*>(base + (size_t)s * P::STAGE + ch * 8192 + r * 128 + (i & 7) * 16) =
-                                make_uint4(0, 0, 0, 0);
+                        if (left % 16) {
+                            if constexpr (PAIR) {
+                                if (elect()) arrive_at(in_block(tc::smem_u32(tail), 1));
+                                __syncwarp();
+                            }
+                            clear_rows<MODE, BN, EB, PAIR>(base + (size_t)s * P::STAGE, left, lane);
+                            if constexpr (PAIR) {
+                                if (!(ok = wait<true>(clean, cph, gone))) break;
+                                cph ^= 1;
+                            }
                         }
-                        tc::fence_proxy_async();
-                        __syncwarp();
                     }
                 }
                 if (elect()) {
@@ -479,7 +541,10 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
                 if (++s == S) { s = 0; ph ^= 1; }
             }
             if (MODE == WEIGHT_GRAD && blocks == 0) {             // no rows: the output is zero
-                if (elect()) arrive(done + acc);
+                if (elect()) {
+                    arrive(done + acc);
+                    if constexpr (PAIR) arrive_at(in_block(tc::smem_u32(done + acc), 1));
+                }
                 __syncwarp();
             }
             if (++acc == 2) { acc = 0; aph ^= 1; }
@@ -492,7 +557,7 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
         Walk<MODE, BN, EB, PAIR> walk;
         for (int t = first + acc * stride; t < total; t += 2 * stride) {
             const Tile k = walk.at(p, prefix, ends, t);
-            const int64_t row = (MODE == WEIGHT_GRAD ? k.mrow : k.row + rank * BM) + quarter * 32;  // this warp's first row
+            const int64_t row = (MODE == WEIGHT_GRAD ? k.mrow : k.row) + rank * BM + quarter * 32;  // this warp's first row
             const int64_t end = MODE == WEIGHT_GRAD ? p.rows_m : k.end;
             float sr = 1.0f;
             if constexpr (EB == 1 && MODE == FORWARD) sr = row + lane < end ? __ldg(p.a_scale + row + lane) : 0.0f;
@@ -695,7 +760,7 @@ int launch(const Args& a0, const CUtensorMap& ma, const CUtensorMap& mb, const C
     Args a = a0;
     constexpr int NT = MODE == FEW_ROWS ? BM : BN, RT = P::ROWS;
     a.ntiles = (a.cols + NT - 1) / NT;
-    a.mtiles = (a.rows_m + BM - 1) / BM;
+    a.mtiles = (a.rows_m + (PAIR ? 2 : 1) * BM - 1) / ((PAIR ? 2 : 1) * BM);
     // an upper bound of the tiles: the counts are on the device
     const int64_t most = MODE == WEIGHT_GRAD ? units_most(a.n, a.experts, a.chunk) : a.n / RT + a.experts;
     const int64_t tiles = most * a.ntiles * (MODE == WEIGHT_GRAD ? a.mtiles : 1);
@@ -842,6 +907,10 @@ __global__ void __launch_bounds__(256) units_sum_kernel(const Args p, const floa
 
 constexpr int64_t WIDE = 1 << 20;     // dW: the depth is cut instead of the tiles
 
+bool weight_pair(int64_t n, int experts, int k, int m, int sms) {
+    return tile_width(k, WIDE, sms) == 256 && m > BM && n >= (int64_t)experts * PAIR_ROWS;
+}
+
 // Stages of depth in a unit of dW, or 0.  Experts share the rows unevenly and a small W has few output
 // tiles: 64 experts of 64 x 64 have 64, the largest of them several times the average depth.  Below two
 // tiles an SM the depth is cut into units, whose fp32 sums go through the workspace: as many as make two
@@ -850,7 +919,9 @@ constexpr int64_t WIDE = 1 << 20;     // dW: the depth is cut instead of the til
 // 600 tiles (158 MB of sums).
 int weight_chunk(int64_t n, int experts, int k, int m, int sms) {
     const int bn = tile_width(k, WIDE, sms);
-    const int64_t per = (int64_t)((m + BM - 1) / BM) * ((k + bn - 1) / bn), blocks = n / 64 + experts;
+    const int bm = weight_pair(n, experts, k, m, sms) ? 2 * BM : BM;
+    if (bm > BM) sms /= 2;                                        // a tile takes two
+    const int64_t per = (int64_t)((m + bm - 1) / bm) * ((k + bn - 1) / bn), blocks = n / 64 + experts;
     const int64_t least = per * experts;                          // every expert has a unit
     if (least >= 2 * (int64_t)sms) return 0;
     const int64_t room = (least > sms ? 4 : 2) * (int64_t)sms - least;
@@ -876,7 +947,8 @@ int weight_product(Operand dy, Operand x, const int32_t* offsets, void* dw, int6
     if (p.tma_out && !make_map(&mo, out, out_type, k, m, k, units_most(n, experts, p.chunk), 32)) return bad_map();
     if (!make_map(&ma, dy.p, dtype, m, n, dy.ld, 0, 64) || !make_map(&mb, x.p, dtype, k, n, x.ld, 0, 64)) return bad_map();
     const int bn = tile_width(k, WIDE, sms);
-    const int rc = bn == 256 ? launch_typed<WEIGHT_GRAD, 256>(p, ma, mb, mo, dtype, out_type, sms, st)
+    const int rc = weight_pair(n, experts, k, m, sms) ? launch_typed<WEIGHT_GRAD, 256, true>(p, ma, mb, mo, dtype, out_type, sms, st)
+                 : bn == 256 ? launch_typed<WEIGHT_GRAD, 256>(p, ma, mb, mo, dtype, out_type, sms, st)
                  : bn == 128 ? launch_typed<WEIGHT_GRAD, 128>(p, ma, mb, mo, dtype, out_type, sms, st)
                              : launch_typed<WEIGHT_GRAD, 64>(p, ma, mb, mo, dtype, out_type, sms, st);
     if (rc != FFN_OK || !p.chunk) return rc;

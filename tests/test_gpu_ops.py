@@ -346,7 +346,7 @@ def test_expert_mm_e4m3(ops, case, out):
 
 def test_expert_mm_ignores_other_rows(ops):
     """NaN and infinity in the rows of one expert, or of none, reach no other expert's results."""
-    for counts, k, m in (([70, 3, 61, 20], 64, 96), ([5, 2, 9, 3], 256, 64)):
+    for counts, k, m in (([70, 3, 61, 20], 64, 96), ([5, 2, 9, 3], 256, 64), ([1030, 900, 1201, 1100], 520, 576)):
         off = lens_to_offsets(counts)
         n = off[-1] + 9
         offsets = torch.tensor(off, dtype=torch.int32, device="cuda")
