@@ -678,17 +678,22 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
     }
 }
 
-// Rows of `cols` elements copied to rows of `ld` elements (zeros after the columns): operands whose rows
-// are no multiples of 16 bytes, which TMA cannot read.
+// Operands whose rows are no multiples of 16 bytes, which TMA cannot read, copied to rows that are (zeros
+// after the columns): all of a call's in one launch, an operand per blockIdx.y, 32 columns x 8 rows a block.
+struct PadJob {
+    const void* src; void* dst;
+    int64_t src_ld, rows;
+    int cols, ld;
+};
+struct PadJobs { PadJob j[3]; };
+
 template <typename T>
-__global__ void __launch_bounds__(256) pad_rows_kernel(const T* __restrict__ src, int64_t src_ld, T* __restrict__ dst,
-                                                       int64_t rows, int cols, int ld) {
-    const int64_t count = rows * ld;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < count; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t r = i / ld;
-        const int c = (int)(i - r * ld);
-        dst[i] = c < cols ? src[r * src_ld + c] : T(0);
-    }
+__global__ void __launch_bounds__(256) pad_rows_kernel(const PadJobs jobs) {
+    const PadJob p = jobs.j[blockIdx.y];
+    const T* src = static_cast<const T*>(p.src);
+    T* dst = static_cast<T*>(p.dst);
+    for (int64_t r = (int64_t)blockIdx.x * 8 + threadIdx.y; r < p.rows; r += (int64_t)gridDim.x * 8)
+        for (int c = threadIdx.x; c < p.ld; c += 32) dst[r * p.ld + c] = c < p.cols ? src[r * p.src_ld + c] : T(0);
 }
 
 using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -736,20 +741,32 @@ int padded(int cols, int dtype) {
 uint64_t pad_bytes(const void* p, int64_t ld, int64_t rows, int cols, int dtype) {
     return readable(p, ld, dtype) ? 0 : ((uint64_t)rows * padded(cols, dtype) * type_size(dtype) + 255) / 256 * 256;
 }
-Operand pad(const void* p, int64_t ld, int64_t rows, int cols, int dtype, unsigned char*& ws, int sms, cudaStream_t st) {
-    if (readable(p, ld, dtype)) return {p, ld};
-    const int to = padded(cols, dtype);
-    const int64_t count = rows * to;
-    const int blocks = (int)((count + 255) / 256 < (int64_t)sms * 16 ? (count + 255) / 256 : (int64_t)sms * 16);
-    if (dtype == FFN_E4M3)
-        pad_rows_kernel<uint8_t><<<blocks, 256, 0, st>>>(static_cast<const uint8_t*>(p), ld, ws, rows, cols, to);
-    else
-        pad_rows_kernel<uint16_t><<<blocks, 256, 0, st>>>(static_cast<const uint16_t*>(p), ld,
-                                                          reinterpret_cast<uint16_t*>(ws), rows, cols, to);
-    const Operand o{ws, to};
-    ws += pad_bytes(p, ld, rows, cols, dtype);
-    return o;
-}
+
+// Collects the operands of a call that have to be copied and copies them together.
+struct Padding {
+    PadJobs jobs{};
+    int count = 0;
+    unsigned char* ws;
+    int dtype;
+    Operand take(const void* p, int64_t ld, int64_t rows, int cols) {
+        if (readable(p, ld, dtype)) return {p, ld};
+        const int to = padded(cols, dtype);
+        const Operand o{ws, to};
+        jobs.j[count++] = PadJob{p, ws, ld, rows, cols, to};
+        ws += pad_bytes(p, ld, rows, cols, dtype);
+        return o;
+    }
+    int run(int sms, cudaStream_t st) {
+        if (!count) return FFN_OK;
+        int64_t rows = 0;
+        for (int i = 0; i < count; ++i) rows = jobs.j[i].rows > rows ? jobs.j[i].rows : rows;
+        const int64_t blocks = (rows + 7) / 8, most = (int64_t)sms * 8;
+        const dim3 grid((unsigned)(blocks < most ? blocks : most), (unsigned)count), block(32, 8);
+        if (dtype == FFN_E4M3) pad_rows_kernel<uint8_t><<<grid, block, 0, st>>>(jobs);
+        else pad_rows_kernel<uint16_t><<<grid, block, 0, st>>>(jobs);
+        return op_launched("ffn_expert_mm rows");
+    }
+};
 
 // The most units that n rows make.
 int64_t units_most(int64_t n, int experts, int chunk) { return chunk ? n / (64 * (int64_t)chunk) + experts : experts; }
@@ -1001,8 +1018,11 @@ int ffn_expert_mm(const void* x, int64_t x_ld, const void* w, const int32_t* off
     const int sms = op_sms();
     if (sms <= 0) return op_fail(FFN_E_CUDA, "no CUDA device");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    unsigned char* ws = static_cast<unsigned char*>(workspace);
-    const Operand a = pad(x, x_ld, n, k, dtype, ws, sms, st), b = pad(w, k, (int64_t)experts * m, k, dtype, ws, sms, st);
+    Padding pads;
+    pads.ws = static_cast<unsigned char*>(workspace);
+    pads.dtype = dtype;
+    const Operand a = pads.take(x, x_ld, n, k), b = pads.take(w, k, (int64_t)experts * m, k);
+    if (int rc = pads.run(sms, st)) return rc;
     const int mode = n <= (int64_t)experts * 48 ? FEW_ROWS : FORWARD;
     return rows_product(mode, a, b, x_scale, w_scale, offsets, y, n, experts, k, m, dtype, out_dtype, sms, st);
 }
@@ -1036,17 +1056,17 @@ int ffn_expert_mm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld
                                        "not 16-byte aligned");
     const int sms = op_sms();
     if (sms <= 0) return op_fail(FFN_E_CUDA, "no CUDA device");
-    unsigned char* ws = static_cast<unsigned char*>(workspace);
-    const Operand a = pad(dy, dy_ld, n, m, dtype, ws, sms, st);
-    if (dx) {
-        const Operand b = pad(w, k, (int64_t)experts * m, k, dtype, ws, sms, st);
-        if (int rc = rows_product(INPUT_GRAD, a, b, nullptr, nullptr, offsets, dx, n, experts, m, k, dtype, dtype, sms, st))
+    Padding pads;
+    pads.ws = static_cast<unsigned char*>(workspace);
+    pads.dtype = dtype;
+    const Operand a = pads.take(dy, dy_ld, n, m);
+    const Operand bw = dx ? pads.take(w, k, (int64_t)experts * m, k) : Operand{}, bx = dw ? pads.take(x, x_ld, n, k) : Operand{};
+    if (int rc = pads.run(sms, st)) return rc;
+    if (dx)
+        if (int rc = rows_product(INPUT_GRAD, a, bw, nullptr, nullptr, offsets, dx, n, experts, m, k, dtype, dtype, sms, st))
             return rc;
-    }
-    if (dw) {
-        const Operand b = pad(x, x_ld, n, k, dtype, ws, sms, st);
-        if (int rc = weight_product(a, b, offsets, dw, n, experts, k, m, dtype, dw_dtype, ws, sms, st)) return rc;
-    }
+    if (dw)
+        if (int rc = weight_product(a, bx, offsets, dw, n, experts, k, m, dtype, dw_dtype, pads.ws, sms, st)) return rc;
     return FFN_OK;
 }
 

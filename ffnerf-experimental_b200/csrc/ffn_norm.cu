@@ -401,7 +401,7 @@ Shape norm_shape(int d, int full_vec, bool aligned, int group) {
     Shape s{};
     s.vec = aligned ? full_vec : 1;
     const int vectors = (d + s.vec - 1) / s.vec;
-    const int most = s.vec == 1 ? 8 : 4;                 // vectors (or elements) of a thread
+    const int most = s.vec == 1 ? 16 : 4;                // vectors (or elements) of a thread
     s.threads = 256;
     if (vectors <= 32 * most) {
         // two vectors a thread halve what a row costs besides its elements (2^20 rows of 64 to e4m3: 70 us
@@ -418,7 +418,7 @@ Shape norm_shape(int d, int full_vec, bool aligned, int group) {
     } else {
         s.loop = true;
     }
-    if (s.vec == 1) s.nv = 8;
+    if (s.vec == 1) s.nv = 16;
     else if (s.nv == 3) s.nv = 4;
     if (s.vec == 1 && group) s.loop = true;
     return s;
@@ -444,8 +444,8 @@ int norm_launch(const NormArgs& a0, bool aligned, cudaStream_t st) {
     const int grid = norm_grid(s, a.n, sms, at_once);
     if (s.loop) rmsnorm_long_kernel<T, OUT8><<<grid, 256, 0, st>>>(a);
     else if (s.vec == 1) {
-        if (s.block) rmsnorm_kernel<T, OUT8, 1, 8, 1, true><<<grid, s.threads, 0, st>>>(a);
-        else rmsnorm_kernel<T, OUT8, 1, 8, 1, false><<<grid, s.threads, 0, st>>>(a);
+        if (s.block) rmsnorm_kernel<T, OUT8, 1, 16, 1, true><<<grid, s.threads, 0, st>>>(a);
+        else rmsnorm_kernel<T, OUT8, 1, 16, 1, false><<<grid, s.threads, 0, st>>>(a);
     } else if (s.block) {
         if (s.nv == 1) rmsnorm_kernel<T, OUT8, VEC, 1, 1, true><<<grid, s.threads, 0, st>>>(a);
         else if (s.nv == 2) rmsnorm_kernel<T, OUT8, VEC, 2, 1, true><<<grid, s.threads, 0, st>>>(a);
@@ -478,8 +478,8 @@ int norm_bwd_launch(const NormBwdArgs& a0, float* dgamma, bool aligned, cudaStre
     const size_t sm = (size_t)(s.threads / 32) * a.d * sizeof(float);   // at most 8 x 1024 floats
     if (s.loop) rmsnorm_bwd_long_kernel<T><<<grid, 256, 0, st>>>(a);
     else if (s.vec == 1) {
-        if (s.block) rmsnorm_bwd_kernel<T, 1, 8, true><<<grid, s.threads, 0, st>>>(a);
-        else rmsnorm_bwd_kernel<T, 1, 8, false><<<grid, s.threads, sm, st>>>(a);
+        if (s.block) rmsnorm_bwd_kernel<T, 1, 16, true><<<grid, s.threads, 0, st>>>(a);
+        else rmsnorm_bwd_kernel<T, 1, 16, false><<<grid, s.threads, sm, st>>>(a);
     } else if (s.block) {
         if (s.nv == 1) rmsnorm_bwd_kernel<T, VEC, 1, true><<<grid, s.threads, 0, st>>>(a);
         else if (s.nv == 2) rmsnorm_bwd_kernel<T, VEC, 2, true><<<grid, s.threads, 0, st>>>(a);
