@@ -376,6 +376,153 @@ __global__ void __launch_bounds__(256) rmsnorm_bwd_long_kernel(const NormBwdArgs
     }
 }
 
+// Rows of a width that is no multiple of a vector: a row then begins anywhere in its 16 bytes, and
+// element accesses reach a sixth of the copy rate (20,000 x 1001 forward and backward in bf16: 287 us, now
+// 127; forward alone 42 us = 0.59 of the rate, bound by the element accesses to shared memory).  But
+// R = 16 / sizeof(T) rows of a contiguous matrix begin and end on 16 bytes.  A block moves R rows between
+// memory and shared memory in vectors; there a warp takes a row for its sums, and a thread a column for
+// the results, with the weight read once for the R rows.
+template <typename T> constexpr int CHUNK_ROWS = 16 / (int)sizeof(T);
+
+// Copies `count` elements between memory and shared memory, both 16-byte aligned: into shared memory
+// without waiting (chunk_wait), so that all of a chunk's loads fly together.
+template <typename T>
+__device__ __forceinline__ void chunk_in(T* dst, const T* src, int count) {
+    constexpr int V = 16 / (int)sizeof(T);
+    const int whole = count / V;
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst);
+    for (int i = threadIdx.x; i < whole; i += blockDim.x)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(to + 16 * i), "l"(src + V * i) : "memory");
+    for (int i = whole * V + threadIdx.x; i < count; i += blockDim.x) dst[i] = src[i];
+}
+__device__ __forceinline__ void chunk_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+template <typename T>
+__device__ __forceinline__ void chunk_out(T* dst, const T* src, int count) {
+    constexpr int V = 16 / (int)sizeof(T);
+    const int whole = count / V;
+    for (int i = threadIdx.x; i < whole; i += blockDim.x)
+        reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
+    for (int i = whole * V + threadIdx.x; i < count; i += blockDim.x) dst[i] = src[i];
+}
+
+template <typename T, bool OUT8>
+__global__ void __launch_bounds__(32 * CHUNK_ROWS<T>) rmsnorm_chunk_kernel(const NormArgs a) {
+    constexpr int R = CHUNK_ROWS<T>;
+    extern __shared__ __align__(16) unsigned char chunk[];
+    __shared__ float factor[R], inverse[R];
+    T* sx = reinterpret_cast<T*>(chunk);
+    T* sr = sx + R * a.d;                                         // the residual, then y
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const float inv_d = 1.0f / (float)a.d;
+    for (int64_t r0 = (int64_t)blockIdx.x * R; r0 < a.n; r0 += (int64_t)gridDim.x * R) {
+        const int rows = (int)min(a.n - r0, (int64_t)R), count = rows * a.d;
+        chunk_in(sx, static_cast<const T*>(a.x) + r0 * a.d, count);
+        if (a.res) chunk_in(sr, static_cast<const T*>(a.res) + r0 * a.d, count);
+        chunk_wait();
+        __syncthreads();
+        if (w < rows) {
+            const T* x = sx + w * a.d;
+            const T* r = sr + w * a.d;
+            float ss = 0.0f, top = 0.0f;
+            for (int c = lane; c < a.d; c += 32) {
+                const float v = to_f(x[c]) + (a.res ? to_f(r[c]) : 0.0f);
+                ss = fmaf(v, v, ss);
+                if constexpr (OUT8) top = max_abs(top, v * __ldg(a.gamma + c));
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                if constexpr (OUT8) top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, o));
+            }
+            if (lane == 0) {
+                const float s = rsqrtf(fmaf(ss, inv_d, a.eps));
+                if (a.rstd) a.rstd[r0 + w] = s;
+                factor[w] = s;
+                if constexpr (OUT8) {
+                    const float sc = e4m3_scale(fabsf(top) * s);
+                    a.scale[r0 + w] = sc;
+                    inverse[w] = s * e4m3_inverse(sc);
+                }
+            }
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
+            const float g = __ldg(a.gamma + c);
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                if (i >= rows) break;
+                const float v = to_f(sx[i * a.d + c]) + (a.res ? to_f(sr[i * a.d + c]) : 0.0f);
+                if (a.h) sx[i * a.d + c] = from_f<T>(v);
+                if constexpr (OUT8)
+                    static_cast<uint8_t*>(a.y)[(r0 + i) * a.d + c] =
+                        (uint8_t)__nv_cvt_float_to_fp8(v * g * inverse[i], __NV_SATFINITE, __NV_E4M3);
+                else sr[i * a.d + c] = from_f<T>(v * (factor[i] * g));
+            }
+        }
+        __syncthreads();
+        if (a.h) chunk_out(static_cast<T*>(a.h) + r0 * a.d, sx, count);
+        if constexpr (!OUT8) chunk_out(static_cast<T*>(a.y) + r0 * a.d, sr, count);
+        __syncthreads();
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(32 * CHUNK_ROWS<T>) rmsnorm_bwd_chunk_kernel(const NormBwdArgs a) {
+    constexpr int R = CHUNK_ROWS<T>;
+    extern __shared__ __align__(16) unsigned char chunk[];
+    __shared__ float factor[R], mean[R];
+    T* sd = reinterpret_cast<T*>(chunk);                          // dy, then dx
+    T* sx = sd + R * a.d;
+    T* sr = sx + R * a.d;
+    T* sq = sr + (a.res ? R * a.d : 0);
+    float* sum = reinterpret_cast<float*>(sq + (a.dres ? R * a.d : 0));   // of dy xhat, a column each
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const float inv_d = 1.0f / (float)a.d;
+    for (int c = threadIdx.x; c < a.d; c += blockDim.x) sum[c] = 0.0f;
+    for (int64_t r0 = (int64_t)blockIdx.x * R; r0 < a.n; r0 += (int64_t)gridDim.x * R) {
+        const int rows = (int)min(a.n - r0, (int64_t)R), count = rows * a.d;
+        chunk_in(sd, static_cast<const T*>(a.dy) + r0 * a.d, count);
+        chunk_in(sx, static_cast<const T*>(a.x) + r0 * a.d, count);
+        if (a.res) chunk_in(sr, static_cast<const T*>(a.res) + r0 * a.d, count);
+        if (a.dres) chunk_in(sq, static_cast<const T*>(a.dres) + r0 * a.d, count);
+        chunk_wait();
+        __syncthreads();
+        if (w < rows) {
+            float dot = 0.0f;
+            for (int c = lane; c < a.d; c += 32) {
+                const int i = w * a.d + c;
+                dot = fmaf(to_f(sd[i]) * __ldg(a.gamma + c), to_f(sx[i]) + (a.res ? to_f(sr[i]) : 0.0f), dot);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+            if (lane == 0) {
+                const float s = __ldg(a.rstd + r0 + w);
+                factor[w] = s;
+                mean[w] = dot * s * inv_d;
+            }
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
+            const float g = __ldg(a.gamma + c);
+            float add = 0.0f;
+#pragma unroll
+            for (int q = 0; q < R; ++q) {
+                if (q >= rows) break;
+                const int i = q * a.d + c;
+                const float s = factor[q], dy = to_f(sd[i]), xh = (to_f(sx[i]) + (a.res ? to_f(sr[i]) : 0.0f)) * s;
+                add = fmaf(dy, xh, add);
+                sd[i] = from_f<T>(fmaf(s, fmaf(-xh, mean[q], dy * g), a.dres ? to_f(sq[i]) : 0.0f));
+            }
+            sum[c] += add;
+        }
+        __syncthreads();
+        chunk_out(static_cast<T*>(a.dx) + r0 * a.d, sd, count);
+        __syncthreads();
+    }
+    float* out = a.partial + (int64_t)blockIdx.x * a.d;
+    for (int c = threadIdx.x; c < a.d; c += blockDim.x) out[c] = sum[c];
+}
+
 // dgamma[c] = sum over blocks of partial[block][c]: 32 columns x 32 slices of the blocks per block,
 // each slice summed in order, then the slices in order.
 __global__ void __launch_bounds__(1024) norm_dgamma_kernel(const float* __restrict__ partial, float* __restrict__ dgamma,
@@ -431,13 +578,46 @@ int norm_grid(const Shape& s, int64_t n, int sms, int at_once) {
     return (int)(want < most ? want : most);
 }
 
+// Whether rows go through shared memory in chunks: whole matrices of unaligned rows, one scale a row at
+// most, enough of them for a block of rows on every SM, and three blocks an SM at least (5000 x 4411
+// forward and backward, one block an SM: 318 us, with element accesses 232).
+constexpr size_t CHUNK_MOST = 225 * 1024;
+template <typename T>
+bool chunked(int64_t n, int d, int sms, size_t bytes) {
+    return bytes <= CHUNK_MOST / 3 && n >= (int64_t)sms * CHUNK_ROWS<T>;
+}
+template <typename T>
+int chunk_grid(int64_t n, int sms, size_t bytes) {
+    const int64_t blocks = (n + CHUNK_ROWS<T> - 1) / CHUNK_ROWS<T>;
+    int64_t resident = (int64_t)(CHUNK_MOST / bytes);
+    if (resident > 8) resident = 8;
+    return (int)(blocks < sms * resident ? blocks : sms * resident);
+}
+// The limit of dynamic shared memory of a kernel, set once a device.
+int chunk_ready(const void* kernel, std::atomic<uint64_t>& ready) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev <= 63 && (ready.load(std::memory_order_acquire) >> dev & 1)) return FFN_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)CHUNK_MOST);
+    if (e != cudaSuccess) return op_fail(FFN_E_CUDA, std::string("ffn_rmsnorm: ") + cudaGetErrorString(e));
+    if (dev <= 63) ready.fetch_or(1ull << dev, std::memory_order_release);
+    return FFN_OK;
+}
+
 template <typename T, bool OUT8>
-int norm_launch(const NormArgs& a0, bool aligned, cudaStream_t st) {
+int norm_launch(const NormArgs& a0, bool aligned, bool whole, cudaStream_t st) {
     NormArgs a = a0;
     constexpr int VEC = 16 / sizeof(T);
     const Shape s = norm_shape(a.d, VEC, aligned, a.group);
     const int sms = op_sms();
     if (sms <= 0) return op_fail(FFN_E_CUDA, "no CUDA device");
+    const size_t bytes = (size_t)2 * 16 * a.d;
+    if (s.vec == 1 && whole && !a.group && chunked<T>(a.n, a.d, sms, bytes)) {
+        static std::atomic<uint64_t> ready{0};
+        if (int rc = chunk_ready(reinterpret_cast<const void*>(rmsnorm_chunk_kernel<T, OUT8>), ready)) return rc;
+        rmsnorm_chunk_kernel<T, OUT8><<<chunk_grid<T>(a.n, sms, bytes), 32 * CHUNK_ROWS<T>, bytes, st>>>(a);
+        return op_launched("ffn_rmsnorm");
+    }
     a.tpr = s.tpr;
     // rows at a time: only where there are enough of them to keep every SM's blocks
     const int at_once = !s.block && !s.loop && s.vec > 1 && a.n * s.tpr >= (int64_t)sms * 2048 * 4 / s.nv ? 4 / s.nv : 1;
@@ -462,10 +642,10 @@ int norm_launch(const NormArgs& a0, bool aligned, cudaStream_t st) {
 
 constexpr int MOST_D = 1 << 30;        // columns are counted in 32 bits, in steps of a block
 
-constexpr int BWD_BLOCKS_PER_SM = 4;   // at most; as many as are resident: their rows of partial sums are read again
+constexpr int BWD_BLOCKS_PER_SM = 8;   // at most; as many as are resident: their rows of partial sums are read again
 
 template <typename T>
-int norm_bwd_launch(const NormBwdArgs& a0, float* dgamma, bool aligned, cudaStream_t st) {
+int norm_bwd_launch(const NormBwdArgs& a0, float* dgamma, bool aligned, bool whole, cudaStream_t st) {
     NormBwdArgs a = a0;
     constexpr int VEC = 16 / sizeof(T);
     const Shape s = norm_shape(a.d, VEC, aligned, 0);
@@ -473,10 +653,16 @@ int norm_bwd_launch(const NormBwdArgs& a0, float* dgamma, bool aligned, cudaStre
     if (sms <= 0) return op_fail(FFN_E_CUDA, "no CUDA device");
     a.tpr = s.tpr;
     int grid = norm_grid(s, a.n, sms, 1);
-    const int most = sms * (s.nv >= 4 ? 2 : BWD_BLOCKS_PER_SM);
+    const int most = sms * (s.nv >= 4 ? 2 : 4);
     grid = grid < most ? grid : most;
     const size_t sm = (size_t)(s.threads / 32) * a.d * sizeof(float);   // at most 8 x 1024 floats
-    if (s.loop) rmsnorm_bwd_long_kernel<T><<<grid, 256, 0, st>>>(a);
+    const size_t bytes = (size_t)(2 + (a.res != nullptr) + (a.dres != nullptr)) * 16 * a.d + 4 * (size_t)a.d;
+    if (s.vec == 1 && whole && chunked<T>(a.n, a.d, sms, bytes)) {
+        static std::atomic<uint64_t> ready{0};
+        if (int rc = chunk_ready(reinterpret_cast<const void*>(rmsnorm_bwd_chunk_kernel<T>), ready)) return rc;
+        grid = chunk_grid<T>(a.n, sms, bytes);
+        rmsnorm_bwd_chunk_kernel<T><<<grid, 32 * CHUNK_ROWS<T>, bytes, st>>>(a);
+    } else if (s.loop) rmsnorm_bwd_long_kernel<T><<<grid, 256, 0, st>>>(a);
     else if (s.vec == 1) {
         if (s.block) rmsnorm_bwd_kernel<T, 1, 16, true><<<grid, s.threads, 0, st>>>(a);
         else rmsnorm_bwd_kernel<T, 1, 16, false><<<grid, s.threads, sm, st>>>(a);
@@ -519,11 +705,13 @@ int ffn_rmsnorm(const void* x, int64_t x_ld, const void* residual, int64_t resid
     const int vec = (int)(16 / z);
     const bool aligned = d % vec == 0 && x_ld % vec == 0 && (!residual || residual_ld % vec == 0) && op_aligned(x, 16) &&
                          op_aligned(residual, 16) && op_aligned(gamma, 16) && op_aligned(h, 16) && op_aligned(y, out8 ? vec : 16);
+    const bool whole = x_ld == d && (!residual || residual_ld == d) && op_aligned(x, 16) && op_aligned(residual, 16) &&
+                       op_aligned(h, 16) && op_aligned(y, out8 ? 1 : 16);
     NormArgs a{x, residual, gamma, h, y, scale, rstd, n, x_ld, residual_ld, d, group, 0, group == 32 ? 5 : group == 64 ? 6 : 7, eps};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == FFN_F32) return out8 ? norm_launch<float, true>(a, aligned, st) : norm_launch<float, false>(a, aligned, st);
-    if (dtype == FFN_F16) return out8 ? norm_launch<__half, true>(a, aligned, st) : norm_launch<__half, false>(a, aligned, st);
-    return out8 ? norm_launch<__nv_bfloat16, true>(a, aligned, st) : norm_launch<__nv_bfloat16, false>(a, aligned, st);
+    if (dtype == FFN_F32) return out8 ? norm_launch<float, true>(a, aligned, whole, st) : norm_launch<float, false>(a, aligned, whole, st);
+    if (dtype == FFN_F16) return out8 ? norm_launch<__half, true>(a, aligned, whole, st) : norm_launch<__half, false>(a, aligned, whole, st);
+    return out8 ? norm_launch<__nv_bfloat16, true>(a, aligned, whole, st) : norm_launch<__nv_bfloat16, false>(a, aligned, whole, st);
 }
 
 uint64_t ffn_rmsnorm_bwd_workspace(int64_t n, int32_t d) {
@@ -556,11 +744,14 @@ int ffn_rmsnorm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, 
     const bool aligned = d % vec == 0 && dy_ld % vec == 0 && x_ld % vec == 0 && (!residual || residual_ld % vec == 0) &&
                          (!dresidual || dresidual_ld % vec == 0) && op_aligned(dy, 16) && op_aligned(x, 16) &&
                          op_aligned(residual, 16) && op_aligned(dresidual, 16) && op_aligned(gamma, 16) && op_aligned(dx, 16);
+    const bool whole = dy_ld == d && x_ld == d && (!residual || residual_ld == d) && (!dresidual || dresidual_ld == d) &&
+                       op_aligned(dy, 16) && op_aligned(x, 16) && op_aligned(residual, 16) && op_aligned(dresidual, 16) &&
+                       op_aligned(dx, 16);
     NormBwdArgs a{dy, x, residual, dresidual, gamma, rstd, dx, static_cast<float*>(workspace), n,
                   dy_ld, x_ld, residual_ld, dresidual_ld, d, 0};
-    if (dtype == FFN_F32) return norm_bwd_launch<float>(a, dgamma, aligned, st);
-    if (dtype == FFN_F16) return norm_bwd_launch<__half>(a, dgamma, aligned, st);
-    return norm_bwd_launch<__nv_bfloat16>(a, dgamma, aligned, st);
+    if (dtype == FFN_F32) return norm_bwd_launch<float>(a, dgamma, aligned, whole, st);
+    if (dtype == FFN_F16) return norm_bwd_launch<__half>(a, dgamma, aligned, whole, st);
+    return norm_bwd_launch<__nv_bfloat16>(a, dgamma, aligned, whole, st);
 }
 
 }  // extern "C"

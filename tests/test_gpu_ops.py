@@ -31,7 +31,7 @@ def strided(t, extra):
 
 # ------------------------------------------------------------------------------------------- norm
 NORM_SIZES = [(1, 1), (1, 1024), (3, 8), (5, 64), (33, 100), (7, 1000), (2, 1001), (9, 2056), (300, 40), (4, 8200),
-              (3, 16384), (2, 20011), (1000, 72)]
+              (3, 16384), (2, 20011), (1000, 72), (1203, 77), (1500, 1001), (2500, 3)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -50,7 +50,7 @@ def test_rmsnorm(ops, n, d, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,d,group", [(1, 64, 0), (5, 1024, 0), (3, 1001, 0), (130, 64, 32), (9, 128, 128), (7, 4096, 64),
-                                       (6, 192, 64), (2, 20000, 0), (2, 32768, 128)])
+                                       (6, 192, 64), (2, 20000, 0), (2, 32768, 128), (1301, 85, 0)])
 def test_rmsnorm_e4m3(ops, n, d, group, dtype):
     x, r, g = draw(4, n, d, dtype=dtype, scale=2), draw(5, n, d, dtype=dtype), 1 + 0.3 * draw(6, d)
     y, h, rstd, scale = ops.rmsnorm(x, g, r, out="e4m3", group=group)
