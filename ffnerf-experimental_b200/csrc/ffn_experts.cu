@@ -186,7 +186,8 @@ struct Plan {
     static constexpr int A_BYTES = BM * KB;
     static constexpr int B_BYTES = BH * KB;
     static constexpr int STAGE = A_BYTES + B_BYTES;
-    static constexpr int EPI = MODE == FEW_ROWS ? 0 : EPI_WARPS * SLAB;
+    static constexpr int SLABS = BN == 256 ? 1 : 2;                           // of a result warp
+    static constexpr int EPI = MODE == FEW_ROWS ? 0 : EPI_WARPS * SLABS * SLAB;
     static constexpr int MISC = 2 * COUNTS + 256;                          // tile counts, rows' ends, barriers
     static constexpr int FIT = (int)((SMEM_MOST - EPI - MISC) / STAGE);
     static constexpr int STAGES = FIT > 12 ? 12 : FIT;
@@ -553,7 +554,8 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
         const int acc = warp >> 2, quarter = warp & 3;            // this group's accumulator, this warp's lanes
         uint32_t aph = 0;
         TO* out = static_cast<TO*>(p.out);
-        unsigned char* sl = slabs + warp * SLAB;
+        unsigned char* slab = slabs + warp * P::SLABS * SLAB;
+        [[maybe_unused]] int turn = 0;
         Walk<MODE, BN, EB, PAIR> walk;
         for (int t = first + acc * stride; t < total; t += 2 * stride) {
             const Tile k = walk.at(p, prefix, ends, t);
@@ -614,8 +616,10 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
                             for (int j = 0; j < 32; ++j) pk[j] = 0u;
                     }
                     // the slab's previous store has been read out of shared memory
-                    if (lane == 0) bulk_wait_read<0>();
+                    if (lane == 0) bulk_wait_read<P::SLABS - 1>();
                     __syncwarp();
+                    unsigned char* sl = slab + (P::SLABS > 1 ? turn * SLAB : 0);
+                    turn ^= 1;
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                         *reinterpret_cast<uint4*>(sl + lane * 128 + ((j ^ (lane & 7)) << 4)) =
@@ -626,7 +630,6 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
                         if (lane == 0) {
                             if constexpr (MODE == WEIGHT_GRAD) tma_store3(&mo, col, (int)row, k.plane, tc::smem_u32(sl));
                             else tma_store2(&mo, col, (int)row, tc::smem_u32(sl));
-                            bulk_commit();
                         }
                     } else {
                         __syncwarp();
@@ -640,15 +643,19 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
                                         *reinterpret_cast<const uint4*>(sl + r * 128 + ((j ^ (r & 7)) << 4));
                             }
                         } else {
+#pragma unroll 4
                             for (int r = 0; r < live; ++r)
-                                for (int j = lane; j < cols; j += 32) {
-                                    const int byte = j * (int)sizeof(TO);
-                                    o[(int64_t)r * p.cols + j] = *reinterpret_cast<const TO*>(
-                                        sl + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15));
+#pragma unroll
+                                for (int j0 = 0; j0 < W; j0 += 32) {
+                                    const int j = j0 + lane, byte = j * (int)sizeof(TO);
+                                    if (j < cols)
+                                        o[(int64_t)r * p.cols + j] = *reinterpret_cast<const TO*>(
+                                            sl + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15));
                                 }
                         }
                         __syncwarp();
                     }
+                    if (lane == 0) bulk_commit();                 // (an empty group where no store was issued)
                 }
             }
             tc::fence_before_sync();
@@ -693,7 +700,14 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const PadJobs jobs) {
     const T* src = static_cast<const T*>(p.src);
     T* dst = static_cast<T*>(p.dst);
     for (int64_t r = (int64_t)blockIdx.x * 8 + threadIdx.y; r < p.rows; r += (int64_t)gridDim.x * 8)
-        for (int c = threadIdx.x; c < p.ld; c += 32) dst[r * p.ld + c] = c < p.cols ? src[r * p.src_ld + c] : T(0);
+        for (int c0 = threadIdx.x; c0 < p.ld; c0 += 256) {
+            T v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = c0 + 32 * i < p.cols ? src[r * p.src_ld + c0 + 32 * i] : T(0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c0 + 32 * i < p.ld) dst[r * p.ld + c0 + 32 * i] = v[i];
+        }
 }
 
 using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -963,8 +977,9 @@ int weight_product(Operand dy, Operand x, const int32_t* offsets, void* dw, int6
     CUtensorMap ma, mb, mo{};
     if (p.tma_out && !make_map(&mo, out, out_type, k, m, k, units_most(n, experts, p.chunk), 32)) return bad_map();
     if (!make_map(&ma, dy.p, dtype, m, n, dy.ld, 0, 64) || !make_map(&mb, x.p, dtype, k, n, x.ld, 0, 64)) return bad_map();
-    const int bn = tile_width(k, WIDE, sms);
-    const int rc = weight_pair(n, experts, k, m, sms) ? launch_typed<WEIGHT_GRAD, 256, true>(p, ma, mb, mo, dtype, out_type, sms, st)
+    // cut along the rows a tile may be wide; whole, few tiles are made narrower
+    const int bn = tile_width(k, p.chunk ? WIDE : (int64_t)experts * ((m + BM - 1) / BM), sms);
+    const int rc = bn == 256 && weight_pair(n, experts, k, m, sms) ? launch_typed<WEIGHT_GRAD, 256, true>(p, ma, mb, mo, dtype, out_type, sms, st)
                  : bn == 256 ? launch_typed<WEIGHT_GRAD, 256>(p, ma, mb, mo, dtype, out_type, sms, st)
                  : bn == 128 ? launch_typed<WEIGHT_GRAD, 128>(p, ma, mb, mo, dtype, out_type, sms, st)
                              : launch_typed<WEIGHT_GRAD, 64>(p, ma, mb, mo, dtype, out_type, sms, st);
