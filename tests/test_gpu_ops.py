@@ -435,6 +435,34 @@ def test_streams(ops):
     assert torch.equal(h, h2) and torch.equal(last, last2)
 
 
+def test_matrices_of_more_than_2_31_elements(ops):
+    """Element offsets that pass 32 bits: the last rows are what a call on them alone gives."""
+    n, d = 1_100_000, 2048
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(n, d, generator=g, device="cuda", dtype=BF16)
+    gamma = torch.ones(d, device="cuda")
+    y, _, st, _ = ops.rmsnorm(x, gamma)
+    tail = x[-7:].clone()
+    torch.testing.assert_close(y[-7:], ops.rmsnorm(tail, gamma)[0], rtol=0, atol=0)
+    dx, _ = ops.rmsnorm_bwd(x, x, gamma, st)
+    torch.testing.assert_close(dx[-7:], ops.rmsnorm_bwd(tail, tail, gamma, st.rstd[-7:].clone())[0], rtol=0, atol=0)
+    del dx, st
+    h, last = ops.gated_scan(x.view(1100, 1000, d), y.view(1100, 1000, d))
+    h1, last1 = ops.gated_scan(x.view(1100, 1000, d)[-1:].clone(), y.view(1100, 1000, d)[-1:].clone())
+    torch.testing.assert_close(h[-1:], h1, rtol=2.0 ** -7, atol=1e-5)          # another split of time, one bf16 step
+    torch.testing.assert_close(last[-1:], last1, rtol=1e-4, atol=1e-5)
+    dg, dv, _ = ops.gated_scan_bwd(y.view(1100, 1000, d), x.view(1100, 1000, d), y.view(1100, 1000, d), h)
+    dg1, dv1, _ = ops.gated_scan_bwd(y[-1000:][None], x[-1000:][None], y[-1000:][None], h[-1:])
+    torch.testing.assert_close(dv[-1:], dv1, rtol=2.0 ** -7, atol=1e-5)
+    del h, dg, dv, y
+    w, off = draw(1, 2, 64, d, dtype=BF16), torch.tensor([0, 500_000, n], dtype=torch.int32, device="cuda")
+    z = ops.expert_mm(x, w, off)
+    short = torch.tensor([0, 0, 300], dtype=torch.int32, device="cuda")
+    torch.testing.assert_close(z[-300:], ops.expert_mm(x[-300:], w, short), rtol=0, atol=0)
+    back, _ = ops.expert_mm_bwd(z, x, w, off, need_dw=False)
+    torch.testing.assert_close(back[-300:], ops.expert_mm_bwd(z[-300:], x[-300:], w, short, need_dw=False)[0], rtol=0, atol=0)
+
+
 def test_calls_in_a_graph(ops):
     """Every operator can be captured: nothing synchronises or reads sizes back, and a replay on new inputs
     and other offsets gives what a call on them gives."""
