@@ -9,6 +9,7 @@
 #include <tuple>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
@@ -77,7 +78,10 @@ T* plain(const Maybe& t, const char* name, at::IntArrayRef shape, at::ScalarType
 }
 
 void* ptr(const Maybe& t) { return t ? t->data_ptr() : nullptr; }
-Tensor make(at::IntArrayRef shape, at::ScalarType type, const Tensor& like) { return at::empty(shape, like.options().dtype(type)); }
+// An output on like's device, from the caching allocator without the dispatcher's detour.
+Tensor make(at::IntArrayRef shape, at::ScalarType type, const Tensor& like) {
+    return Tensor(at::detail::empty_cuda(shape, type, like.device(), std::nullopt));
+}
 
 // The device and stream of a call, and its workspace.
 struct Call {
@@ -87,7 +91,7 @@ struct Call {
     explicit Call(const Tensor& t) : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream(t.device().index()).stream()) {}
     void* space(uint64_t bytes, const Tensor& like) {
         if (!bytes) return nullptr;
-        buffer = at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+        buffer = make({(int64_t)bytes}, at::kByte, like);
         return buffer.data_ptr();
     }
 };
