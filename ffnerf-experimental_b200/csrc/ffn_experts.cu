@@ -899,7 +899,7 @@ int rows_product(int mode, Operand a, Operand b, const float* a_scale, const flo
 }
 
 // Sums the units of each expert in order: dw[e] = sum of part[unit], fp32 to TO.
-template <typename TO>
+template <typename TO, int V>
 __global__ void __launch_bounds__(256) units_sum_kernel(const Args p, const float* __restrict__ part, TO* __restrict__ dw,
                                                         int64_t size) {
     __shared__ int first, units;
@@ -928,18 +928,53 @@ __global__ void __launch_bounds__(256) units_sum_kernel(const Args p, const floa
         if (threadIdx.x == 0) first = sum;
     }
     __syncthreads();
+    // a thread takes V neighbouring elements; four units' loads fly together, their sums stay in order
     const float* src = part + (int64_t)first * size;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.x * 256) {
-        float v = 0.0f;
-        for (int u = 0; u < units; ++u) v += src[(int64_t)u * size + i];
-        dw[(int64_t)e * size + i] = from_f<TO>(v);
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < size; i += (int64_t)gridDim.x * 256 * V) {
+        float v[V] = {};
+        for (int u0 = 0; u0 < units; u0 += 4) {
+            float t[4][V];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (u0 + u < units) {
+                    if constexpr (V == 4) {
+                        const float4 q = __ldg(reinterpret_cast<const float4*>(src + (int64_t)(u0 + u) * size + i));
+                        t[u][0] = q.x; t[u][1] = q.y; t[u][2] = q.z; t[u][3] = q.w;
+                    } else {
+                        t[u][0] = __ldg(src + (int64_t)(u0 + u) * size + i);
+                    }
+                }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (u0 + u < units)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) v[j] += t[u][j];
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) dw[(int64_t)e * size + i + j] = from_f<TO>(v[j]);
     }
+}
+
+template <typename TO>
+int units_sum(const Args& p, const float* part, TO* dw, int64_t size, int sms, cudaStream_t st) {
+    const int v = size % 4 ? 1 : 4;
+    int64_t bx = (size / v + 255) / 256;
+    const int64_t cap = (16 * (int64_t)sms + p.experts - 1) / p.experts;
+    const dim3 grid((unsigned)(bx < cap ? bx : cap), (unsigned)p.experts);
+    if (v == 4) units_sum_kernel<TO, 4><<<grid, 256, 0, st>>>(p, part, dw, size);
+    else units_sum_kernel<TO, 1><<<grid, 256, 0, st>>>(p, part, dw, size);
+    return op_launched("ffn_expert_mm_bwd sums");
 }
 
 constexpr int64_t WIDE = 1 << 20;     // dW: the depth is cut instead of the tiles
 
+// Pairs for dW: their tiles waste no rows, but the second block's clearing of the last stage costs a round
+// trip.  Pair / single in us: 16 experts of 1024 x 4096 with 512 rows each 83 / 73, 1024 120 / 120, 4096
+// 426 / 441; 22 of 1744 x 3216 with 1024 rows 248 / 252, 4096 829 / 1022; 32 of 2048 x 512 with 1024 rows
+// 101 / 98, 4096 244 / 257; 64 of 256 x 320 with 4096 rows 134 / 126.
+constexpr int PAIR_ROWS_DW = 1024, PAIR_SIZE_DW = 1 << 20;
 bool weight_pair(int64_t n, int experts, int k, int m, int sms) {
-    return tile_width(k, WIDE, sms) == 256 && m > BM && n >= (int64_t)experts * PAIR_ROWS;
+    return tile_width(k, WIDE, sms) == 256 && m > BM && n >= (int64_t)experts * PAIR_ROWS_DW && (int64_t)m * k >= PAIR_SIZE_DW;
 }
 
 // Stages of depth in a unit of dW, or 0.  Experts share the rows unevenly and a small W has few output
@@ -947,18 +982,20 @@ bool weight_pair(int64_t n, int experts, int k, int m, int sms) {
 // tiles an SM the depth is cut into units, whose fp32 sums go through the workspace: as many as make two
 // full rounds of the SMs (four where the experts alone come near two), of 16 stages at least.  More units
 // balance no better and write and read more sums: 200,000 rows, 8 experts of 256 x 512, took 89 us with
-// 600 tiles (158 MB of sums).
+// 600 tiles (158 MB of sums).  With short depths the sums cost more than the imbalance: from 64 stages an
+// expert on (8 experts of 512 x 512 with 1024 rows, 16 stages: 31 us cut, 15 whole), or 24 where the tiles
+// leave three SMs in four idle.
 int weight_chunk(int64_t n, int experts, int k, int m, int sms) {
     const int bn = tile_width(k, WIDE, sms);
     const int bm = weight_pair(n, experts, k, m, sms) ? 2 * BM : BM;
     if (bm > BM) sms /= 2;                                        // a tile takes two
     const int64_t per = (int64_t)((m + bm - 1) / bm) * ((k + bn - 1) / bn), blocks = n / 64 + experts;
     const int64_t least = per * experts;                          // every expert has a unit
-    if (least >= 2 * (int64_t)sms) return 0;
+    if (least >= 2 * (int64_t)sms || n < (int64_t)experts * 64 * (4 * least <= sms ? 24 : 64)) return 0;
     const int64_t room = (least > sms ? 4 : 2) * (int64_t)sms - least;
     int64_t c = (blocks * per + room - 1) / room;
     c = c > 16 ? c : 16;
-    return blocks <= c * experts ? 0 : (int)c;
+    return (int)c;
 }
 uint64_t weight_workspace(int64_t n, int experts, int k, int m, int sms) {
     const int chunk = sms > 0 ? weight_chunk(n, experts, k, m, sms) : 0;
@@ -985,15 +1022,10 @@ int weight_product(Operand dy, Operand x, const int32_t* offsets, void* dw, int6
                              : launch_typed<WEIGHT_GRAD, 64>(p, ma, mb, mo, dtype, out_type, sms, st);
     if (rc != FFN_OK || !p.chunk) return rc;
     const int64_t size = (int64_t)m * k;
-    int64_t bx = (size + 255) / 256;
-    const int64_t cap = (8 * (int64_t)sms + experts - 1) / experts;
-    if (bx > cap) bx = cap;
-    const dim3 grid((unsigned)bx, (unsigned)experts);
     const float* part = reinterpret_cast<const float*>(ws);
-    if (dw_dtype == FFN_F32) units_sum_kernel<float><<<grid, 256, 0, st>>>(p, part, static_cast<float*>(dw), size);
-    else if (dw_dtype == FFN_F16) units_sum_kernel<__half><<<grid, 256, 0, st>>>(p, part, static_cast<__half*>(dw), size);
-    else units_sum_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p, part, static_cast<__nv_bfloat16*>(dw), size);
-    return op_launched("ffn_expert_mm_bwd sums");
+    if (dw_dtype == FFN_F32) return units_sum<float>(p, part, static_cast<float*>(dw), size, sms, st);
+    if (dw_dtype == FFN_F16) return units_sum<__half>(p, part, static_cast<__half*>(dw), size, sms, st);
+    return units_sum<__nv_bfloat16>(p, part, static_cast<__nv_bfloat16*>(dw), size, sms, st);
 }
 
 int check(const char* who, int64_t n, int32_t experts, int32_t k, int32_t m) {

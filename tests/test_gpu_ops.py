@@ -294,6 +294,7 @@ EXPERT_CASES = [  # rows of each expert, rows of none, in, out
     ([17, 300, 64], 5, 200, 136), ([33] * 8, 0, 256, 512), ([700], 1, 1000, 264), ([9, 40, 0, 21], 7, 77, 131),
     ([2, 1, 0, 0, 4, 1, 0, 8], 0, 2048, 320), ([63, 65, 127, 129, 255], 1, 72, 40), ([1024, 512], 0, 128, 256),
     ([10], 0, 8, 8), ([3000, 17, 0, 2100], 3, 72, 56), ([5000], 0, 200, 130),
+    ([9001, 30, 4800], 3, 72, 56), ([5000], 2, 201, 130), ([4500, 4100], 0, 1040, 1032),
     ([700, 513, 901], 3, 192, 264),
     ([1100, 600, 1537], 5, 520, 576), ([1201, 0, 2090, 805], 3, 1040, 200)]
 
