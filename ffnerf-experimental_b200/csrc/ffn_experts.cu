@@ -983,15 +983,15 @@ bool weight_pair(int64_t n, int experts, int k, int m, int sms) {
 // full rounds of the SMs (four where the experts alone come near two), of 16 stages at least.  More units
 // balance no better and write and read more sums: 200,000 rows, 8 experts of 256 x 512, took 89 us with
 // 600 tiles (158 MB of sums).  With short depths the sums cost more than the imbalance: from 64 stages an
-// expert on (8 experts of 512 x 512 with 1024 rows, 16 stages: 31 us cut, 15 whole), or 24 where the tiles
-// leave three SMs in four idle.
+// expert on (8 experts of 512 x 512 with 1024 rows, 16 stages: 31 us cut, 15 whole; one of 256 x 256 with
+// 2048 rows 17 cut, 13 whole).
 int weight_chunk(int64_t n, int experts, int k, int m, int sms) {
     const int bn = tile_width(k, WIDE, sms);
     const int bm = weight_pair(n, experts, k, m, sms) ? 2 * BM : BM;
     if (bm > BM) sms /= 2;                                        // a tile takes two
     const int64_t per = (int64_t)((m + bm - 1) / bm) * ((k + bn - 1) / bn), blocks = n / 64 + experts;
     const int64_t least = per * experts;                          // every expert has a unit
-    if (least >= 2 * (int64_t)sms || n < (int64_t)experts * 64 * (4 * least <= sms ? 24 : 64)) return 0;
+    if (least >= 2 * (int64_t)sms || n < (int64_t)experts * 64 * 64) return 0;
     const int64_t room = (least > sms ? 4 : 2) * (int64_t)sms - least;
     int64_t c = (blocks * per + room - 1) / room;
     c = c > 16 ? c : 16;
