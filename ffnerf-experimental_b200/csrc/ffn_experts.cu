@@ -686,7 +686,8 @@ experts_kernel(const Args p, const __grid_constant__ CUtensorMap ma, const __gri
 }
 
 // Operands whose rows are no multiples of 16 bytes, which TMA cannot read, copied to rows that are (zeros
-// after the columns): all of a call's in one launch, an operand per blockIdx.y, 32 columns x 8 rows a block.
+// after the columns): all of a call's in one launch, an operand per blockIdx.y.  A warp moves 4 rows x 64
+// columns at a time, its eight loads in flight together.
 struct PadJob {
     const void* src; void* dst;
     int64_t src_ld, rows;
@@ -699,14 +700,19 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const PadJobs jobs) {
     const PadJob p = jobs.j[blockIdx.y];
     const T* src = static_cast<const T*>(p.src);
     T* dst = static_cast<T*>(p.dst);
-    for (int64_t r = (int64_t)blockIdx.x * 8 + threadIdx.y; r < p.rows; r += (int64_t)gridDim.x * 8)
-        for (int c0 = threadIdx.x; c0 < p.ld; c0 += 256) {
-            T v[8];
+    for (int64_t r0 = ((int64_t)blockIdx.x * 8 + threadIdx.y) * 4; r0 < p.rows; r0 += (int64_t)gridDim.x * 32)
+        for (int c0 = threadIdx.x; c0 < p.ld; c0 += 64) {
+            T v[4][2];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = c0 + 32 * i < p.cols ? src[r * p.src_ld + c0 + 32 * i] : T(0);
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (c0 + 32 * i < p.ld) dst[r * p.ld + c0 + 32 * i] = v[i];
+                for (int j = 0; j < 2; ++j)
+                    v[i][j] = r0 + i < p.rows && c0 + 32 * j < p.cols ? src[(r0 + i) * p.src_ld + c0 + 32 * j] : T(0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    if (r0 + i < p.rows && c0 + 32 * j < p.ld) dst[(r0 + i) * p.ld + c0 + 32 * j] = v[i][j];
         }
 }
 
@@ -774,7 +780,7 @@ struct Padding {
         if (!count) return FFN_OK;
         int64_t rows = 0;
         for (int i = 0; i < count; ++i) rows = jobs.j[i].rows > rows ? jobs.j[i].rows : rows;
-        const int64_t blocks = (rows + 7) / 8, most = (int64_t)sms * 8;
+        const int64_t blocks = (rows + 31) / 32, most = (int64_t)sms * 8;
         const dim3 grid((unsigned)(blocks < most ? blocks : most), (unsigned)count), block(32, 8);
         if (dtype == FFN_E4M3) pad_rows_kernel<uint8_t><<<grid, block, 0, st>>>(jobs);
         else pad_rows_kernel<uint16_t><<<grid, block, 0, st>>>(jobs);

@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(1024) scan_join_kernel(const ScanArgs a) {
 }
 
 template <typename T, bool SIG, bool BACK, int C, int U>
-__global__ void __launch_bounds__(THREADS, U == STEPS ? 4 : BACK && sizeof(T) * C > 4 ? 5 : 8) scan_kernel(const ScanArgs a) {
+__global__ void __launch_bounds__(THREADS, U == STEPS ? (C == 1 && sizeof(T) == 4 ? 6 : 4) : BACK && sizeof(T) * C > 4 ? 5 : 8) scan_kernel(const ScanArgs a) {
     const int64_t item = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (item >= a.items) return;
     const int part = blockIdx.y, seq = (int)(item / a.groups), ch = (int)(item % a.groups) * C;
