@@ -10,11 +10,16 @@
 //
 // Both passes read each element once and write each result once, a few operations per element: HBM
 // is the bound.  A row therefore stays in the registers of the threads that loaded it: `tpr` lanes of
-// a warp where the row has at most 32 lanes x NV vectors of 16 bytes (so a 64-wide row takes 8 lanes
-// and a warp takes four rows; no barrier), a whole block above that.  Statistics are fp32.  y is
+// a warp where the row has at most 32 lanes x NV vectors of 16 bytes (so a 64-wide row of 16-bit values
+// takes four lanes and a warp eight rows; no barrier), a whole block above that.  Statistics are fp32.  y is
 // formed from the unrounded fp32 sum x + r; the h that is written for the residual stream is rounded to
 // the stream's type.  The backward pass forms the same fp32 sum again: from the rounded h its dg, an fp32
 // sum over rows, would be off by the stream's rounding (1.7e-3 of it in bf16 against 2e-7).
+//
+// Measured on one B200, bf16 with a residual: 16384 x 4096 to e4m3 79 us (0.92 of the measured copy rate);
+// 49999 x 1000 forward 72 us (0.86), backward 108 us (0.72: the kernel, whose 128 registers leave 16 warps
+// an SM, and the launch that sums dg); 2^18 x 64 fp16 to e4m3 with a scale per 32 columns 17.5 us (0.46: 23
+// instructions an element, most of them for a group's scale and a row's factor that few elements share).
 #include "ffn_ops.cuh"
 
 namespace ffn {

@@ -22,12 +22,17 @@
 // the kernel needs is enough loads in flight.  Where sequences x channels give too few threads for
 // that, each sequence's time is cut into parts and there are three launches: one composes the map of
 // every part, walking it from its end to its beginning, a small one joins the maps into the states that
-// the parts begin with, and the last goes through each part.  That reads the gates and inputs a second time, in part from L2 (the
-// first launch ends where the last begins); in return every thread streams its own part and waits for
+// the parts begin with (few parts compose the maps before them themselves), and the last goes through
+// each part.  That reads the gates and inputs a second time, in part from L2 (the first launch ends where
+// the last begins); in return every thread streams its own part and waits for
 // nobody.  A one-read form was built and measured: blocks of a cluster that take turns along time and
 // exchange maps through distributed shared memory (with a cluster barrier, then with st.async and
 // mbarriers).  A turn's chain -- map, exchange, composition -- took 3 us of which memory was a quarter:
-// 433 us forward and backward at 2 sequences x 32768 steps x 1024 channels in bf16.
+// 433 us forward and backward at 2 sequences x 32768 steps x 1024 channels in bf16, in parts 310.
+//
+// Measured on one B200: 16384 sequences x 64 steps x 64 channels in fp16 forward 70, backward 140 us (0.89
+// of the measured copy rate); 512 x 128 x 1024 in bf16 68 and 139 us (0.92, 0.90); 2 x 32768 x 1024 123 and
+// 188 us (0.51, 0.66 of what reading once would take); 1500 x 0..1000 x 200 in fp32 forward 328 us (0.80).
 #include <initializer_list>
 #include <type_traits>
 
