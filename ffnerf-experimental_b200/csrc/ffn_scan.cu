@@ -257,6 +257,14 @@ __device__ __forceinline__ void load_floats(const float* p, float (&v)[C]) {
     for (int j = 0; j < C; ++j) v[j] = __uint_as_float(reinterpret_cast<const uint32_t*>(&r)[j]);
 }
 
+// Blocks that share an SM's registers: as many as the loads of a turn leave room for without spills.
+// Single channels wait for narrow loads, so more of them pay (fwd + bwd, bf16, against 4 blocks:
+// 2 x 20000 x 333 181 -> 152 us, 3000 x 64 x 129 147 -> 140; 400 x 700 x 101 lost, 249 -> 261).
+constexpr int blocks_an_sm(int u, int c, int size, bool back) {
+    if (u == STEPS) return c > 1 ? 4 : size == 4 ? 6 : back ? 5 : 7;
+    return back && size * c > 4 ? 5 : 8;
+}
+
 // A thread's steps: all of its sequence's, or one of `parts` equal parts of them (multiples of U).
 template <int U>
 __device__ __forceinline__ void part_of(const ScanArgs& a, const Span& s, int part, int64_t& lo, int64_t& hi) {
@@ -268,7 +276,7 @@ __device__ __forceinline__ void part_of(const ScanArgs& a, const Span& s, int pa
 // Composes the map of every part but each sequence's last, from the part's last step to its first:
 // with m the map of the steps after it, a step x -> a x + b makes it x -> (p a) x + (p b + h).
 template <typename T, bool SIG, bool BACK, int C, int U>
-__global__ void __launch_bounds__(THREADS, 4) scan_maps_kernel(const ScanArgs a) {
+__global__ void __launch_bounds__(THREADS, C == 1 ? 5 : 4) scan_maps_kernel(const ScanArgs a) {
     const int64_t item = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (item >= a.items) return;
     const int part = blockIdx.y, seq = (int)(item / a.groups), ch = (int)(item % a.groups) * C;
@@ -351,8 +359,9 @@ __global__ void __launch_bounds__(1024) scan_join_kernel(const ScanArgs a) {
     }
 }
 
+// Goes through each thread's steps and writes the results.
 template <typename T, bool SIG, bool BACK, int C, int U>
-__global__ void __launch_bounds__(THREADS, U == STEPS ? (C == 1 && sizeof(T) == 4 ? 6 : 4) : BACK && sizeof(T) * C > 4 ? 5 : 8) scan_kernel(const ScanArgs a) {
+__global__ void __launch_bounds__(THREADS, blocks_an_sm(U, C, (int)sizeof(T), BACK)) scan_kernel(const ScanArgs a) {
     const int64_t item = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (item >= a.items) return;
     const int part = blockIdx.y, seq = (int)(item / a.groups), ch = (int)(item % a.groups) * C;
