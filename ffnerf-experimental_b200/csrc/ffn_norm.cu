@@ -728,7 +728,8 @@ uint64_t ffn_rmsnorm_bwd_workspace(int64_t n, int32_t d) {
 }
 
 int ffn_rmsnorm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, const void* residual,
-                    int64_t residual_ld, const float* gamma, const float* rstd, const void* dresidual, int64_t dresidual_ld, void* dx, float* dgamma, void* workspace,
+                    int64_t residual_ld, const float* gamma, const float* rstd, const void* dresidual,
+                    int64_t dresidual_ld, void* dx, float* dgamma, void* workspace,
                     uint64_t workspace_bytes, int64_t n, int32_t d, int dtype, void* stream) {
     if (n < 0 || d < 1 || d > MOST_D) return op_fail(FFN_E_CONFIG, "ffn_rmsnorm_bwd: n must be >= 0 and 1 <= d <= 2^30");
     if (dtype != FFN_F32 && dtype != FFN_F16 && dtype != FFN_BF16)
