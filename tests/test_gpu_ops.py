@@ -245,6 +245,28 @@ def test_gated_scan_extreme_gates(ops):
     assert bool((h == 0).all()) and bool((last == 0).all())
 
 
+@pytest.mark.parametrize("at", [0, 1, 31, 32, 1999, 3999])
+def test_gated_scan_nan_gate_meets_zeros(ops, at):
+    """A linear gate of NaN leaves NaN in every later step (backward: in every earlier one's), zero states
+    and values included, with time cut into parts or not, and in its own channel and sequence only."""
+    for seqs in (2, 4000):
+        t = 4000 if seqs == 2 else 40
+        if at >= t:
+            continue
+        gate = torch.full((seqs, t, 8), 0.5, device="cuda")
+        gate[1, at, 3] = float("nan")
+        value = torch.zeros_like(gate)
+        bad = torch.zeros(seqs, t, 8, dtype=torch.bool, device="cuda")
+        bad[1, at:, 3] = True
+        h, last = ops.gated_scan(gate, value, form="linear")
+        assert torch.equal(torch.isnan(h), bad) and torch.equal(torch.isnan(last), bad[:, -1])
+        _, dv, dh0 = ops.gated_scan_bwd(value, gate, value, value, h0=last, form="linear")
+        back = torch.zeros_like(bad)                     # dv of a step takes the gates after it
+        back[1, :at, 3] = True
+        assert torch.equal(torch.isnan(dv), back)
+        assert bool(torch.isnan(dh0[1, 3])) and int(torch.isnan(dh0).sum()) == 1
+
+
 def test_gated_scan_rows_of_no_sequence(ops):
     gate, value = draw(1, 20, 6), draw(2, 20, 6)
     off = torch.tensor([3, 7, 7, 15], dtype=torch.int32, device="cuda")
