@@ -218,12 +218,14 @@ struct Step {
     }
 };
 
-// Rows that belong to no sequence (before the first, after the last) get zeros.
+// Rows that belong to no sequence (before the first, after the last) get zeros, from all threads of their channels
+// (131072 rows of which 65536 are used, 256 channels in bf16: forward 39 us, 35 without the others).
 template <typename T, bool BACK, int C>
-__device__ __forceinline__ void clear_outside(const ScanArgs& a, int seq, int ch) {
-    if (!a.offsets || (seq != 0 && seq != a.seqs - 1)) return;
+__device__ __forceinline__ void clear_outside(const ScanArgs& a, int seq, int part, int ch) {
+    if (!a.offsets) return;
     const int64_t lo = min(max((int64_t)__ldg(a.offsets), (int64_t)0), a.rows);
     const int64_t hi = min(max((int64_t)__ldg(a.offsets + a.seqs), lo), a.rows);
+    const int64_t mine = (int64_t)part * a.seqs + seq, all = (int64_t)a.parts * a.seqs;
     const Pack<T, C> z{};
     auto zero = [&](int64_t row) {
         if constexpr (!BACK) store_pack<T, C>(static_cast<T*>(a.h) + row * a.d + ch, z);
@@ -232,8 +234,8 @@ __device__ __forceinline__ void clear_outside(const ScanArgs& a, int seq, int ch
             store_pack<T, C>(static_cast<T*>(a.dvalue) + row * a.d + ch, z);
         }
     };
-    if (seq == 0) for (int64_t r = 0; r < lo; ++r) zero(r);
-    if (seq == a.seqs - 1) for (int64_t r = hi; r < a.rows; ++r) zero(r);
+    for (int64_t r = mine; r < lo; r += all) zero(r);
+    for (int64_t r = hi + mine; r < a.rows; r += all) zero(r);
 }
 
 template <bool BACK, int C>
@@ -258,11 +260,13 @@ __device__ __forceinline__ void load_floats(const float* p, float (&v)[C]) {
     for (int j = 0; j < C; ++j) v[j] = __uint_as_float(reinterpret_cast<const uint32_t*>(&r)[j]);
 }
 
-// Blocks that share an SM's registers: as many as the loads of a turn leave room for without spills.
-// Single channels wait for narrow loads, so more of them pay (fwd + bwd, bf16, against 4 blocks:
-// 2 x 20000 x 333 181 -> 152 us, 3000 x 64 x 129 147 -> 140; 400 x 700 x 101 lost, 249 -> 261).
+// Blocks that share an SM's registers: as many as the loads of a turn leave room for (at most 40 bytes of
+// a thread spill).  Single channels wait for narrow loads, so more of them pay:
+// fwd + bwd, against 4 blocks, 2 x 20000 x 333 bf16 181 -> 146 us, 3000 x 64 x 129 147 -> 132,
+// 400 x 700 x 101 249 -> 244; in fp32 4000 x 300 x 31 103 -> 84, and 20 x 5000 x 255
+// takes 313 us with a sixth block in the backward pass, 279 with five.
 constexpr int blocks_an_sm(int u, int c, int size, bool back) {
-    if (u == STEPS) return c > 1 ? 4 : size == 4 ? 6 : back ? 5 : 7;
+    if (u == STEPS) return c > 1 ? 4 : back ? 5 : size == 4 ? 6 : 7;
     return back && size * c > 4 ? 5 : 8;
 }
 
@@ -405,7 +409,7 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(U, C, (int)sizeof(T), BA
             }
     }
     if (part == a.parts - 1) put_state<C>(a, seq, ch, state);
-    if (part == 0) clear_outside<T, BACK, C>(a, seq, ch);
+    clear_outside<T, BACK, C>(a, seq, part, ch);
 }
 
 constexpr int SHORT = 4;             // the same for sequences of at most 8 steps: fewer registers, more threads

@@ -279,6 +279,25 @@ def test_gated_scan_rows_of_no_sequence(ops):
         assert all(bool((t[:3] == 0).all()) and bool((t[15:] == 0).all()) for t in (dg, dv))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("seqs,each,before,after,d", [(1, 700, 900, 1500, 8), (3, 5, 1, 3000, 7), (40, 9, 2001, 0, 20)])
+def test_gated_scan_many_rows_of_no_sequence(ops, seqs, each, before, after, d, dtype):
+    """Every row outside the sequences is written, on memory that held other values."""
+    used, rows = seqs * each, seqs * each + before + after
+    gate, value, dh = (draw(i, rows, d, dtype=dtype) for i in (1, 2, 3))
+    off = (before + each * torch.arange(seqs + 1, device="cuda")).to(torch.int32)
+    inside = slice(before, before + used)
+    for _ in range(2):
+        junk = [torch.full((rows, d), 7.0, dtype=dtype, device="cuda") for _ in range(3)]
+        del junk                                     # the outputs below take this memory
+        h, _ = ops.gated_scan(gate, value, offsets=off, max_len=each)
+        dg, dv, _ = ops.gated_scan_bwd(dh, gate, value, h, offsets=off, max_len=each)
+        tight, _ = ops.gated_scan(gate[inside], value[inside], offsets=off - before, max_len=each)
+        assert torch.equal(h[inside], tight)
+        for t in (h, dg, dv):
+            assert bool((t[:before] == 0).all()) and bool((t[before + used:] == 0).all())
+
+
 def test_gated_scan_gradient_against_differences(ops):
     b, t, d = 3, 40, 8
     gate, value, h0, dh, dl = draw(1, b, t, d), draw(2, b, t, d), draw(3, b, d), draw(4, b, t, d), draw(5, b, d)
